@@ -175,6 +175,7 @@ static inline float *state_of(const llb_spec *m, int il, int b) { return m->S[il
 static inline int *hist_of(const llb_spec *m, int b) { return m->hist ? m->hist + (size_t)b * (m->max_ctx + 16) : nullptr; }
 // the launchers' stream geometry and GEMM kernels while this engine enqueues (engines of different shapes may coexist)
 static std::recursive_mutex g_enqueue;
+std::recursive_mutex &llb_enqueue_lock(void) { return g_enqueue; }
 struct StreamScope {
   std::lock_guard<std::recursive_mutex> hold{g_enqueue};   // (a prompt enqueues kernels outside any graph, and another thread's engine may at the same time)
   Streams was;

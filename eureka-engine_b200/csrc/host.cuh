@@ -5,6 +5,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <mutex>
+
 #include "common.cuh"
 #include "gemm.cuh"
 
@@ -79,6 +81,12 @@ int gemm_launch_ffn(cudaStream_t s, GemmArgs &a1, int fmt2, GemmArgs &a2);   // 
 int gemm_launch_moe_gu(cudaStream_t s, int fmt, const XPlanes &xp, const MoeArgs &m);   // moe.cuh
 int gemm_moe_dn_ksplit(int fmt, const MoeArgs &m);
 int gemm_launch_moe_dn(cudaStream_t s, int fmt, const MoeArgs &m, int ks);
+
+// engine.cu: held while work is queued outside a graph, and while an engine captures one
+std::recursive_mutex &llb_enqueue_lock(void);
+
+// kv.cu
+int kv_setup(void);
 
 // api.cu: from the first to the last of a series of uploads, the staging buffer of those from host memory is kept
 void upload_hold(bool from_host);

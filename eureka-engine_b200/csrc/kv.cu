@@ -1,0 +1,536 @@
+// kv.cu -- the paged key-value cache's operators (llb_b200_kv_*): rows in, attention, eviction.
+#include <algorithm>
+#include <limits.h>
+#include <math.h>
+
+#include "../../include/llb_b200.h"
+#include "host.cuh"
+#include "kv.cuh"
+
+static unsigned int *g_kv_err = nullptr;   // what the kernels met (KV_ERR_*)
+
+// ---- rows in ------------------------------------------------------------------------------------
+// A warp a head of a row, eight of them a block, whose threads make the row's sines first.  Angles in 64 bits: at position
+// 200,000 a 32-bit product is 0.008 off; what is left of whole turns, taken off in 64 bits too, fits a float.  Bound by bytes.
+struct KvAppend {
+  const void *q, *k, *v;
+  long long qs, ks, vs;
+  int qhs;
+  const float *qn, *kn;
+  const double *invfreq;
+  const int *pos;
+  uint16_t *qo;
+  long long qos;
+  int H, rope;
+  float eps;
+  int wide;                    // q, k, v and q_out: a lane's elements lie on a multiple of their size
+};
+template <typename X, int E> __device__ __forceinline__ void kv_row_in(const X *p, bool wide, float (&x)[E]) {
+  if constexpr (sizeof(X) == 4) {
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) { const float2 f = __ldcg((const float2 *)(p + i)); x[i] = f.x; x[i + 1] = f.y; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i++) x[i] = __ldcg((const float *)p + i);
+    }
+  } else {
+    if (wide) {
+      uint32_t w[E / 2];
+      if constexpr (E == 2) w[0] = __ldcg((const uint32_t *)p);
+      else if constexpr (E == 4) { const uint2 t = __ldcg((const uint2 *)p); w[0] = t.x; w[1] = t.y; }
+      else { const uint4 t = __ldcg((const uint4 *)p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
+#pragma unroll
+      for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<X>::to2(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i++) x[i] = KvEl<X>::to(__ldcg((const uint16_t *)p + i));
+    }
+  }
+}
+template <typename T, int E> __device__ __forceinline__ void kv_row_out(uint16_t *p, bool wide, const float (&x)[E]) {
+  if (wide) {
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) w[i] = KvEl<T>::of2(x[2 * i], x[2 * i + 1]);
+    if constexpr (E == 2) *(uint32_t *)p = w[0];
+    else if constexpr (E == 4) *(uint2 *)p = make_uint2(w[0], w[1]);
+    else *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++) p[i] = KvEl<T>::of(x[i]);
+  }
+}
+__device__ __forceinline__ float kv_warp_sum(float v) {
+#pragma unroll
+  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+template <typename T, typename X, int HD>
+__global__ void __launch_bounds__(256) k_kv_append(const KvDev c, const KvRows rw, const KvAppend a) {
+  constexpr int E = HD / 32;
+  __shared__ float2 turn[HD / 2];
+  __shared__ float ys[8][HD];
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope >> 1;
+  const int b = kv_find(rw, c.seqs, r, lane);
+  if (!blockIdx.x && !blockIdx.y) kv_check_rows(c, rw);
+  if (b < 0) return;           // behind the last row, or row_start is not what it should be
+  const int i = r - __ldcg(rw.start + b), slot = kv_len(c, b) - (__ldcg(rw.start + b + 1) - __ldcg(rw.start + b)) + i;
+  const int pos = a.pos ? __ldcg(a.pos + b) + i : slot;
+  for (int p = threadIdx.x; p < half; p += blockDim.x) {
+    const double th = (double)pos * __ldg(a.invfreq + p), t = th - 6.283185307179586476925 * rint(th * 0.15915494309189533577);
+    float s, co;
+    sincosf((float)t, &s, &co);
+    turn[p] = make_float2(co, s);
+  }
+  __syncthreads();
+  const int u = blockIdx.y * 8 + warp;         // query heads, then kv heads of keys, then of values
+  if (u >= a.H + 2 * c.KV) return;
+  const bool isq = u < a.H, isv = u >= a.H + c.KV;
+  const int g = isq ? u : isv ? u - a.H - c.KV : u - a.H;
+  if (isq && !a.q) return;
+  const X *src = isq ? (const X *)a.q + r * a.qs + (long long)g * a.qhs : isv ? (const X *)a.v + r * a.vs + (long long)g * HD : (const X *)a.k + r * a.ks + (long long)g * HD;
+  float x[E];
+  kv_row_in<X, E>(src + lane * E, a.wide, x);
+  if (!isv) {
+    const float *w = isq ? a.qn : a.kn;
+    if (w) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < E; j++) ss += x[j] * x[j];
+      const float sc = 1.0f / sqrtf(kv_warp_sum(ss) / (float)HD + a.eps);
+#pragma unroll
+      for (int j = 0; j < E; j++) x[j] = x[j] * sc * __ldg(w + lane * E + j);
+    }
+    if (half) {
+#pragma unroll
+      for (int j = 0; j < E; j++) ys[warp][lane * E + j] = x[j];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < E; j++) {
+        const int d = lane * E + j;
+        if (d < half) x[j] = x[j] * turn[d].x - ys[warp][d + half] * turn[d].y;
+        else if (d < a.rope) x[j] = ys[warp][d - half] * turn[d - half].y + x[j] * turn[d - half].x;
+      }
+    }
+  }
+  if (isq) { kv_row_out<T, E>(a.qo + r * a.qos + (long long)g * HD + lane * E, a.wide, x); return; }
+  if (slot < 0) return;
+  const int id = kv_page(c, b, slot >> c.page_sh);
+  if (id < 0) return;
+  kv_row_out<T, E>((isv ? c.v : c.k) + kv_at(c, id, g, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD + lane * E, true, x);
+}
+
+// ---- attention, a warp a head of a row --------------------------------------------------------------
+struct KvAttn {
+  const uint16_t *q;
+  void *out;
+  long long qs, os;            // elements between rows
+  int H, window, sinks, out32;
+  float scale2;                // times log2(e): probabilities are powers of two
+  const float *w_in;
+  float *w_out;
+  int wstride;
+  float *lse;                  // [rows][H], base 2; where w_out is wanted
+};
+// one row and head over the slots that it sees, a slot at a time; lane's dimensions E lane ..
+template <typename T, int HD>
+__device__ __forceinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float (&o)[HD / 32], float &m, float &l) {
+  constexpr int E = HD / 32;
+  const int g = h / (a.H / c.KV), pm = (1 << c.page_sh) - 1;
+  float q[E];
+  kv_row_in<T, E>((const T *)a.q + r * a.qs + (long long)h * HD + lane * E, true, q);
+#pragma unroll
+  for (int i = 0; i < E; i++) { q[i] *= a.scale2; o[i] = 0.0f; }
+  m = -INFINITY; l = 0.0f;
+  const int lo = kv_first(e, a.window), ns = min(a.sinks, lo);
+  int id = -1, at = -1;
+  for (int n = 0; n < ns + e + 1 - lo; n++) {
+    const int j = n < ns ? n : lo + n - ns;
+    if (j >> c.page_sh != at) { at = j >> c.page_sh; id = kv_page(c, b, at); }
+    if (id < 0) continue;
+    const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + lane * E;
+    float k[E], v[E];
+    kv_row_in<T, E>((const T *)c.k + p, true, k);
+    kv_row_in<T, E>((const T *)c.v + p, true, v);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; i++) s += q[i] * k[i];
+    s = kv_warp_sum(s);
+    const float mn = fmaxf(m, s), cf = m == -INFINITY ? 0.0f : exp2f(m - mn), w = s == -INFINITY ? 0.0f : exp2f(s - mn);
+    l = l * cf + w;
+#pragma unroll
+    for (int i = 0; i < E; i++) o[i] = o[i] * cf + w * v[i];
+    m = mn;
+  }
+}
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) k_kv_attn_row(const KvDev c, const KvRows rw, const KvAttn a) {
+  constexpr int E = HD / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), r = blockIdx.x;
+  const int b = kv_find(rw, c.seqs, r, lane);
+  if (!blockIdx.x && !blockIdx.y) kv_check_rows(c, rw);
+  if (b < 0 || h >= a.H) return;
+  int first;
+  const int n = kv_rows(c, rw, b, first), e = kv_len(c, b) - n + r - first;
+  if (r - first >= rw.max_rows) return;
+  float o[E], m, l;
+  kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
+  if (a.lse && lane == 0) a.lse[(size_t)r * a.H + h] = l > 0.0f ? m + log2f(l) : INFINITY;
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] = l > 0.0f ? o[i] / l : l == 0.0f ? 0.0f : o[i] / l;
+  const long long at = r * a.os + (long long)h * HD + lane * E;
+  if (a.out32) {
+#pragma unroll
+    for (int i = 0; i < E; i++) ((float *)a.out)[at + i] = o[i];
+  } else kv_row_out<T, E>((uint16_t *)a.out + at, true, o);
+}
+// what every slot got: a warp a slot of a kv head
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) k_kv_weights(const KvDev c, const KvRows rw, const KvAttn a) {
+  constexpr int E = HD / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, j = blockIdx.x * 8 + (threadIdx.x >> 5), g = blockIdx.y, b = blockIdx.z, G = a.H / c.KV;
+  const int len = kv_len(c, b);
+  if (j >= len) return;
+  int first;
+  const int n = kv_rows(c, rw, b, first);
+  bool any = false;
+  for (int i = 0; i < min(n, rw.max_rows); i++) any = any || kv_sees(j, len - n + i, a.window, a.sinks);
+  const int id = any ? kv_page(c, b, j >> c.page_sh) : -1;
+  const size_t wi = ((size_t)b * c.KV + g) * a.wstride + j;
+  float k[E], sum = 0.0f;
+  if (id >= 0) {
+    kv_row_in<T, E>((const T *)c.k + kv_at(c, id, g, HD) + (size_t)(j & ((1 << c.page_sh) - 1)) * HD + lane * E, true, k);
+    for (int i = 0; i < min(n, rw.max_rows); i++) {
+      if (!kv_sees(j, len - n + i, a.window, a.sinks)) continue;
+      for (int h = g * G; h < (g + 1) * G; h++) {
+        float q[E], s = 0.0f;
+        kv_row_in<T, E>((const T *)a.q + (first + i) * a.qs + (long long)h * HD + lane * E, true, q);
+#pragma unroll
+        for (int d = 0; d < E; d++) s += q[d] * a.scale2 * k[d];
+        sum += exp2f(kv_warp_sum(s) - __ldcg(a.lse + (size_t)(first + i) * a.H + h));
+      }
+    }
+  }
+  if (lane == 0) a.w_out[wi] = (a.w_in ? __ldcg(a.w_in + wi) : 0.0f) + sum;
+}
+
+// ---- eviction -------------------------------------------------------------------------------------
+struct KvEvict {
+  int budget, sinks, recent;
+  const float *w;
+  int wstride;
+  float *w_out;
+  int w_out_stride;
+  int *kept;
+  int kept_stride;             // (kept: the caller's, or the workspace)
+  int *dst_lens;
+};
+// order-preserving key of a weight; NaN below every number, zeros alike
+__device__ __forceinline__ uint32_t kv_key(float w) {
+  if (w != w) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+// Which slots stay: a block a kv head of a sequence.  The weight that the last one has, by four passes over the keys' bytes (counts in shared
+// memory), then the slots above it and the first of those that equal it, in order.
+template <int NT>
+__global__ void __launch_bounds__(NT) k_kv_pick(const KvDev c, const KvEvict e) {
+  __shared__ int hist[256], part[NT / 32][2], base[2], pick[2];
+  pdl_trigger();
+  pdl_wait();
+  const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int len = kv_len(c, b), now = min(len, e.budget);
+  int *kept = e.kept + ((size_t)b * c.KV + g) * e.kept_stride;
+  if (g == 0 && tid == 0) e.dst_lens[b] = now;
+  if (len <= e.budget) {
+    for (int i = tid; i < len; i += NT) kept[i] = i;
+    return;
+  }
+  const float *w = e.w + ((size_t)b * c.KV + g) * e.wstride;
+  const int lo = e.sinks, hi = len - e.recent;
+  int want = e.budget - e.sinks - e.recent;    // of lo .. hi - 1, more than it
+  for (int i = tid; i < lo; i += NT) kept[i] = i;
+  for (int i = tid; i < e.recent; i += NT) kept[e.budget - e.recent + i] = hi + i;
+  if (!want) return;
+  uint32_t key = 0;
+  for (int sh = 24; sh >= 0; sh -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+    for (int i = lo + tid; i < hi; i += NT) {
+      const uint32_t u = kv_key(__ldcg(w + i));
+      if (sh == 24 || u >> (sh + 8) == key >> (sh + 8)) atomicAdd(hist + ((u >> sh) & 255), 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int left = want, d = 255;
+      while (hist[d] < left) left -= hist[d--];
+      pick[0] = d; pick[1] = left;
+    }
+    __syncthreads();
+    key |= (uint32_t)pick[0] << sh;
+    want = pick[1];                            // of those that equal the key so far
+  }
+  if (tid < 2) base[tid] = 0;
+  __syncthreads();
+  for (int i0 = lo; i0 < hi; i0 += NT) {
+    const int i = i0 + tid;
+    const uint32_t u = i < hi ? kv_key(__ldcg(w + i)) : 0;
+    const bool over = i < hi && u > key, same = i < hi && u == key;
+    const unsigned mo = __ballot_sync(0xffffffffu, over), ms = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
+    if (lane == 0) { part[warp][0] = __popc(mo); part[warp][1] = __popc(ms); }
+    __syncthreads();
+    int no = base[0] + __popc(mo & below), ne = base[1] + __popc(ms & below), to = 0, te = 0;
+    for (int k = 0; k < NT / 32; k++) {
+      if (k < warp) { no += part[k][0]; ne += part[k][1]; }
+      to += part[k][0]; te += part[k][1];
+    }
+    if (over || (same && ne < want)) kept[lo + no + min(ne, want)] = i;
+    __syncthreads();
+    if (tid == 0) { base[0] += to; base[1] += te; }
+    __syncthreads();
+  }
+}
+// K, V and weights of the kept slots into their new pages: 16 bytes a thread
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, const KvEvict e) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int P = HD / 8;    // pieces of a row
+  const int g = blockIdx.y, b = blockIdx.z, now = min(kv_len(c, b), e.budget);
+  const int *kept = e.kept + ((size_t)b * c.KV + g) * e.kept_stride;
+  for (int u = blockIdx.x * 256 + threadIdx.x; u < now * P; u += gridDim.x * 256) {
+    const int i = u / P, p = u % P, j = __ldcg(kept + i);
+    if (p == 0 && e.w_out) e.w_out[((size_t)b * c.KV + g) * e.w_out_stride + i] = __ldcg(e.w + ((size_t)b * c.KV + g) * e.wstride + j);
+    const int from = kv_page(c, b, j >> c.page_sh), to = kv_page(d, b, i >> d.page_sh);
+    if (from < 0 || to < 0) continue;
+    const size_t x = kv_at(c, from, g, HD) + (size_t)(j & ((1 << c.page_sh) - 1)) * HD + 8 * p, y = kv_at(d, to, g, HD) + (size_t)(i & ((1 << d.page_sh) - 1)) * HD + 8 * p;
+    *(uint4 *)(d.k + y) = __ldcg((const uint4 *)(c.k + x));
+    *(uint4 *)(d.v + y) = __ldcg((const uint4 *)(c.v + x));
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+int kv_setup(void) {
+  if (!g_kv_err) {
+    CU_OK(cudaMalloc(&g_kv_err, 4));
+    CU_OK(cudaMemset(g_kv_err, 0, 4));
+  }
+  return 0;
+}
+// A call's scope: the library's device for the calling thread, no launch recording, and no engine capturing meanwhile
+namespace {
+struct KvScope {
+  int was = -1;
+  std::lock_guard<std::recursive_mutex> hold{llb_enqueue_lock()};
+  KvScope() {
+    int d = 0;
+    if (cudaGetDevice(&d) == cudaSuccess && d != g_llb.device) { was = d; cudaSetDevice(g_llb.device); }
+  }
+  ~KvScope() { if (was >= 0) cudaSetDevice(was); }
+};
+}
+#define KV_BEGIN \
+  if (!g_llb.stream) return llb_fail("llb_b200_init has not been called"); \
+  KvScope scope; \
+  if (backend_graph_bail()) return -1
+
+static bool off(llb_b200_dptr p, unsigned n) { return p % n != 0; }
+static int kv_check(const llb_kv *kv, const char *what) {
+  if (!kv) return llb_fail("%s: no cache", what);
+  if (kv->el != LLB_EL_F16 && kv->el != LLB_EL_BF16) return llb_fail("%s: el %d (a cache is of f16 or bf16)", what, kv->el);
+  if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return llb_fail("%s: head_dim %d (64, 128 or 256)", what, kv->head_dim);
+  if (kv->kv_heads < 1 || kv->kv_heads > 1024) return llb_fail("%s: %d kv heads", what, kv->kv_heads);
+  if (kv->page != 16 && kv->page != 32 && kv->page != 64 && kv->page != 128) return llb_fail("%s: pages of %d slots (16, 32, 64 or 128)", what, kv->page);
+  if (kv->n_pages < 1) return llb_fail("%s: %d pages", what, kv->n_pages);
+  if (kv->seqs < 1 || kv->seqs > 65535) return llb_fail("%s: %d sequences (1 .. 65535)", what, kv->seqs);
+  if (kv->table_stride < 1) return llb_fail("%s: table_stride %d", what, kv->table_stride);
+  if (!kv->k || !kv->v || off(kv->k, 16) || off(kv->v, 16)) return llb_fail("%s: k and v lie on multiples of 16 bytes", what);
+  if (!kv->table || !kv->lens || off(kv->table, 4) || off(kv->lens, 4)) return llb_fail("%s: table and lens are int32 on the device", what);
+  return 0;
+}
+static long long kv_most(const llb_kv *kv) { return std::min((long long)kv->table_stride * kv->page, (long long)INT_MAX - 256); }
+static KvDev kv_dev(const llb_kv *kv, long long cap) {
+  KvDev c;
+  c.k = (uint16_t *)(uintptr_t)kv->k; c.v = (uint16_t *)(uintptr_t)kv->v;
+  c.table = (const int *)(uintptr_t)kv->table; c.lens = (const int *)(uintptr_t)kv->lens;
+  c.KV = kv->kv_heads; c.page_sh = kv->page == 16 ? 4 : kv->page == 32 ? 5 : kv->page == 64 ? 6 : 7;
+  c.n_pages = kv->n_pages; c.seqs = kv->seqs; c.tstride = kv->table_stride;
+  c.cap = (int)std::min(kv_most(kv), cap);
+  c.err = g_kv_err;
+  return c;
+}
+static int heads_check(const llb_kv *kv, int heads, const char *what) {
+  if (heads < 1 || heads % kv->kv_heads || heads / kv->kv_heads > 64) return llb_fail("%s: %d heads on %d kv heads", what, heads, kv->kv_heads);
+  return 0;
+}
+
+template <typename T, typename X> static int append_go(const KvDev &c, const KvRows &rw, const KvAppend &a, int hd) {
+  const dim3 grid(rw.rows, (a.H + 2 * c.KV + 7) / 8);
+  if (hd == 64) CU_OK(llb_launch(k_kv_append<T, X, 64>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+  else if (hd == 128) CU_OK(llb_launch(k_kv_append<T, X, 128>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+  else CU_OK(llb_launch(k_kv_append<T, X, 256>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+  return 0;
+}
+template <typename T, int HD> static int attn_go(const KvDev &c, const KvRows &rw, const KvAttn &a) {
+  if (rw.rows) CU_OK(llb_launch(k_kv_attn_row<T, HD>, dim3(rw.rows, (a.H + 3) / 4), dim3(128), (size_t)0, g_llb.stream, c, rw, a));
+  if (a.w_out && c.cap) CU_OK(llb_launch(k_kv_weights<T, HD>, dim3((c.cap + 7) / 8, c.KV, c.seqs), dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+  return 0;
+}
+
+static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
+  const char *const me = "kv_attn";
+  if (kv_check(kv, me)) return -1;
+  if (!a) return llb_fail("kv_attn: no call");
+  if (heads_check(kv, a->heads, me)) return -1;
+  if (a->rows < 0) return llb_fail("kv_attn: %d rows", a->rows);
+  if (a->max_rows < 1 || a->max_len < 0) return llb_fail("kv_attn: max_rows %d, max_len %d", a->max_rows, a->max_len);
+  if (a->window < 0 || a->sinks < 0) return llb_fail("kv_attn: window %d, sinks %d", a->window, a->sinks);
+  if (a->sinks && !a->window) return llb_fail("kv_attn: sinks without a window (every first slot is seen anyway)");
+  if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return llb_fail("kv_attn: scale %g", (double)a->scale);
+  if (a->el_out != LLB_EL_F32 && a->el_out != kv->el) return llb_fail("kv_attn: el_out %d (f32 or the cache's type)", a->el_out);
+  const long long row = (long long)a->heads * kv->head_dim;
+  if ((a->rows && (!a->q || !a->out)) || off(a->q, 16) || off(a->out, 16)) return llb_fail("kv_attn: q and out lie on multiples of 16 bytes");
+  if (a->q_stride < row || a->q_stride % 8) return llb_fail("kv_attn: q_stride %lld for rows of %lld", a->q_stride, row);
+  if (a->out_stride < row || a->out_stride % (a->el_out == LLB_EL_F32 ? 4 : 8)) return llb_fail("kv_attn: out_stride %lld for rows of %lld", a->out_stride, row);
+  if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");
+  if (a->w_in && !a->w_out) return llb_fail("kv_attn: w_in without w_out");
+  if (a->w_out) {
+    if (off(a->w_in, 4) || off(a->w_out, 4)) return llb_fail("kv_attn: weights are f32 on the device");
+    if (a->w_stride < a->max_len) return llb_fail("kv_attn: w_stride %d for %d slots", a->w_stride, a->max_len);
+    if ((long long)a->heads / kv->kv_heads * a->max_rows > 64) return llb_fail("kv_attn: weights of %d rows of %d heads a kv head (64 together at most)", a->max_rows, a->heads / kv->kv_heads);
+  }
+  return 0;
+}
+static size_t attn_ws(const llb_kv *kv, const llb_kv_attn *a) {
+  (void)kv;
+  size_t n = 16;
+  if (a->w_out) n += (size_t)a->rows * a->heads * 4;
+  return n;
+}
+static int evict_check(const llb_kv *src, const llb_kv_evict *e) {
+  if (kv_check(src, "kv_evict")) return -1;
+  if (!e) return llb_fail("kv_evict: no call");
+  if (e->budget < 1 || e->sinks < 0 || e->recent < 0 || (long long)e->sinks + e->recent > e->budget)
+    return llb_fail("kv_evict: budget %d with %d first and %d last slots", e->budget, e->sinks, e->recent);
+  if (e->max_len < 0) return llb_fail("kv_evict: max_len %d", e->max_len);
+  const int most = std::min(e->budget, e->max_len);
+  if (!e->w || off(e->w, 4) || e->w_stride < e->max_len) return llb_fail("kv_evict: weights of %d slots a head for %d", e->w_stride, e->max_len);
+  if (e->w_out && (off(e->w_out, 4) || e->w_out == e->w || e->w_out_stride < most)) return llb_fail("kv_evict: w_out is not w and has %d slots a head or more", most);
+  if (e->kept && (off(e->kept, 4) || e->kept_stride < most)) return llb_fail("kv_evict: kept has %d slots a head or more", most);
+  return 0;
+}
+static size_t evict_ws(const llb_kv *src, const llb_kv_evict *e) { return 16 + (e->kept ? 0 : (size_t)src->seqs * src->kv_heads * std::min(e->budget, e->max_len) * 4); }
+
+extern "C" {
+
+int llb_b200_kv_errors(void) {
+  KV_BEGIN;
+  unsigned int v = 0;
+  CU_OK(cudaMemcpyAsync(&v, g_kv_err, 4, cudaMemcpyDeviceToHost, g_llb.stream));
+  CU_OK(cudaStreamSynchronize(g_llb.stream));
+  return (int)v;
+}
+int llb_b200_kv_errors_clear(void) {
+  KV_BEGIN;
+  CU_OK(cudaMemsetAsync(g_kv_err, 0, 4, g_llb.stream));
+  return 0;
+}
+
+int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a) {
+  const char *const me = "kv_append";
+  if (kv_check(kv, me)) return -1;
+  if (!a) return llb_fail("kv_append: no call");
+  if (heads_check(kv, a->heads, me)) return -1;
+  const int hd = kv->head_dim;
+  if (a->rows < 0) return llb_fail("kv_append: %d rows", a->rows);
+  if (a->el_in < LLB_EL_F32 || a->el_in > LLB_EL_BF16) return llb_fail("kv_append: el_in %d", a->el_in);
+  if (a->rope_dim < 0 || a->rope_dim > hd || a->rope_dim % 2) return llb_fail("kv_append: rope_dim %d with head_dim %d", a->rope_dim, hd);
+  if (!(a->eps > 0.0f) || a->eps > 3.0e38f) return llb_fail("kv_append: eps %g", (double)a->eps);
+  const unsigned es = a->el_in == LLB_EL_F32 ? 4 : 2;
+  if ((a->rows && (!a->k || !a->v)) || off(a->q, es) || off(a->k, es) || off(a->v, es)) return llb_fail("kv_append: q, k and v lie on multiples of their elements");
+  if (a->q && (a->q_head_stride < hd || a->q_stride < (long long)(a->heads - 1) * a->q_head_stride + hd)) return llb_fail("kv_append: heads of q %d apart, rows %lld", a->q_head_stride, a->q_stride);
+  if (a->k_stride < (long long)kv->kv_heads * hd || a->v_stride < (long long)kv->kv_heads * hd) return llb_fail("kv_append: k_stride %lld, v_stride %lld", a->k_stride, a->v_stride);
+  if (a->q && (!a->q_out || off(a->q_out, 2) || a->q_out_stride < (long long)a->heads * hd)) return llb_fail("kv_append: q_out with rows %lld apart", a->q_out_stride);
+  if (off(a->q_norm, 4) || off(a->k_norm, 4)) return llb_fail("kv_append: norm weights are f32 on the device");
+  if (a->rope_dim && (!a->invfreq || off(a->invfreq, 8))) return llb_fail("kv_append: invfreq is f64 on the device");
+  if (!a->row_start || off(a->row_start, 4) || off(a->pos, 4)) return llb_fail("kv_append: row_start and pos are int32 on the device");
+  KV_BEGIN;
+  if (!a->rows) return 0;
+  const KvDev c = kv_dev(kv, LLONG_MAX);
+  const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, a->rows};
+  KvAppend k;
+  k.q = (const void *)(uintptr_t)a->q; k.k = (const void *)(uintptr_t)a->k; k.v = (const void *)(uintptr_t)a->v;
+  k.qs = a->q_stride; k.ks = a->k_stride; k.vs = a->v_stride; k.qhs = a->q_head_stride;
+  k.qn = (const float *)(uintptr_t)a->q_norm; k.kn = (const float *)(uintptr_t)a->k_norm;
+  k.invfreq = (const double *)(uintptr_t)a->invfreq; k.pos = (const int *)(uintptr_t)a->pos;
+  k.qo = (uint16_t *)(uintptr_t)a->q_out; k.qos = a->q_out_stride;
+  k.H = a->heads; k.rope = a->rope_dim; k.eps = a->eps;
+  // a lane's head_dim / 32 elements in wide words, where all of q, k, v and q_out have them there
+  const int E = hd / 32;
+  const unsigned in = es == 4 ? 8 : 2 * E;
+  k.wide = !off(a->q, in) && !off(a->k, in) && !off(a->v, in) && a->q_stride % E == 0 && a->k_stride % E == 0 && a->v_stride % E == 0 && a->q_head_stride % E == 0 &&
+           !off(a->q_out, 2 * E) && a->q_out_stride % E == 0;
+  if (kv->el == LLB_EL_F16) {
+    if (a->el_in == LLB_EL_F32) return append_go<__half, float>(c, rw, k, hd);
+    if (a->el_in == LLB_EL_F16) return append_go<__half, __half>(c, rw, k, hd);
+    return append_go<__half, __nv_bfloat16>(c, rw, k, hd);
+  }
+  if (a->el_in == LLB_EL_F32) return append_go<__nv_bfloat16, float>(c, rw, k, hd);
+  if (a->el_in == LLB_EL_F16) return append_go<__nv_bfloat16, __half>(c, rw, k, hd);
+  return append_go<__nv_bfloat16, __nv_bfloat16>(c, rw, k, hd);
+}
+
+size_t llb_b200_kv_attn_ws(const llb_kv *kv, const llb_kv_attn *a) { return attn_check(kv, a) ? 0 : attn_ws(kv, a); }
+int llb_b200_kv_attn(const llb_kv *kv, const llb_kv_attn *a) {
+  if (attn_check(kv, a)) return -1;
+  const size_t need = attn_ws(kv, a);
+  if (!a->ws || off(a->ws, 16) || a->ws_bytes < need) return llb_fail("kv_attn: a workspace of %zu bytes (%zu are needed, on a multiple of 16)", a->ws_bytes, need);
+  KV_BEGIN;
+  if (!a->rows && !a->w_out) return 0;
+  const KvDev c = kv_dev(kv, a->max_len);
+  const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, a->max_rows};
+  KvAttn k;
+  k.q = (const uint16_t *)(uintptr_t)a->q; k.out = (void *)(uintptr_t)a->out;
+  k.qs = a->q_stride; k.os = a->out_stride; k.H = a->heads; k.window = a->window; k.sinks = a->sinks; k.out32 = a->el_out == LLB_EL_F32;
+  k.scale2 = (float)((a->scale > 0.0f ? (double)a->scale : 1.0 / sqrt((double)kv->head_dim)) * 1.4426950408889634);
+  k.w_in = (const float *)(uintptr_t)a->w_in; k.w_out = (float *)(uintptr_t)a->w_out; k.wstride = a->w_stride;
+  k.lse = a->w_out ? (float *)(uintptr_t)a->ws : nullptr;
+  if (kv->el == LLB_EL_F16) return kv->head_dim == 64 ? attn_go<__half, 64>(c, rw, k) : kv->head_dim == 128 ? attn_go<__half, 128>(c, rw, k) : attn_go<__half, 256>(c, rw, k);
+  return kv->head_dim == 64 ? attn_go<__nv_bfloat16, 64>(c, rw, k) : kv->head_dim == 128 ? attn_go<__nv_bfloat16, 128>(c, rw, k) : attn_go<__nv_bfloat16, 256>(c, rw, k);
+}
+
+size_t llb_b200_kv_evict_ws(const llb_kv *src, const llb_kv_evict *e) { return evict_check(src, e) ? 0 : evict_ws(src, e); }
+int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *e) {
+  if (evict_check(src, e) || kv_check(dst, "kv_evict: dst")) return -1;
+  if (dst->el != src->el || dst->kv_heads != src->kv_heads || dst->head_dim != src->head_dim || dst->seqs != src->seqs)
+    return llb_fail("kv_evict: dst has another type, other heads or other sequences than src");
+  if (dst->table == src->table || dst->lens == src->lens) return llb_fail("kv_evict: dst has a table and lens of its own");
+  const int most = std::min(e->budget, e->max_len);
+  if (kv_most(dst) < most) return llb_fail("kv_evict: dst holds %lld slots a sequence, %d may be kept", kv_most(dst), most);
+  const size_t need = evict_ws(src, e);
+  if (!e->kept && (!e->ws || off(e->ws, 16) || e->ws_bytes < need)) return llb_fail("kv_evict: a workspace of %zu bytes (%zu are needed, on a multiple of 16)", e->ws_bytes, need);
+  KV_BEGIN;
+  const KvDev c = kv_dev(src, e->max_len), d = kv_dev(dst, LLONG_MAX);
+  KvEvict k;
+  k.budget = e->budget; k.sinks = e->sinks; k.recent = e->recent;
+  k.w = (const float *)(uintptr_t)e->w; k.wstride = e->w_stride;
+  k.w_out = (float *)(uintptr_t)e->w_out; k.w_out_stride = e->w_out_stride;
+  k.kept = (int *)(uintptr_t)(e->kept ? e->kept : e->ws); k.kept_stride = e->kept ? e->kept_stride : most;
+  k.dst_lens = (int *)(uintptr_t)dst->lens;
+  CU_OK(llb_launch(k_kv_pick<1024>, dim3(c.KV, c.seqs), dim3(1024), (size_t)0, g_llb.stream, c, k));
+  if (!most) return 0;
+  const dim3 grid(std::max(1, std::min(256, most * (src->head_dim / 8) / 1024)), c.KV, c.seqs);
+  if (src->head_dim == 64) CU_OK(llb_launch(k_kv_move<64>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
+  else if (src->head_dim == 128) CU_OK(llb_launch(k_kv_move<128>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
+  else CU_OK(llb_launch(k_kv_move<256>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
+  return 0;
+}
+
+}  // extern "C"

@@ -83,6 +83,9 @@ def lib() -> C.CDLL:
             "llb_spec_position_stream": (i32, [vp, i32]), "llb_spec_stats_stream": (i32, [vp, i32, vp]),
             "llb_spec_read_state_stream": (i32, [vp, i32, i32, i32, i32, vp, sz]),
             "llb_spec_set_prefill": (i32, [vp, i32]), "llb_spec_fast_rows": (C.c_double, [vp]), "llb_spec_prefill_extra": (i32, [vp, C.c_size_t]),
+            "llb_b200_kv_append": (i32, [vp, vp]), "llb_b200_kv_attn": (i32, [vp, vp]), "llb_b200_kv_attn_ws": (sz, [vp, vp]),
+            "llb_b200_kv_evict": (i32, [vp, vp, vp]), "llb_b200_kv_evict_ws": (sz, [vp, vp]),
+            "llb_b200_kv_errors": (i32, []), "llb_b200_kv_errors_clear": (i32, []),
             "llb_b200_pf_gemm": (i32, [i32, u64, i32, i32, u64, i32, u64, i32]),
             "llb_b200_gemm_fits": (i32, [i32, i32, i32, i32]), "llb_b200_gemm_kernel": (i32, [i32, i32, i32, i32, i32, i32, C.POINTER(i32)]),
             "llb_b200_gemm3_trace": (i32, [i32, i32, i32, i32, C.POINTER(i32), i32]), "llb_b200_gemm3_bar_count": (i32, [i32, i32]),
@@ -192,6 +195,68 @@ def gemm(fmt: int, ws, rows, outs, K: int, xp, ksplit: int = 0):
         rc = lib().llb_b200_gemm(fmt, n, arr(C.c_uint64, ws), arr(C.c_int, rows), arr(C.c_uint64, outs), K, xp, ksplit)
     if rc < 0:
         check(rc, "llb_b200_gemm")
+
+
+EL = {"f32": 0, "f16": 1, "bf16": 2}   # element types (LLB_EL_*)
+_INT, _PTR, _LONG = C.c_int, C.c_uint64, C.c_longlong
+
+
+class Kv(C.Structure):
+    """llb_kv: the paged key-value cache of `seqs` sequences.  Memory is the caller's (device addresses)."""
+    _fields_ = [(n, _INT) for n in ("el", "kv_heads", "head_dim", "page", "n_pages", "seqs", "table_stride")] + [(n, _PTR) for n in ("k", "v", "table", "lens")]
+
+
+class KvAppend(C.Structure):
+    """llb_kv_append: rows to be normed, rotated and stored."""
+    _fields_ = [("rows", _INT), ("heads", _INT), ("el_in", _INT), ("rope_dim", _INT), ("eps", C.c_float), ("q", _PTR), ("k", _PTR), ("v", _PTR),
+                ("q_stride", _LONG), ("k_stride", _LONG), ("v_stride", _LONG), ("q_head_stride", _INT), ("q_norm", _PTR), ("k_norm", _PTR), ("invfreq", _PTR),
+                ("row_start", _PTR), ("pos", _PTR), ("q_out", _PTR), ("q_out_stride", _LONG)]
+
+
+class KvAttn(C.Structure):
+    """llb_kv_attn: the attention of a call's rows."""
+    _fields_ = [("rows", _INT), ("max_rows", _INT), ("max_len", _INT), ("heads", _INT), ("window", _INT), ("sinks", _INT), ("scale", C.c_float), ("el_out", _INT),
+                ("q", _PTR), ("out", _PTR), ("q_stride", _LONG), ("out_stride", _LONG), ("row_start", _PTR), ("w_in", _PTR), ("w_out", _PTR), ("w_stride", _INT),
+                ("ws", _PTR), ("ws_bytes", C.c_size_t)]
+
+
+class KvEvict(C.Structure):
+    """llb_kv_evict: how sequences are thinned."""
+    _fields_ = [("budget", _INT), ("sinks", _INT), ("recent", _INT), ("max_len", _INT), ("w", _PTR), ("w_stride", _INT), ("w_out", _PTR), ("w_out_stride", _INT),
+                ("kept", _PTR), ("kept_stride", _INT), ("ws", _PTR), ("ws_bytes", C.c_size_t)]
+
+
+def kv_append(kv: Kv, a: KvAppend):
+    """Norm and rotation of a call's queries and keys; keys and values into their slots."""
+    if lib().llb_b200_kv_append(C.byref(kv), C.byref(a)) < 0:
+        check(-1, "llb_b200_kv_append")
+
+
+def kv_attn_ws(kv: Kv, a: KvAttn) -> int:
+    """Bytes of the call's workspace (no GPU needed)."""
+    return handle(lib().llb_b200_kv_attn_ws(C.byref(kv), C.byref(a)), "llb_b200_kv_attn_ws")
+
+
+def kv_attn(kv: Kv, a: KvAttn):
+    """Attention of a call's rows over the cache."""
+    if lib().llb_b200_kv_attn(C.byref(kv), C.byref(a)) < 0:
+        check(-1, "llb_b200_kv_attn")
+
+
+def kv_evict_ws(kv: Kv, e: KvEvict) -> int:
+    """Bytes of the call's workspace (no GPU needed)."""
+    return handle(lib().llb_b200_kv_evict_ws(C.byref(kv), C.byref(e)), "llb_b200_kv_evict_ws")
+
+
+def kv_evict(src: Kv, dst: Kv, e: KvEvict):
+    """Sequences thinned to a budget of slots, into dst's pages."""
+    if lib().llb_b200_kv_evict(C.byref(src), C.byref(dst), C.byref(e)) < 0:
+        check(-1, "llb_b200_kv_evict")
+
+
+def kv_errors() -> int:
+    """What the calls met in device memory, as bits: 1 page ids, 2 lengths, 4 row_start."""
+    return check(lib().llb_b200_kv_errors(), "llb_b200_kv_errors")
 
 
 class SmpParams(C.Structure):

@@ -141,6 +141,100 @@ LLB_API int llb_b200_pf_gemm(int fmt, llb_b200_dptr w, int rows, int K, llb_b200
  * so two calls whose GPU work overlaps (different streams, different threads) race. */
 LLB_API int llb_b200_gemm_noalloc(int fmt, llb_b200_dptr w, int rows, int K, llb_b200_dptr x_f32, int T, llb_b200_dptr out_f32);
 
+/* ---- 2b. a paged key-value cache ---------------------------------------------------------------- */
+/* For hosts that build a model's attention from operators and serve many sequences: a pool of pages that sequences take and give back
+ * (the engine of layer 3 has one contiguous cache a stream, as host/llb_host.c:1627-1628).  Three calls: llb_b200_kv_append stores a
+ * step's rows, llb_b200_kv_attn reads, llb_b200_kv_evict thins a sequence.  All of them only queue work on the library's stream, allocate
+ * nothing, and may be captured into a graph of the caller's; lengths, tables and positions are device memory, so that a captured
+ * step runs again with other contents.  Memory is the caller's throughout: pool, tables, rows, workspaces. */
+/* element types of the operators that take one */
+enum { LLB_EL_F32 = 0, LLB_EL_F16 = 1, LLB_EL_BF16 = 2 };
+/* The cache of `seqs` sequences.  Slot j of sequence b is slot j % page of page table[b * table_stride + j / page]; that page holds
+ * it at k + (((id * kv_heads + g) * page + j % page) * head_dim) elements for kv head g, and likewise in v.  Sequences may share pages
+ * that they only read.  Entries behind a sequence's last slot (and, in llb_b200_kv_attn, of slots that no row of the call sees) are not
+ * looked at.  lens[b] counts the slots in use, the rows of the call among them: llb_b200_kv_append stores the n rows of a sequence in its last n slots. */
+typedef struct {
+  int el;                      /* LLB_EL_F16 or LLB_EL_BF16 */
+  int kv_heads, head_dim;      /* head_dim 64, 128 or 256 */
+  int page;                    /* slots of a page: 16, 32, 64 or 128 */
+  int n_pages;                 /* of the pool */
+  int seqs;                    /* 1 .. 65535 */
+  int table_stride;            /* entries of a sequence in the table: table_stride * page slots are the most it can have */
+  llb_b200_dptr k, v;          /* [n_pages][kv_heads][page][head_dim], 16-byte aligned */
+  llb_b200_dptr table;         /* int32 [seqs][table_stride] */
+  llb_b200_dptr lens;          /* int32 [seqs] */
+} llb_kv;
+/* The rows of a call: sequence b has rows row_start[b] .. row_start[b + 1] - 1 (int32 [seqs + 1] on the device, not falling, within
+ * 0 .. rows); row i of n is at slot lens[b] - n + i.  Rows behind row_start[seqs] are left as they are.
+ *
+ * Norm and rotation of queries and keys in the pass that stores K and V (llb_t_qkr, tools/payload-spec2.patch:159-204): every head of q
+ * and k is divided by sqrt(mean square + eps) and multiplied by q_norm / k_norm (either 0: no norm), the first rope_dim
+ * dimensions are rotated in pairs (i, i + rope_dim / 2) by the angle position * invfreq[i], taken in 64 bits.  q goes to q_out in the cache's type, k
+ * and v into their slots; q = 0: keys and values only.  A row at a slot below 0 (a length smaller than the rows) is not stored. */
+typedef struct {
+  int rows;                          /* rows that q, k, v and q_out have */
+  int heads;                         /* query heads, a multiple of kv_heads */
+  int el_in;                         /* type of q, k and v: LLB_EL_* */
+  int rope_dim;                      /* even, 0 (no rotation) .. head_dim */
+  float eps;                         /* > 0 */
+  llb_b200_dptr q, k, v;             /* aligned to their elements; head h of row r of q at r * q_stride + h * q_head_stride, of k and v at r * stride + h * head_dim */
+  long long q_stride, k_stride, v_stride;   /* elements */
+  int q_head_stride;                 /* elements, head_dim or more (2 * head_dim where a gate lies behind every head) */
+  llb_b200_dptr q_norm, k_norm;      /* f32 [head_dim], or 0 */
+  llb_b200_dptr invfreq;             /* f64 [rope_dim / 2] */
+  llb_b200_dptr row_start;
+  llb_b200_dptr pos;                 /* int32 [seqs], the position of a sequence's first row; 0: a row's position is its slot */
+  llb_b200_dptr q_out;               /* [rows][q_out_stride], the cache's type */
+  long long q_out_stride;            /* elements, heads * head_dim or more */
+} llb_kv_append;
+LLB_API int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a);
+/* Attention of a call's rows: the row at slot e sees slots j <= e, with window > 0 only those with j > e - window or j < sinks.
+ * out = sum_j softmax_j(scale q . K_j) V_j for head h on kv head h / (heads / kv_heads); a row that sees nothing gets zeros.  K and V may
+ * hold anything, infinities and NaN included, where a row does not see them.  Scores, softmax and sums are f32; the probabilities take
+ * part in the second product in the cache's type.
+ * w_out (0: not wanted): w_out[b][g][j] = w_in[b][g][j] + the probabilities that slot j got, summed over the rows of the sequence and
+ * the heads of kv head g, for j < lens[b]; other entries are left as they are.  w_in may be w_out, or 0 for zeros. */
+typedef struct {
+  int rows, max_rows, max_len;       /* rows that q and out have; the most rows and slots of a sequence */
+  int heads;                         /* query heads, a multiple of kv_heads, at most 64 a kv head */
+  int window, sinks;                 /* 0, 0: all slots up to the row's own */
+  float scale;                       /* 0: 1 / sqrt(head_dim) */
+  int el_out;                        /* LLB_EL_F32 or the cache's type */
+  llb_b200_dptr q, out;              /* [rows][stride], heads of head_dim side by side; q in the cache's type; 16-byte aligned */
+  long long q_stride, out_stride;    /* elements, heads * head_dim or more, whole 16 bytes */
+  llb_b200_dptr row_start;
+  llb_b200_dptr w_in, w_out;         /* f32 [seqs][kv_heads][w_stride]; heads / kv_heads * max_rows is 64 at most then */
+  int w_stride;                      /* max_len or more */
+  llb_b200_dptr ws;                  /* llb_b200_kv_attn_ws bytes, 16-byte aligned; needed from the call's first kernel to its last: calls on the one stream can share it */
+  size_t ws_bytes;
+} llb_kv_attn;
+LLB_API size_t llb_b200_kv_attn_ws(const llb_kv *kv, const llb_kv_attn *a);   /* 0 with a reason in llb_b200_last_error() where the call would be refused; needs no GPU */
+LLB_API int llb_b200_kv_attn(const llb_kv *kv, const llb_kv_attn *a);
+/* Every sequence of `src` of more than `budget` slots is thinned to budget, kv head by kv head: its first `sinks` and last `recent`
+ * slots stay, and of those between the ones of the largest weight w (equal ones: the lowest slots; NaN counts as less than every number), in their order.  A shorter
+ * one is kept whole.  K, V and weights of the kept slots go to the pages of `dst` (same type, heads and head_dim; another page size, or the same
+ * pool, are fine; src's lens are read, dst's written).  dst's pages have to be pages that no sequence of src or dst reads besides:
+ * a host takes fresh pages, thins, and gives the old ones back.  Slots behind the new length are left as they are. */
+typedef struct {
+  int budget, sinks, recent;         /* 0 <= sinks + recent <= budget, budget >= 1 */
+  int max_len;                       /* the most slots of a sequence */
+  llb_b200_dptr w;                   /* f32 [seqs][kv_heads][w_stride] */
+  int w_stride;                      /* max_len or more */
+  llb_b200_dptr w_out;               /* f32 [seqs][kv_heads][w_out_stride], the kept slots' weights; 0: not wanted; not w */
+  int w_out_stride;                  /* min(budget, max_len) or more */
+  llb_b200_dptr kept;                /* int32 [seqs][kv_heads][kept_stride], the slots of src that were kept; 0: not wanted */
+  int kept_stride;                   /* min(budget, max_len) or more */
+  llb_b200_dptr ws;                  /* llb_b200_kv_evict_ws bytes, 16-byte aligned */
+  size_t ws_bytes;
+} llb_kv_evict;
+LLB_API size_t llb_b200_kv_evict_ws(const llb_kv *src, const llb_kv_evict *e);   /* as llb_b200_kv_attn_ws */
+LLB_API int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *e);
+/* What the calls met in device memory since llb_b200_init, as bits: 1 a page id outside the pool (its slots were not read, not
+ * stored, not seen), 2 a length below 0 or above what the table or the call's max_len holds (it was cut to that), 4 row_start falling, outside 0 .. rows, or more than max_rows
+ * rows of a sequence (its rows, or those behind, were left out).  Synchronises.  -1 on a CUDA error. */
+LLB_API int llb_b200_kv_errors(void);
+LLB_API int llb_b200_kv_errors_clear(void);
+
 /* ---- 3. the speculative cycle ----------------------------------------------------------------- */
 /* Replaces host/llb_host.c:1474-1950 for greedy decoding with either of the reference's drafters.
  * index_text: the pack's index.tsv (tools/qwen35_engine.c:379-433); pack: pack.bin bytes (host, or a
