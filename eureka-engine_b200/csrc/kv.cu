@@ -6,8 +6,10 @@
 #include "../../include/llb_b200.h"
 #include "host.cuh"
 #include "kv.cuh"
+#include "kvatt.cuh"
 
 static unsigned int *g_kv_err = nullptr;   // what the kernels met (KV_ERR_*)
+static decltype(&cuTensorMapEncodeTiled) g_kv_map = nullptr;
 
 // ---- rows in ------------------------------------------------------------------------------------
 // A warp a head of a row, eight of them a block, whose threads make the row's sines first.  Angles in 64 bits: at position
@@ -25,47 +27,6 @@ struct KvAppend {
   float eps;
   int wide;                    // q, k, v and q_out: a lane's elements lie on a multiple of their size
 };
-template <typename X, int E> __device__ __forceinline__ void kv_row_in(const X *p, bool wide, float (&x)[E]) {
-  if constexpr (sizeof(X) == 4) {
-    if (wide) {
-#pragma unroll
-      for (int i = 0; i < E; i += 2) { const float2 f = __ldcg((const float2 *)(p + i)); x[i] = f.x; x[i + 1] = f.y; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; i++) x[i] = __ldcg((const float *)p + i);
-    }
-  } else {
-    if (wide) {
-      uint32_t w[E / 2];
-      if constexpr (E == 2) w[0] = __ldcg((const uint32_t *)p);
-      else if constexpr (E == 4) { const uint2 t = __ldcg((const uint2 *)p); w[0] = t.x; w[1] = t.y; }
-      else { const uint4 t = __ldcg((const uint4 *)p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
-#pragma unroll
-      for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<X>::to2(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; i++) x[i] = KvEl<X>::to(__ldcg((const uint16_t *)p + i));
-    }
-  }
-}
-template <typename T, int E> __device__ __forceinline__ void kv_row_out(uint16_t *p, bool wide, const float (&x)[E]) {
-  if (wide) {
-    uint32_t w[E / 2];
-#pragma unroll
-    for (int i = 0; i < E / 2; i++) w[i] = KvEl<T>::of2(x[2 * i], x[2 * i + 1]);
-    if constexpr (E == 2) *(uint32_t *)p = w[0];
-    else if constexpr (E == 4) *(uint2 *)p = make_uint2(w[0], w[1]);
-    else *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; i++) p[i] = KvEl<T>::of(x[i]);
-  }
-}
-__device__ __forceinline__ float kv_warp_sum(float v) {
-#pragma unroll
-  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-  return v;
-}
 template <typename T, typename X, int HD>
 __global__ void __launch_bounds__(256) k_kv_append(const KvDev c, const KvRows rw, const KvAppend a) {
   constexpr int E = HD / 32;
@@ -123,52 +84,9 @@ __global__ void __launch_bounds__(256) k_kv_append(const KvDev c, const KvRows r
   kv_row_out<T, E>((isv ? c.v : c.k) + kv_at(c, id, g, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD + lane * E, true, x);
 }
 
-// ---- attention, a warp a head of a row --------------------------------------------------------------
-struct KvAttn {
-  const uint16_t *q;
-  void *out;
-  long long qs, os;            // elements between rows
-  int H, window, sinks, out32;
-  float scale2;                // times log2(e): probabilities are powers of two
-  const float *w_in;
-  float *w_out;
-  int wstride;
-  float *lse;                  // [rows][H], base 2; where w_out is wanted
-};
-// one row and head over the slots that it sees, a slot at a time; lane's dimensions E lane ..
-template <typename T, int HD>
-__device__ __forceinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float (&o)[HD / 32], float &m, float &l) {
-  constexpr int E = HD / 32;
-  const int g = h / (a.H / c.KV), pm = (1 << c.page_sh) - 1;
-  float q[E];
-  kv_row_in<T, E>((const T *)a.q + r * a.qs + (long long)h * HD + lane * E, true, q);
-#pragma unroll
-  for (int i = 0; i < E; i++) { q[i] *= a.scale2; o[i] = 0.0f; }
-  m = -INFINITY; l = 0.0f;
-  const int lo = kv_first(e, a.window), ns = min(a.sinks, lo);
-  int id = -1, at = -1;
-  for (int n = 0; n < ns + e + 1 - lo; n++) {
-    const int j = n < ns ? n : lo + n - ns;
-    if (j >> c.page_sh != at) { at = j >> c.page_sh; id = kv_page(c, b, at); }
-    if (id < 0) continue;
-    const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + lane * E;
-    float k[E], v[E];
-    kv_row_in<T, E>((const T *)c.k + p, true, k);
-    kv_row_in<T, E>((const T *)c.v + p, true, v);
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; i++) s += q[i] * k[i];
-    s = kv_warp_sum(s);
-    const float mn = fmaxf(m, s), cf = m == -INFINITY ? 0.0f : exp2f(m - mn), w = s == -INFINITY ? 0.0f : exp2f(s - mn);
-    l = l * cf + w;
-#pragma unroll
-    for (int i = 0; i < E; i++) o[i] = o[i] * cf + w * v[i];
-    m = mn;
-  }
-}
+// ---- attention, a warp a head of a row ------------------------------------------------------------
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) k_kv_attn_row(const KvDev c, const KvRows rw, const KvAttn a) {
-  constexpr int E = HD / 32;
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), r = blockIdx.x;
@@ -178,47 +96,9 @@ __global__ void __launch_bounds__(128) k_kv_attn_row(const KvDev c, const KvRows
   int first;
   const int n = kv_rows(c, rw, b, first), e = kv_len(c, b) - n + r - first;
   if (r - first >= rw.max_rows) return;
-  float o[E], m, l;
+  float o[HD / 32], m, l;
   kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
-  if (a.lse && lane == 0) a.lse[(size_t)r * a.H + h] = l > 0.0f ? m + log2f(l) : INFINITY;
-#pragma unroll
-  for (int i = 0; i < E; i++) o[i] = l > 0.0f ? o[i] / l : l == 0.0f ? 0.0f : o[i] / l;
-  const long long at = r * a.os + (long long)h * HD + lane * E;
-  if (a.out32) {
-#pragma unroll
-    for (int i = 0; i < E; i++) ((float *)a.out)[at + i] = o[i];
-  } else kv_row_out<T, E>((uint16_t *)a.out + at, true, o);
-}
-// what every slot got: a warp a slot of a kv head
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_kv_weights(const KvDev c, const KvRows rw, const KvAttn a) {
-  constexpr int E = HD / 32;
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, j = blockIdx.x * 8 + (threadIdx.x >> 5), g = blockIdx.y, b = blockIdx.z, G = a.H / c.KV;
-  const int len = kv_len(c, b);
-  if (j >= len) return;
-  int first;
-  const int n = kv_rows(c, rw, b, first);
-  bool any = false;
-  for (int i = 0; i < min(n, rw.max_rows); i++) any = any || kv_sees(j, len - n + i, a.window, a.sinks);
-  const int id = any ? kv_page(c, b, j >> c.page_sh) : -1;
-  const size_t wi = ((size_t)b * c.KV + g) * a.wstride + j;
-  float k[E], sum = 0.0f;
-  if (id >= 0) {
-    kv_row_in<T, E>((const T *)c.k + kv_at(c, id, g, HD) + (size_t)(j & ((1 << c.page_sh) - 1)) * HD + lane * E, true, k);
-    for (int i = 0; i < min(n, rw.max_rows); i++) {
-      if (!kv_sees(j, len - n + i, a.window, a.sinks)) continue;
-      for (int h = g * G; h < (g + 1) * G; h++) {
-        float q[E], s = 0.0f;
-        kv_row_in<T, E>((const T *)a.q + (first + i) * a.qs + (long long)h * HD + lane * E, true, q);
-#pragma unroll
-        for (int d = 0; d < E; d++) s += q[d] * a.scale2 * k[d];
-        sum += exp2f(kv_warp_sum(s) - __ldcg(a.lse + (size_t)(first + i) * a.H + h));
-      }
-    }
-  }
-  if (lane == 0) a.w_out[wi] = (a.w_in ? __ldcg(a.w_in + wi) : 0.0f) + sum;
+  kv_finish<T, HD>(c, a, b, r, h, e, lane, o, m, l);
 }
 
 // ---- eviction -------------------------------------------------------------------------------------
@@ -317,7 +197,18 @@ __global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, c
 }
 
 // ---- host -----------------------------------------------------------------------------------------
+template <typename T, int HD> static int few_attr() {
+  CU_OK(cudaFuncSetAttribute(k_kv_few<T, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kf_smem(HD)));
+  CU_OK(cudaFuncSetAttribute(k_kv_few<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kf_smem(HD)));
+  return 0;
+}
 int kv_setup(void) {
+  if (few_attr<__half, 64>() || few_attr<__half, 128>() || few_attr<__half, 256>() || few_attr<__nv_bfloat16, 64>() || few_attr<__nv_bfloat16, 128>() || few_attr<__nv_bfloat16, 256>()) return -1;
+  if (!g_kv_map) {
+    cudaDriverEntryPointQueryResult found;
+    CU_OK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", (void **)&g_kv_map, 12000, cudaEnableDefault, &found));
+    if (!g_kv_map) return llb_fail("the driver has no cuTensorMapEncodeTiled");
+  }
   if (!g_kv_err) {
     CU_OK(cudaMalloc(&g_kv_err, 4));
     CU_OK(cudaMemset(g_kv_err, 0, 4));
@@ -378,9 +269,55 @@ template <typename T, typename X> static int append_go(const KvDev &c, const KvR
   else CU_OK(llb_launch(k_kv_append<T, X, 256>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
   return 0;
 }
-template <typename T, int HD> static int attn_go(const KvDev &c, const KvRows &rw, const KvAttn &a) {
-  if (rw.rows) CU_OK(llb_launch(k_kv_attn_row<T, HD>, dim3(rw.rows, (a.H + 3) / 4), dim3(128), (size_t)0, g_llb.stream, c, rw, a));
-  if (a.w_out && c.cap) CU_OK(llb_launch(k_kv_weights<T, HD>, dim3((c.cap + 7) / 8, c.KV, c.seqs), dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+// pages as [page][kv head][slot][dims], in boxes of 64 dims of `slots` slots of a kv head of a page
+static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int slots) {
+  const cuuint64_t row = (cuuint64_t)kv->head_dim * 2;
+  const cuuint64_t dim[4] = {(cuuint64_t)kv->head_dim, (cuuint64_t)kv->page, (cuuint64_t)kv->kv_heads, (cuuint64_t)kv->n_pages}, step[3] = {row, row * kv->page, row * kv->page * kv->kv_heads};
+  const cuuint32_t box[4] = {64, (cuuint32_t)slots, 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = g_kv_map(map, kv->el == LLB_EL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)(uintptr_t)base, dim, step, box, one,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : llb_fail("kv: tensor map of %d pages: error %d", kv->n_pages, (int)r);
+}
+// ---- which kernel, and its workspace ----
+#define KV_FEW 64              // queries a kv head up to which a call goes to k_kv_few
+#define KF_LEAST 8             // fewest chunks of a block's stretch: two a warp
+static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * a->max_rows <= KV_FEW; }
+static int few_grid(const llb_kv *kv) { return (g_llb.sms ? g_llb.sms : 148) * (kv->head_dim == 256 ? 1 : 2); }
+// its parts, one behind the other; the size where `base` is 0
+static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, KvPlan *p) {
+  const size_t blocks = few_grid(kv), queries = (size_t)kv->seqs * kv->kv_heads * (a->heads / kv->kv_heads) * a->max_rows;
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
+  p->least = KF_LEAST;
+  p->before = (long long *)take((size_t)(kv->seqs + 2) * 8);
+  p->pm = (float *)take(blocks * 2 * 16 * 4);
+  p->pl = (float *)take(blocks * 2 * 16 * 4);
+  p->po = (float *)take(blocks * 2 * 16 * kv->head_dim * 4);
+  p->sstride = std::max(16, (a->max_len + 15) & ~15);
+  p->lse = (float *)take(a->w_out ? queries * 4 : 0);
+  p->sc = (float *)take(a->w_out ? queries * p->sstride * 4 : 0);
+  return at;
+}
+template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_attn *call, const KvDev &c, const KvRows &rw, const KvAttn &a) {
+  KvPlan p;
+  few_plan(kv, call, (uintptr_t)call->ws, &p);
+  p.err = gemm_err_word();
+  CUtensorMap km, vm;
+  if (pool_map(&km, kv, kv->k, KF_SLOTS) || pool_map(&vm, kv, kv->v, KF_SLOTS)) return -1;
+  const dim3 grid(few_grid(kv)), block(32 * KF_WARPS);
+  const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + 511) / 512;   // (attn_check: they fit)
+  if (a.w_out) {
+    CU_OK(llb_launch(k_kv_few<T, HD, true>, grid, block, (size_t)kf_smem(HD), g_llb.stream, c, rw, a, p, km, vm));
+    CU_OK(llb_launch(k_kv_join<T, HD, true>, dim3(joins + wblocks * c.KV * c.seqs), dim3(128), (size_t)0, g_llb.stream, c, rw, a, p, joins, wblocks));
+  } else {
+    CU_OK(llb_launch(k_kv_few<T, HD, false>, grid, block, (size_t)kf_smem(HD), g_llb.stream, c, rw, a, p, km, vm));
+    CU_OK(llb_launch(k_kv_join<T, HD, false>, dim3(joins), dim3(128), (size_t)0, g_llb.stream, c, rw, a, p, joins, 0));
+  }
+  return 0;
+}
+template <typename T, int HD> static int attn_go(const llb_kv *kv, const llb_kv_attn *call, const KvDev &c, const KvRows &rw, const KvAttn &a) {
+  if (attn_few(kv, call)) return few_go<T, HD>(kv, call, c, rw, a);
+  CU_OK(llb_launch(k_kv_attn_row<T, HD>, dim3(rw.rows, (a.H + 3) / 4), dim3(128), (size_t)0, g_llb.stream, c, rw, a));
   return 0;
 }
 
@@ -401,6 +338,8 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   if (a->out_stride < row || a->out_stride % (a->el_out == LLB_EL_F32 ? 4 : 8)) return llb_fail("kv_attn: out_stride %lld for rows of %lld", a->out_stride, row);
   if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");
   if (a->w_in && !a->w_out) return llb_fail("kv_attn: w_in without w_out");
+  if ((long long)kv->seqs * kv->kv_heads * ((long long)a->heads / kv->kv_heads * std::min(a->max_rows, 64) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
+    return llb_fail("kv_attn: %d sequences of %d kv heads, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, a->max_len);
   if (a->w_out) {
     if (off(a->w_in, 4) || off(a->w_out, 4)) return llb_fail("kv_attn: weights are f32 on the device");
     if (a->w_stride < a->max_len) return llb_fail("kv_attn: w_stride %d for %d slots", a->w_stride, a->max_len);
@@ -409,10 +348,8 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   return 0;
 }
 static size_t attn_ws(const llb_kv *kv, const llb_kv_attn *a) {
-  (void)kv;
-  size_t n = 16;
-  if (a->w_out) n += (size_t)a->rows * a->heads * 4;
-  return n;
+  KvPlan p;
+  return attn_few(kv, a) ? few_plan(kv, a, 0, &p) : 16;
 }
 static int evict_check(const llb_kv *src, const llb_kv_evict *e) {
   if (kv_check(src, "kv_evict")) return -1;
@@ -498,12 +435,11 @@ int llb_b200_kv_attn(const llb_kv *kv, const llb_kv_attn *a) {
   const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, a->max_rows};
   KvAttn k;
   k.q = (const uint16_t *)(uintptr_t)a->q; k.out = (void *)(uintptr_t)a->out;
-  k.qs = a->q_stride; k.os = a->out_stride; k.H = a->heads; k.window = a->window; k.sinks = a->sinks; k.out32 = a->el_out == LLB_EL_F32;
+  k.qs = a->q_stride; k.os = a->out_stride; k.H = a->heads; k.G = a->heads / kv->kv_heads; k.window = a->window; k.sinks = a->sinks; k.out32 = a->el_out == LLB_EL_F32;
   k.scale2 = (float)((a->scale > 0.0f ? (double)a->scale : 1.0 / sqrt((double)kv->head_dim)) * 1.4426950408889634);
   k.w_in = (const float *)(uintptr_t)a->w_in; k.w_out = (float *)(uintptr_t)a->w_out; k.wstride = a->w_stride;
-  k.lse = a->w_out ? (float *)(uintptr_t)a->ws : nullptr;
-  if (kv->el == LLB_EL_F16) return kv->head_dim == 64 ? attn_go<__half, 64>(c, rw, k) : kv->head_dim == 128 ? attn_go<__half, 128>(c, rw, k) : attn_go<__half, 256>(c, rw, k);
-  return kv->head_dim == 64 ? attn_go<__nv_bfloat16, 64>(c, rw, k) : kv->head_dim == 128 ? attn_go<__nv_bfloat16, 128>(c, rw, k) : attn_go<__nv_bfloat16, 256>(c, rw, k);
+  if (kv->el == LLB_EL_F16) return kv->head_dim == 64 ? attn_go<__half, 64>(kv, a, c, rw, k) : kv->head_dim == 128 ? attn_go<__half, 128>(kv, a, c, rw, k) : attn_go<__half, 256>(kv, a, c, rw, k);
+  return kv->head_dim == 64 ? attn_go<__nv_bfloat16, 64>(kv, a, c, rw, k) : kv->head_dim == 128 ? attn_go<__nv_bfloat16, 128>(kv, a, c, rw, k) : attn_go<__nv_bfloat16, 256>(kv, a, c, rw, k);
 }
 
 size_t llb_b200_kv_evict_ws(const llb_kv *src, const llb_kv_evict *e) { return evict_check(src, e) ? 0 : evict_ws(src, e); }

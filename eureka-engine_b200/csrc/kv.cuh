@@ -82,3 +82,135 @@ __device__ __forceinline__ void kv_check_rows(const KvDev &c, const KvRows &r) {
 // what the row at slot e sees
 __device__ __forceinline__ bool kv_sees(int j, int e, int window, int sinks) { return j <= e && (!window || j > e - window || j < sinks); }
 __device__ __forceinline__ int kv_first(int e, int window) { return window && e >= window ? e - window + 1 : 0; }   // first slot of its window
+
+// ---- a call's attention ----------------------------------------------------------------------------
+struct KvAttn {
+  const uint16_t *q;
+  void *out;
+  long long qs, os;            // elements between rows
+  int H, G, window, sinks, out32;   // G: query heads a kv head
+  float scale2;                // times log2(e): probabilities are powers of two
+  const float *w_in;
+  float *w_out;
+  int wstride;
+};
+// one sequence's share of a call.  What its rows see is cut into chunks of `1 << sh` slots: cs of first tokens, then those from slot lo's on.
+struct KvSeq {
+  int first, n, len;           // first row, rows; slots
+  int nc;                      // rows that are computed: max_rows at most
+  int e0;                      // slot of the first row
+  int lo, cs, chunks;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvDev &c, const KvRows &r, int b, int window, int sinks, int sh) {
+  KvSeq s;
+  s.n = kv_rows(c, r, b, s.first);
+  s.len = kv_len(c, b);
+  s.nc = min(s.n, r.max_rows);
+  if (s.n > r.max_rows) atomicOr(c.err, KV_ERR_ROWS);
+  s.e0 = s.len - s.n;
+  const int last = s.e0 + s.nc - 1;
+  s.lo = kv_first(max(s.e0, 0), window);
+  s.cs = min((min(sinks, s.lo) + (1 << sh) - 1) >> sh, s.lo >> sh);
+  s.chunks = !s.nc ? 0 : last < 0 ? 1 : s.cs + (last >> sh) - (s.lo >> sh) + 1;   // (rows that see nothing: one chunk with nothing in it)
+  return s;
+}
+__device__ __forceinline__ int kv_chunk_slot(const KvSeq &s, int ch, int sh) { return (ch < s.cs ? ch : (s.lo >> sh) + ch - s.cs) << sh; }
+// whether some row of the sequence sees slot j
+__device__ __forceinline__ bool kv_any_sees(const KvSeq &s, int j, int window, int sinks) {
+  return j <= s.e0 + s.nc - 1 && (!window || j > s.e0 - window || j < sinks);
+}
+
+template <typename X, int E> __device__ __forceinline__ void kv_row_in(const X *p, bool wide, float (&x)[E]) {
+  if constexpr (sizeof(X) == 4) {
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) { const float2 f = __ldcg((const float2 *)(p + i)); x[i] = f.x; x[i + 1] = f.y; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i++) x[i] = __ldcg((const float *)p + i);
+    }
+  } else {
+    if (wide) {
+      uint32_t w[E / 2];
+      if constexpr (E == 2) w[0] = __ldcg((const uint32_t *)p);
+      else if constexpr (E == 4) { const uint2 t = __ldcg((const uint2 *)p); w[0] = t.x; w[1] = t.y; }
+      else { const uint4 t = __ldcg((const uint4 *)p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
+#pragma unroll
+      for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<X>::to2(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i++) x[i] = KvEl<X>::to(__ldcg((const uint16_t *)p + i));
+    }
+  }
+}
+template <typename T, int E> __device__ __forceinline__ void kv_row_out(uint16_t *p, bool wide, const float (&x)[E]) {
+  if (wide) {
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) w[i] = KvEl<T>::of2(x[2 * i], x[2 * i + 1]);
+    if constexpr (E == 2) *(uint32_t *)p = w[0];
+    else if constexpr (E == 4) *(uint2 *)p = make_uint2(w[0], w[1]);
+    else *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++) p[i] = KvEl<T>::of(x[i]);
+  }
+}
+__device__ __forceinline__ float kv_warp_sum(float v) {
+#pragma unroll
+  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+// The row at slot e and head h over the slots that it sees, one after the other, by a warp; lane's dimensions E lane ..
+// The attention kernels take a row to it whose result is no number: their products multiply V by a probability of zero where a row
+// does not see a slot that another one does, which is NaN where that slot holds an infinity or NaN.
+template <typename T, int HD>
+__device__ __noinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float *o, float &m, float &l) {
+  constexpr int E = HD / 32;
+  const int g = h / a.G, pm = (1 << c.page_sh) - 1;
+  float q[E];
+  kv_row_in<T, E>((const T *)a.q + r * a.qs + (long long)h * HD + lane * E, true, q);
+#pragma unroll
+  for (int i = 0; i < E; i++) { q[i] *= a.scale2; o[i] = 0.0f; }
+  m = -INFINITY; l = 0.0f;
+  const int lo = kv_first(e, a.window), ns = min(a.sinks, lo);
+  int id = -1, at = -1;
+#pragma unroll 1
+  for (int n = 0; n < ns + e + 1 - lo; n++) {
+    const int j = n < ns ? n : lo + n - ns;
+    if (j >> c.page_sh != at) { at = j >> c.page_sh; id = kv_page(c, b, at); }
+    if (id < 0) continue;
+    const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + lane * E;
+    float k[E], v[E];
+    kv_row_in<T, E>((const T *)c.k + p, true, k);
+    kv_row_in<T, E>((const T *)c.v + p, true, v);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; i++) s += q[i] * k[i];
+    s = kv_warp_sum(s);
+    const float mn = fmaxf(m, s), cf = m == -INFINITY ? 0.0f : exp2f(m - mn), w = s == -INFINITY ? 0.0f : exp2f(s - mn);
+    l = l * cf + w;
+    // (0 times an infinity is no number either: a slot that is seen and whose probability is 0 counts as in the definition, exp(s) V)
+#pragma unroll
+    for (int i = 0; i < E; i++) o[i] = o[i] * cf + w * v[i];
+    m = mn;
+  }
+}
+// A row's result from its sums (base 2: m the maximum that l and o are relative to), by a warp
+template <typename T, int HD>
+__device__ __forceinline__ void kv_finish(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float (&o)[HD / 32], float m, float l) {
+  constexpr int E = HD / 32;
+  float x = l;
+#pragma unroll
+  for (int i = 0; i < E; i++) x += o[i] * 0.0f;
+  if (__any_sync(0xffffffffu, !(fabsf(x) < INFINITY))) kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (nothing seen: zeros)
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] *= inv;
+  const long long at = r * a.os + (long long)h * HD + lane * E;
+  if (a.out32) {
+    float *p = (float *)a.out + at;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) *(float2 *)(p + i) = make_float2(o[i], o[i + 1]);
+  } else kv_row_out<T, E>((uint16_t *)a.out + at, true, o);
+}

@@ -1,0 +1,450 @@
+// kvatt.cuh -- attention of the few rows of a decode or verify step over the paged cache: bound by the cache's bytes.
+//
+// A unit is (sequence, kv head, 16 queries); its queries are the rows' heads side by side, query i G + h is row i, head h of the kv head's
+// G.  What a unit sees is cut into chunks of 16 slots, a page's part each, and the chunks of all units, one after the other, into as many
+// equal stretches as there are blocks, so that sequences of any lengths keep every SM busy to the end; a block's stretch may begin and end inside a unit.  The four warps of a
+// block take its chunks in turn, each with a ring of stages of its own that TMA fills (rows of 128 swizzled bytes) and that runs ahead over
+// the ends of units: no barrier between warps but where a unit ends and their sums are joined.
+//   S[query][slot] = Q K^T      m16n8k16, 16 queries x 16 slots
+//   O[query][dim] += P V        P from the registers of S, rounded to the cache's type (the second product takes 16-bit operands)
+// with the maximum and the sum of every query kept in f32.  A unit that one block has wholly is finished there; the others' sums go to the workspace,
+// and k_kv_join, the second launch, puts them together in the order of the blocks.
+#pragma once
+#include <cuda.h>
+
+#include "kv.cuh"
+#include "tc5.cuh"
+
+#define KF_WARPS 4
+#define KF_SLOTS 16
+#define KF_SH 4
+__host__ __device__ constexpr int kf_stages(int HD) { return HD == 64 ? 5 : HD == 128 ? 3 : 3; }
+__host__ __device__ constexpr int kf_stage_bytes(int HD) { return 2 * KF_SLOTS * HD * 2; }       // K, then V
+__host__ __device__ constexpr int kf_ring(int HD) { return KF_WARPS * kf_stages(HD) * kf_stage_bytes(HD); }
+__host__ __device__ constexpr int kf_row(int HD) { return HD + 8; }                              // floats of a row of a warp's sums
+__host__ __device__ constexpr int kf_sums(int HD) { return HD == 64 ? 2 : 1; }                  // sums of so many warps have room
+__host__ __device__ constexpr int kf_smem(int HD) { return 1024 + kf_ring(HD) + kf_sums(HD) * 16 * kf_row(HD) * 4 + 16 * HD * 2; }
+static_assert(kf_smem(256) <= 232448 && 2 * (kf_smem(128) + 1024) <= 233472 && 2 * (kf_smem(64) + 1024) <= 233472, "one block an SM, or two");
+struct KfHead {                // before the rings
+  uint64_t full[KF_WARPS][5];
+  long long sum[KF_WARPS], rem;
+  int b, bad[KF_WARPS][5];
+  float m[2][16], l[2][16];
+};
+static_assert(sizeof(KfHead) <= 1024, "the rings begin 1024 bytes on");
+
+struct KvPlan {
+  int least;                   // chunks of a block's stretch, at least
+  long long *before;           // [seqs + 2]: chunks of the sequences before; all; chunks of a stretch
+  float *pm, *pl, *po;         // [2 blocks][16](, [hd])
+  float *sc;                   // [seqs][KV][G max_rows][sstride]: scores, where weights are wanted
+  float *lse;                  // [seqs][KV][G max_rows]: of units that one block has wholly
+  int sstride;
+  unsigned int *err;           // a wait ran out
+};
+
+template <typename T> __device__ __forceinline__ void kf_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void kf_mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma16816(d, a[0], a[1], a[2], a[3], b0, b1); }
+template <> __device__ __forceinline__ void kf_mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void kf_ldsm(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void kf_ldsm_t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ float kv_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ void kv_tma(uint32_t dst_s, const CUtensorMap *map, int x, int slot, int g, int page, uint32_t bar_s) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst_s), "l"(map), "r"(x), "r"(slot),
+               "r"(g), "r"(page), "r"(bar_s)
+               : "memory");
+}
+__device__ __forceinline__ void kv_expect(uint32_t bar_s, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_s), "r"(bytes) : "memory");
+}
+
+// a block's way through its stretch: the unit it is in, and the chunks c0 .. c1 - 1 of it that are the block's
+struct KfWalk {
+  KvSeq s;
+  int b, g, qt, c0, c1;
+  long long left;              // chunks of the stretch behind this unit's
+  __device__ __forceinline__ void take() {
+    c1 = (int)min((long long)s.chunks, c0 + left);
+    left -= c1 - c0;
+  }
+  __device__ __forceinline__ bool next(const KvDev &c, const KvRows &r, const KvAttn &a) {
+    if (left <= 0) return false;
+    c0 = 0;
+    if (++qt >= (a.G * s.nc + 15) >> 4) {
+      qt = 0;
+      if (++g == c.KV) {
+        g = 0;
+        do {
+          if (++b >= c.seqs) { left = 0; return false; }
+          s = kv_seq(c, r, b, a.window, a.sinks, KF_SH);
+        } while (!s.chunks);
+      }
+    }
+    take();
+    return true;
+  }
+};
+
+template <typename T, int HD, bool WT>
+__global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
+                                                                             const __grid_constant__ CUtensorMap vm) {
+  constexpr int NS = kf_stages(HD), SB = kf_stage_bytes(HD), KB = SB / 2, ROW = kf_row(HD), E = HD / 32, NT = HD / 8, NB = kf_sums(HD);
+  static_assert(NS <= 5, "KfHead");
+  extern __shared__ __align__(1024) uint8_t smem[];
+  KfHead &hd = *(KfHead *)smem;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, j2 = 2 * (lane & 3), lr = lane & 7, mi = lane >> 3;
+  const uint32_t bar_s = smem_u32(smem), ring_s = bar_s + 1024 + warp * NS * SB;
+  float *sums = (float *)(smem + 1024 + kf_ring(HD));                    // [NB][16][ROW]
+  const uint32_t q_s = bar_s + 1024 + kf_ring(HD) + NB * 16 * ROW * 4;   // the unit's queries: a core matrix's rows of 16 bytes, [dims / 8][16]
+  uint8_t *q_m = smem + 1024 + kf_ring(HD) + NB * 16 * ROW * 4;
+  if (tid < KF_WARPS * 5) mbar_init(bar_s + 8 * tid, 1);
+  if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_trigger();
+  pdl_wait();
+  // ---- the block's stretch: chunks of every sequence, summed over the threads' runs of sequences ----
+  const int run = (c.seqs + 32 * KF_WARPS - 1) / (32 * KF_WARPS), ba = min(c.seqs, tid * run), bz = min(c.seqs, ba + run);
+  auto work = [&](int b) {
+    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
+    return (long long)s.chunks * c.KV * ((a.G * s.nc + 15) >> 4);
+  };
+  long long mine = 0;
+#pragma unroll 1
+  for (int b = ba; b < bz; b++) mine += work(b);
+  long long to = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) { const long long o = __shfl_up_sync(0xffffffffu, to, m); if (lane >= m) to += o; }
+  if (lane == 31) hd.sum[warp] = to;
+  __syncthreads();
+  long long all = 0;
+#pragma unroll
+  for (int w = 0; w < KF_WARPS; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
+  const long long per = max((long long)p.least, (all + gridDim.x - 1) / gridDim.x), start = per * blockIdx.x;
+  if (blockIdx.x == 0) {
+    long long at = to - mine;
+#pragma unroll 1
+    for (int b = ba; b < bz; b++) { p.before[b] = at; at += work(b); }
+    if (tid == 0) { p.before[c.seqs] = all; p.before[c.seqs + 1] = per; }
+  }
+  if (start >= all) return;
+  if (to - mine <= start && start < to) {
+    long long at = to - mine;
+    int b = ba;
+#pragma unroll 1
+    for (;; b++) { const long long w = work(b); if (start < at + w) break; at += w; }
+    hd.b = b; hd.rem = start - at;
+  }
+  __syncthreads();
+  KfWalk use;
+  use.b = hd.b;
+  use.s = kv_seq(c, rw, use.b, a.window, a.sinks, KF_SH);
+  {
+    const int qts = (a.G * use.s.nc + 15) >> 4, u = (int)(hd.rem / use.s.chunks);
+    use.g = u / qts; use.qt = u % qts; use.c0 = (int)(hd.rem % use.s.chunks);
+    use.left = min(per, all - start);
+    use.take();
+  }
+  // ---- the warp's requests: a chunk behind the other, over the ends of units ----
+  KfWalk get = use;
+  int gch = use.c0 + warp, gid_page = -1, issued = 0;
+  bool more = true, dead = false;
+  auto find = [&]() {          // the page of the next chunk, or that there is none
+    while (gch >= get.c1) {
+      if (!get.next(c, rw, a)) { more = false; return; }
+      gch = get.c0 + warp;
+    }
+    const int slot = kv_chunk_slot(get.s, gch, KF_SH);
+    gid_page = get.s.e0 + get.s.nc > 0 ? __ldcg(c.table + (size_t)get.b * c.tstride + (slot >> c.page_sh)) : -1;
+  };
+  auto issue = [&]() {
+    if (!more) return;
+    const int st = issued % NS, slot = kv_chunk_slot(get.s, gch, KF_SH);
+    const uint32_t full = bar_s + 8 * (warp * 5 + st);
+    const bool in = (unsigned)gid_page < (unsigned)c.n_pages;
+    if (lane == 0) {
+      hd.bad[warp][st] = !in;
+      if (in) {
+        kv_expect(full, SB);
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) {
+          kv_tma(ring_s + st * SB + d * (KF_SLOTS * 128), &km, 64 * d, slot & ((1 << c.page_sh) - 1), get.g, gid_page, full);
+          kv_tma(ring_s + st * SB + KB + d * (KF_SLOTS * 128), &vm, 64 * d, slot & ((1 << c.page_sh) - 1), get.g, gid_page, full);
+        }
+      } else {
+        if (get.s.e0 + get.s.nc > 0) atomicOr(c.err, KV_ERR_PAGE);
+        mbar_arrive(full);
+      }
+    }
+    issued++;
+    gch += KF_WARPS;
+    find();
+  };
+  find();
+#pragma unroll 1
+  for (int i = 0; i < NS; i++) issue();
+  int done = 0;
+#pragma unroll 1
+  for (;;) {
+    const KvSeq &s = use.s;
+    const int NQ = a.G * s.nc, q0 = 16 * use.qt, last = s.e0 + s.nc - 1;
+    // the queries: rows of 16 bytes, [dims / 8][query]
+    for (int i = tid; i < 16 * NT; i += 32 * KF_WARPS) {
+      const int qi = q0 + (i & 15), d = i >> 4;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (qi < NQ) v = __ldcg((const uint4 *)(a.q + (long long)(s.first + qi / a.G) * a.qs + (long long)(use.g * a.G + qi % a.G) * HD + 8 * d));
+      *(uint4 *)(q_m + i * 16) = v;
+    }
+    __syncthreads();
+    float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[i][k] = 0.0f;
+    // the slots that the thread's two queries see: from lw to e, and below the first tokens' end
+    int e[2], lw[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int qi = q0 + gid + 8 * k;
+      e[k] = qi < NQ ? s.e0 + qi / a.G : -1;
+      lw[k] = a.window ? e[k] - a.window + 1 : 0;
+    }
+    const int ea = s.e0 + q0 / a.G, ez = s.e0 + min(q0 + 15, NQ - 1) / a.G;      // slots of the unit's first and last row
+#pragma unroll 1
+    for (int ch = use.c0 + warp; ch < use.c1; ch += KF_WARPS, done++) {
+      const int st = done % NS, slot = kv_chunk_slot(s, ch, KF_SH);
+      const uint32_t k_s = ring_s + st * SB, v_s = k_s + KB;
+      if (!dead && !mbar_wait(bar_s + 8 * (warp * 5 + st), (uint32_t)(done / NS) & 1u)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
+      const bool none = hd.bad[warp][st] || dead;
+      float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      if (!none) {
+        // slots that no row sees: their V is taken out, whatever it holds (0 times NaN is NaN)
+        if (slot + 15 > last || (a.window && slot <= s.e0 - a.window && slot + 15 >= a.sinks)) {
+          for (int i = lane; i < KF_SLOTS * NT; i += 32) {
+            const int r = i & 15;
+            if (!kv_any_sees(s, slot + r, a.window, a.sinks)) *(uint4 *)(smem + (v_s - bar_s) + (i >> 7) * (KF_SLOTS * 128) + r * 128 + ((i >> 4) & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ks++) {
+          uint32_t qa[4], kb[4];
+          // queries: matrix mi has queries 8 (mi & 1) .., dims 8 (2 ks + mi / 2) ..; keys: slots 8 (mi / 2) .., dims 8 (2 ks + (mi & 1)) ..
+          kf_ldsm(qa, q_s + (2 * ks + (mi >> 1)) * 256 + (lr + 8 * (mi & 1)) * 16);
+          const int unit = 2 * ks + (mi & 1), row = lr + 8 * (mi >> 1);
+          kf_ldsm(kb, k_s + (unit >> 3) * (KF_SLOTS * 128) + row * 128 + (((unit & 7) ^ lr) << 4));
+          kf_mma<T>(x[0], qa, kb[0], kb[1]);
+          kf_mma<T>(x[1], qa, kb[2], kb[3]);
+        }
+      }
+      const bool whole = !none && slot + 15 <= ea && (!a.window || slot > ez - a.window || slot + 15 < a.sinks) && q0 + 15 < NQ;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int j = slot + 8 * t + j2 + (k & 1), w = k >> 1;
+          x[t][k] *= a.scale2;
+          if (!whole && (none || j > e[w] || (j < lw[w] && j >= a.sinks))) x[t][k] = -INFINITY;
+        }
+      if constexpr (WT) {
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+          if (q0 + gid + 8 * w < NQ) {
+            float *d = p.sc + (((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + gid + 8 * w) * p.sstride + slot + j2;
+            *(float2 *)d = make_float2(x[0][2 * w], x[0][2 * w + 1]);
+            *(float2 *)(d + 8) = make_float2(x[1][2 * w], x[1][2 * w + 1]);
+          }
+      }
+      float cf[2];
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        float t = fmaxf(fmaxf(x[0][2 * w], x[0][2 * w + 1]), fmaxf(x[1][2 * w], x[1][2 * w + 1]));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        t = fmaxf(t, m[w]);
+        const float ref = t == -INFINITY ? 0.0f : t;      // (nothing seen yet: every probability is 0)
+        cf[w] = kv_exp2(m[w] - ref);
+        m[w] = t;
+#pragma unroll
+        for (int k = 0; k < 2; k++) { x[0][2 * w + k] = kv_exp2(x[0][2 * w + k] - ref); x[1][2 * w + k] = kv_exp2(x[1][2 * w + k] - ref); }
+        l[w] = l[w] * cf[w] + ((x[0][2 * w] + x[0][2 * w + 1]) + (x[1][2 * w] + x[1][2 * w + 1]));
+      }
+      if (!none) {
+        if (__any_sync(0xffffffffu, cf[0] != 1.0f || cf[1] != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < NT; i++) { o[i][0] *= cf[0]; o[i][1] *= cf[0]; o[i][2] *= cf[1]; o[i][3] *= cf[1]; }
+        }
+        const uint32_t pa[4] = {KvEl<T>::of2(x[0][0], x[0][1]), KvEl<T>::of2(x[0][2], x[0][3]), KvEl<T>::of2(x[1][0], x[1][1]), KvEl<T>::of2(x[1][2], x[1][3])};
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {
+          uint32_t vb[4];                                  // matrix mi: slots 8 (mi & 1) .., dims 8 (i + mi / 2) ..
+          const int unit = i + (mi >> 1), row = lr + 8 * (mi & 1);
+          kf_ldsm_t(vb, v_s + (unit >> 3) * (KF_SLOTS * 128) + row * 128 + (((unit & 7) ^ lr) << 4));
+          kf_mma<T>(o[i], pa, vb[0], vb[1]);
+          kf_mma<T>(o[i + 1], pa, vb[2], vb[3]);
+        }
+      }
+      __syncwarp();                                        // the stage has been read
+      if (!dead) issue();
+    }
+    // ---- the warps' sums put together: a tree where two have room (2 and 3 to 0 and 1, 1 to 0), else 3, 2 and 1 to 0 ----
+#pragma unroll
+    for (int w = 0; w < 2; w++) { l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1); l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2); }
+    auto leave = [&](int at) {
+      float *d = sums + at * 16 * ROW;
+#pragma unroll
+      for (int i = 0; i < NT; i++) {
+        *(float2 *)(d + gid * ROW + 8 * i + j2) = make_float2(o[i][0], o[i][1]);
+        *(float2 *)(d + (gid + 8) * ROW + 8 * i + j2) = make_float2(o[i][2], o[i][3]);
+      }
+      if (j2 == 0) { hd.m[at][gid] = m[0]; hd.m[at][gid + 8] = m[1]; hd.l[at][gid] = l[0]; hd.l[at][gid + 8] = l[1]; }
+    };
+    auto add = [&](int at) {
+      const float *d = sums + at * 16 * ROW;
+      float fa[2], fb[2];
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        const float mb = hd.m[at][gid + 8 * w], t = fmaxf(m[w], mb), ref = t == -INFINITY ? 0.0f : t;
+        fa[w] = kv_exp2(m[w] - ref); fb[w] = kv_exp2(mb - ref);
+        l[w] = l[w] * fa[w] + hd.l[at][gid + 8 * w] * fb[w];
+        m[w] = t;
+      }
+#pragma unroll
+      for (int i = 0; i < NT; i++) {
+        const float2 u = *(const float2 *)(d + gid * ROW + 8 * i + j2), v = *(const float2 *)(d + (gid + 8) * ROW + 8 * i + j2);
+        o[i][0] = o[i][0] * fa[0] + u.x * fb[0]; o[i][1] = o[i][1] * fa[0] + u.y * fb[0];
+        o[i][2] = o[i][2] * fa[1] + v.x * fb[1]; o[i][3] = o[i][3] * fa[1] + v.y * fb[1];
+      }
+    };
+    const int used = min(KF_WARPS, use.c1 - use.c0);       // warps that had a chunk
+#pragma unroll 1
+    for (int src = KF_WARPS - 1; src > 0; src = NB == 2 ? src >> 1 : src - 1) {   // NB 2: 3 (with 2), then 1
+      if (NB == 2 ? src == 3 && used < 3 : src >= used) continue;
+      if (src == 1 && used < 2) continue;
+      if (NB == 2 && src == 3) { if (warp >= 2) leave(warp - 2); }
+      else if (warp == src) leave(0);
+      __syncthreads();
+      if (NB == 2 && src == 3) { if (warp < 2) add(warp); }
+      else if (warp == 0) add(0);
+      __syncthreads();
+    }
+    if (warp == 0) leave(0);
+    __syncthreads();
+    const bool wholly = use.c0 == 0 && use.c1 == s.chunks;
+    const size_t part = ((size_t)blockIdx.x * 2 + (use.c0 == 0)) * 16;
+#pragma unroll 1
+    for (int r = warp; r < 16 && q0 + r < NQ; r += KF_WARPS) {
+      float v[E];
+#pragma unroll
+      for (int k = 0; k < E; k++) v[k] = sums[r * ROW + lane * E + k];
+      const int row = (q0 + r) / a.G, h = use.g * a.G + (q0 + r) % a.G;
+      if (wholly) {
+        if (WT && lane == 0) p.lse[((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + r] = hd.l[0][r] > 0.0f ? hd.m[0][r] + log2f(hd.l[0][r]) : INFINITY;
+        kv_finish<T, HD>(c, a, use.b, s.first + row, h, s.e0 + row, lane, v, hd.m[0][r], hd.l[0][r]);
+      } else {
+        if (lane == 0) { p.pm[part + r] = hd.m[0][r]; p.pl[part + r] = hd.l[0][r]; }
+#pragma unroll
+        for (int k = 0; k < E; k += 2) *(float2 *)(p.po + (part + r) * HD + lane * E + k) = make_float2(v[k], v[k + 1]);
+      }
+    }
+    if (!use.next(c, rw, a)) break;
+    __syncthreads();                                       // (the queries' and sums' memory is free again)
+  }
+  if (dead) for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies may be on their way
+}
+
+// blocks that have a part of the unit that begins `at` chunks into the call: first, last
+__device__ __forceinline__ void kf_parts(const KvPlan &p, long long at, int chunks, long long per, int &w0, int &w1) {
+  w0 = (int)(at / per); w1 = (int)((at + chunks - 1) / per);
+}
+__device__ __forceinline__ size_t kf_part(long long at, long long per, int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }   // (only the first begins with the unit's first chunk)
+
+// Units that several blocks had: a block a query, its four warps the parts in turn.  Blocks from `joins` on: what every slot got, 512 slots of a kv head each.
+template <typename T, int HD, bool WT>
+__global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
+  constexpr int E = HD / 32;
+  __shared__ float sm[4], sl[4], so[4][HD], lse[64];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NQM = a.G * rw.max_rows;
+  const long long per = __ldcg(p.before + c.seqs + 1);
+  if (!WT || blockIdx.x < joins) {
+    const int qi = blockIdx.x % NQM, g = blockIdx.x / NQM % c.KV, b = blockIdx.x / NQM / c.KV;
+    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
+    if (qi >= a.G * s.nc) return;
+    const int qts = (a.G * s.nc + 15) >> 4;
+    int w0, w1;
+    const long long at = __ldcg(p.before + b) + ((long long)g * qts + (qi >> 4)) * s.chunks;
+    kf_parts(p, at, s.chunks, per, w0, w1);
+    if (w0 == w1) return;
+    float M = -INFINITY;
+    for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, __ldcg(p.pm + kf_part(at, per, w, w0) + (qi & 15)));
+#pragma unroll
+    for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float o[E], l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; k++) o[k] = 0.0f;
+#pragma unroll 4
+    for (int w = w0 + warp; w <= w1; w += 4) {
+      const size_t i = kf_part(at, per, w, w0) + (qi & 15);
+      const float f = exp2f(__ldcg(p.pm + i) - ref);
+      l += __ldcg(p.pl + i) * f;
+#pragma unroll
+      for (int k = 0; k < E; k += 2) { const float2 v = __ldcg((const float2 *)(p.po + i * HD + lane * E + k)); o[k] += v.x * f; o[k + 1] += v.y * f; }
+    }
+    if (lane == 0) sl[warp] = l;
+#pragma unroll
+    for (int k = 0; k < E; k++) so[warp][lane * E + k] = o[k];
+    __syncthreads();
+    if (warp) return;
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+#pragma unroll
+    for (int k = 0; k < E; k++) o[k] = (so[0][lane * E + k] + so[1][lane * E + k]) + (so[2][lane * E + k] + so[3][lane * E + k]);
+    const int row = qi / a.G;
+    kv_finish<T, HD>(c, a, b, s.first + row, g * a.G + qi % a.G, s.e0 + row, lane, o, M, l);
+    return;
+  }
+  if constexpr (WT) {
+    const int u = blockIdx.x - joins, wb = u % wblocks, g = u / wblocks % c.KV, b = u / wblocks / c.KV;
+    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
+    if (wb * 512 >= s.len) return;
+    const int qts = (a.G * s.nc + 15) >> 4, NQ = a.G * s.nc;
+    const size_t ug = (size_t)b * c.KV + g;
+    if (tid < NQ) {
+      int w0, w1;
+      const long long at = __ldcg(p.before + b) + ((long long)g * qts + (tid >> 4)) * s.chunks;
+      kf_parts(p, at, s.chunks, per, w0, w1);
+      if (w0 == w1) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
+      else {
+        float M = -INFINITY, l = 0.0f;
+#pragma unroll 4
+        for (int w = w0; w <= w1; w++) M = fmaxf(M, __ldcg(p.pm + kf_part(at, per, w, w0) + (tid & 15)));
+        const float ref = M == -INFINITY ? 0.0f : M;
+#pragma unroll 4
+        for (int w = w0; w <= w1; w++) { const size_t i = kf_part(at, per, w, w0) + (tid & 15); l += __ldcg(p.pl + i) * exp2f(__ldcg(p.pm + i) - ref); }
+        lse[tid] = l > 0.0f ? M + log2f(l) : INFINITY;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int j = wb * 512 + k * 128 + tid;
+      if (j >= s.len) return;
+      float sum = 0.0f;
+      if (NQ && kv_any_sees(s, j, a.window, a.sinks)) {
+        const float *x = p.sc + ug * NQM * p.sstride + j;
+#pragma unroll 4
+        for (int q = 0; q < NQ; q++) sum += exp2f(__ldcg(x + (size_t)q * p.sstride) - lse[q]);
+      }
+      a.w_out[ug * a.wstride + j] = (a.w_in ? __ldcg(a.w_in + ug * a.wstride + j) : 0.0f) + sum;
+    }
+  }
+}
