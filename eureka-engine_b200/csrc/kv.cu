@@ -7,6 +7,7 @@
 #include "host.cuh"
 #include "kv.cuh"
 #include "kvatt.cuh"
+#include "kvpf.cuh"
 
 static unsigned int *g_kv_err = nullptr;   // what the kernels met (KV_ERR_*)
 static decltype(&cuTensorMapEncodeTiled) g_kv_map = nullptr;
@@ -82,23 +83,6 @@ __global__ void __launch_bounds__(256) k_kv_append(const KvDev c, const KvRows r
   const int id = kv_page(c, b, slot >> c.page_sh);
   if (id < 0) return;
   kv_row_out<T, E>((isv ? c.v : c.k) + kv_at(c, id, g, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD + lane * E, true, x);
-}
-
-// ---- attention, a warp a head of a row ------------------------------------------------------------
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) k_kv_attn_row(const KvDev c, const KvRows rw, const KvAttn a) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), r = blockIdx.x;
-  const int b = kv_find(rw, c.seqs, r, lane);
-  if (!blockIdx.x && !blockIdx.y) kv_check_rows(c, rw);
-  if (b < 0 || h >= a.H) return;
-  int first;
-  const int n = kv_rows(c, rw, b, first), e = kv_len(c, b) - n + r - first;
-  if (r - first >= rw.max_rows) return;
-  float o[HD / 32], m, l;
-  kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
-  kv_finish<T, HD>(c, a, b, r, h, e, lane, o, m, l);
 }
 
 // ---- eviction -------------------------------------------------------------------------------------
@@ -199,6 +183,7 @@ __global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, c
 // ---- host -----------------------------------------------------------------------------------------
 template <typename T, int HD> static int few_attr() {
   CU_OK(cudaFuncSetAttribute(k_kv_few<T, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kf_smem(HD)));
+  CU_OK(cudaFuncSetAttribute(k_kv_pf<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kp<HD>::SMEM));
   CU_OK(cudaFuncSetAttribute(k_kv_few<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kf_smem(HD)));
   return 0;
 }
@@ -281,11 +266,12 @@ static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int 
 // ---- which kernel, and its workspace ----
 #define KV_FEW 64              // queries a kv head up to which a call goes to k_kv_few
 #define KF_LEAST 8             // fewest chunks of a block's stretch: two a warp
-static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * a->max_rows <= KV_FEW; }
+static int most_rows(const llb_kv_attn *a) { return std::min(a->max_rows, std::max(a->rows, 1)); }
+static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * most_rows(a) <= KV_FEW; }
 static int few_grid(const llb_kv *kv) { return (g_llb.sms ? g_llb.sms : 148) * (kv->head_dim == 256 ? 1 : 2); }
 // its parts, one behind the other; the size where `base` is 0
 static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, KvPlan *p) {
-  const size_t blocks = few_grid(kv), queries = (size_t)kv->seqs * kv->kv_heads * (a->heads / kv->kv_heads) * a->max_rows;
+  const size_t blocks = few_grid(kv), queries = (size_t)kv->seqs * a->heads * most_rows(a);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
   p->least = KF_LEAST;
@@ -315,9 +301,33 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   }
   return 0;
 }
+// many rows: query tiles of the longest sequence's rows, and how many blocks share a tile's slots where there are fewer units than SMs
+static int pf_queries(const llb_kv *kv) { return kv->head_dim == 256 ? 128 : 256; }
+static int pf_tiles(const llb_kv *kv, const llb_kv_attn *a) {
+  return (int)(((long long)a->heads / kv->kv_heads * most_rows(a) + pf_queries(kv) - 1) / pf_queries(kv));
+}
+static size_t pf_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, KvPfPlan *p) {
+  const long long sms = g_llb.sms ? g_llb.sms : 148, units = (long long)pf_tiles(kv, a) * kv->kv_heads * kv->seqs;
+  const int slots = a->window ? (int)std::min((long long)a->max_len, (long long)a->window + a->sinks + most_rows(a)) : a->max_len;   // that a unit sees, at most
+  p->splits = (int)std::max(1LL, std::min(sms / std::max(units, 1LL), (long long)slots / 512));
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
+  const size_t parts = p->splits > 1 ? (size_t)kv->seqs * a->heads * most_rows(a) * p->splits : 0;
+  p->pm = (float *)take(parts * 4);
+  p->pl = (float *)take(parts * 4);
+  p->po = (float *)take(parts * 4 * kv->head_dim);
+  return std::max(at, (size_t)16);
+}
 template <typename T, int HD> static int attn_go(const llb_kv *kv, const llb_kv_attn *call, const KvDev &c, const KvRows &rw, const KvAttn &a) {
   if (attn_few(kv, call)) return few_go<T, HD>(kv, call, c, rw, a);
-  CU_OK(llb_launch(k_kv_attn_row<T, HD>, dim3(rw.rows, (a.H + 3) / 4), dim3(128), (size_t)0, g_llb.stream, c, rw, a));
+  KvPfPlan p;
+  pf_plan(kv, call, (uintptr_t)call->ws, &p);
+  p.err = gemm_err_word();
+  const int slots = std::min(kv->page, Kp<HD>::TILE), tiles = pf_tiles(kv, call);
+  CUtensorMap km, vm;
+  if (pool_map(&km, kv, kv->k, slots) || pool_map(&vm, kv, kv->v, slots)) return -1;
+  CU_OK(llb_launch(k_kv_pf<T, HD>, dim3(tiles * c.KV * c.seqs, p.splits), dim3(Kp<HD>::THREADS), (size_t)Kp<HD>::SMEM, g_llb.stream, c, rw, a, p, tiles, km, vm));
+  if (p.splits > 1) CU_OK(llb_launch(k_kv_pf_join<T, HD>, dim3(rw.rows, (a.H + 3) / 4), dim3(128), (size_t)0, g_llb.stream, c, rw, a, p));
   return 0;
 }
 
@@ -338,8 +348,9 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   if (a->out_stride < row || a->out_stride % (a->el_out == LLB_EL_F32 ? 4 : 8)) return llb_fail("kv_attn: out_stride %lld for rows of %lld", a->out_stride, row);
   if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");
   if (a->w_in && !a->w_out) return llb_fail("kv_attn: w_in without w_out");
-  if ((long long)kv->seqs * kv->kv_heads * ((long long)a->heads / kv->kv_heads * std::min(a->max_rows, 64) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
-    return llb_fail("kv_attn: %d sequences of %d kv heads, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, a->max_len);
+  const long long queries = (long long)a->heads / kv->kv_heads * most_rows(a), pairs = (long long)kv->seqs * kv->kv_heads;
+  if (queries > INT_MAX / 2 || pairs * (std::min(queries, (queries + 127) / 128 + KV_FEW) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
+    return llb_fail("kv_attn: %d sequences of %d kv heads, %d rows, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, most_rows(a), a->max_len);
   if (a->w_out) {
     if (off(a->w_in, 4) || off(a->w_out, 4)) return llb_fail("kv_attn: weights are f32 on the device");
     if (a->w_stride < a->max_len) return llb_fail("kv_attn: w_stride %d for %d slots", a->w_stride, a->max_len);
@@ -349,7 +360,8 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
 }
 static size_t attn_ws(const llb_kv *kv, const llb_kv_attn *a) {
   KvPlan p;
-  return attn_few(kv, a) ? few_plan(kv, a, 0, &p) : 16;
+  KvPfPlan f;
+  return attn_few(kv, a) ? few_plan(kv, a, 0, &p) : pf_plan(kv, a, 0, &f);
 }
 static int evict_check(const llb_kv *src, const llb_kv_evict *e) {
   if (kv_check(src, "kv_evict")) return -1;
@@ -432,7 +444,7 @@ int llb_b200_kv_attn(const llb_kv *kv, const llb_kv_attn *a) {
   KV_BEGIN;
   if (!a->rows && !a->w_out) return 0;
   const KvDev c = kv_dev(kv, a->max_len);
-  const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, a->max_rows};
+  const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, most_rows(a)};
   KvAttn k;
   k.q = (const uint16_t *)(uintptr_t)a->q; k.out = (void *)(uintptr_t)a->out;
   k.qs = a->q_stride; k.os = a->out_stride; k.H = a->heads; k.G = a->heads / kv->kv_heads; k.window = a->window; k.sinks = a->sinks; k.out32 = a->el_out == LLB_EL_F32;

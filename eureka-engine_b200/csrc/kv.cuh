@@ -196,14 +196,9 @@ __device__ __noinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b,
     m = mn;
   }
 }
-// A row's result from its sums (base 2: m the maximum that l and o are relative to), by a warp
-template <typename T, int HD>
-__device__ __forceinline__ void kv_finish(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float (&o)[HD / 32], float m, float l) {
+// a row's result, normalised, by a warp
+template <typename T, int HD> __device__ __forceinline__ void kv_store(const KvAttn &a, int r, int h, int lane, float (&o)[HD / 32], float l) {
   constexpr int E = HD / 32;
-  float x = l;
-#pragma unroll
-  for (int i = 0; i < E; i++) x += o[i] * 0.0f;
-  if (__any_sync(0xffffffffu, !(fabsf(x) < INFINITY))) kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (nothing seen: zeros)
 #pragma unroll
   for (int i = 0; i < E; i++) o[i] *= inv;
@@ -213,4 +208,13 @@ __device__ __forceinline__ void kv_finish(const KvDev &c, const KvAttn &a, int b
 #pragma unroll
     for (int i = 0; i < E; i += 2) *(float2 *)(p + i) = make_float2(o[i], o[i + 1]);
   } else kv_row_out<T, E>((uint16_t *)a.out + at, true, o);
+}
+// ... from its sums (base 2: m the maximum that l and o are relative to)
+template <typename T, int HD>
+__device__ __forceinline__ void kv_finish(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float (&o)[HD / 32], float m, float l) {
+  float x = l;
+#pragma unroll
+  for (int i = 0; i < HD / 32; i++) x += o[i] * 0.0f;
+  if (__any_sync(0xffffffffu, !(fabsf(x) < INFINITY))) kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
+  kv_store<T, HD>(a, r, h, lane, o, l);
 }

@@ -1,0 +1,428 @@
+// kvpf.cuh -- attention of many rows (prompts and pieces of them) over the paged cache, on tcgen05: bound by the matrix products.
+//
+// A block has 128 queries of one kv head (query i G + h is row i, head h of the kv head's G) at head dimension 256, two times 128 below, and
+// the slots that they see, KP_TILE at a time.  Two streams of steps take turns on the tensor core, so that one's softmax runs beside the
+// other's products: the two query tiles where there are two, else the even and the odd tiles of slots of the one.
+//   S[query][slot] = Q K^T     into the stream's S columns; Q in shared memory, or in tensor memory at head dimension 256, where reading it from shared
+//                              memory beside 64 slots of K would take longer than the product
+//   P = exp(S - m)             a thread a query; in 16 bits over S's columns
+//   O[query][dim] += P V       V as it lies in the cache (MN-major)
+// m is the maximum of a query's scores as of the last step in which it grew by more than 2^8: O and the sum are only then rescaled, and P stays below 2^8.
+// K and V come by TMA, a page's part of a tile each, in rows of 128 swizzled bytes.  A slot that no row of the block sees is zeroed in V before
+// the product (whatever the page holds there, 0 times it has to be 0).
+//
+// Warps: softmax (4 a query tile), one that loads, one that issues the MMAs.  Every wait is bounded.
+#pragma once
+#include "kvatt.cuh"
+
+template <int HD> struct Kp {
+  static constexpr int NQT = HD == 256 ? 1 : 2;            // query tiles
+  static constexpr int TILE = HD == 256 ? 64 : 128;        // slots
+  static constexpr int SH = HD == 256 ? 6 : 7;
+  static constexpr int GB = TILE * HD * 2;                 // bytes of a tile of K or V
+  static constexpr int QB = HD == 256 ? 0 : NQT * 128 * HD * 2;
+  static constexpr int NS = HD == 256 ? 7 : HD == 128 ? 5 : 6;
+  static constexpr int SMEM = 1024 + QB + NS * GB;
+  static constexpr int SOFT = 4 * NQT, THREADS = 32 * (SOFT + 2);
+  static constexpr uint32_t O = 0, S = HD == 256 ? 384 : 256, SC = TILE, Q = 256;   // tensor memory's columns; S: two times SC
+};
+static_assert(Kp<256>::SMEM <= 232448 && Kp<128>::SMEM <= 232448 && Kp<64>::SMEM <= 232448, "shared memory");
+
+struct KvPfPlan {
+  int splits;                  // blocks a unit's tiles of slots are spread over
+  float *pm, *pl, *po;         // [seqs][KV][queries][splits](, [hd]), where there are several; queries: G max_rows
+  unsigned int *err;
+};
+// a unit's tiles of slots: those of first tokens, then those from the first row's window on
+struct KpTiles { int lo, cs, n; };
+template <int SH> __device__ __forceinline__ KpTiles kp_tiles(int ea, int ez, int window, int sinks) {
+  KpTiles t;
+  t.lo = kv_first(max(ea, 0), window) >> SH;
+  t.cs = min((min(sinks, kv_first(max(ea, 0), window)) + (1 << SH) - 1) >> SH, t.lo);
+  t.n = ez < 0 ? 0 : t.cs + (ez >> SH) - t.lo + 1;
+  return t;
+}
+__device__ __forceinline__ void kp_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D f32, A and B of type T, M = 128; mn: B is MN-major
+template <typename T> __host__ __device__ constexpr uint32_t kp_idesc(int N, bool mn) {
+  return 0x08000010u | (sizeof(T) == 2 && !__is_same(T, __half) ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17);
+}
+// rows of 128 swizzled bytes, eight of them 1024 bytes on from the next eight; step: from 64 columns of an MN-major operand to the next 64
+__device__ __forceinline__ uint64_t kp_desc(uint32_t addr_s, uint32_t step) { return g3_desc(addr_s, step, 1024) | (2ull << 61); }
+__device__ __forceinline__ void kp_ld32(uint32_t taddr, float *v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p, int tiles, const __grid_constant__ CUtensorMap km,
+                                                              const __grid_constant__ CUtensorMap vm) {
+  using C = Kp<HD>;
+  constexpr int NQT = C::NQT, TILE = C::TILE, SH = C::SH, GB = C::GB, NS = C::NS, QT = 128 * NQT, BLK = TILE * 128;   // BLK: 64 dims of a tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t bar_s = smem_u32(smem), q_s = bar_s + 1024, ring_s = q_s + C::QB;
+  auto full = [&](int s) { return bar_s + 8u * (uint32_t)s; };
+  auto empty = [&](int s) { return bar_s + 64u + 8u * (uint32_t)s; };
+  auto s_full = [&](int x) { return bar_s + 128u + 8u * (uint32_t)x; };
+  auto p_full = [&](int x) { return bar_s + 144u + 8u * (uint32_t)x; };
+  auto pv_done = [&](int x) { return bar_s + 160u + 8u * (uint32_t)x; };
+  const uint32_t q_full = bar_s + 176u;
+  uint32_t *tmem_slot = (uint32_t *)(smem + 192);
+  volatile uint32_t *dead = (volatile uint32_t *)(smem + 196);
+  volatile uint32_t *badm = (volatile uint32_t *)(smem + 256);   // [tile & 7]: 16-slot groups whose page is no page
+  pdl_wait();
+  // ---- which unit: the last query tiles first, they see the most ----
+  const int split = blockIdx.y, u = blockIdx.x, g = u % c.KV, b = u / c.KV % c.seqs, tile = tiles - 1 - u / c.KV / c.seqs;
+  const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, SH);
+  const int NQ = a.G * s.nc, q0 = tile * QT;
+  if (q0 >= NQ) return;
+  const int ea = s.e0 + q0 / a.G, ez = s.e0 + min(q0 + QT - 1, NQ - 1) / a.G;   // slots of the first and the last row
+  const KpTiles kt = kp_tiles<SH>(ea, ez, a.window, a.sinks);
+  const int per = (kt.n + p.splits - 1) / p.splits, t0 = min(kt.n, split * per), n = min(kt.n, t0 + per) - t0;
+  auto slot_of = [&](int i) { i += t0; return (i < kt.cs ? i : kt.lo + i - kt.cs) << SH; };
+  auto seen = [&](int j) { return j <= ez && (!a.window || j > ea - a.window || j < a.sinks); };   // by some row of the block
+  auto part_of = [&](int qi) { return (((size_t)b * c.KV + g) * ((size_t)a.G * rw.max_rows) + qi) * p.splits + split; };
+  if (!n) {
+    for (int qi = q0 + tid; qi < min(q0 + QT, NQ); qi += C::THREADS) {
+      if (p.splits > 1) { p.pm[part_of(qi)] = -INFINITY; p.pl[part_of(qi)] = 0.0f; continue; }
+      const long long at = (long long)(s.first + qi / a.G) * a.os + (long long)(g * a.G + qi % a.G) * HD;
+      for (int d = 0; d < HD * (a.out32 ? 4 : 2); d += 16) *(uint4 *)((uint8_t *)a.out + at * (a.out32 ? 4 : 2) + d) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
+    for (int x = 0; x < 2; x++) { mbar_init(s_full(x), 1); mbar_init(p_full(x), 4); mbar_init(pv_done(x), 1); }
+    mbar_init(q_full, C::SOFT);
+    *dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == C::SOFT + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  t5_fence_before();
+  __syncthreads();
+  t5_fence_after();
+  pdl_trigger();                                 // (tensor memory is taken: a later kernel's block cannot sit on it while it waits for this one)
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint32_t bar, uint32_t parity) {   // gives up for the whole block
+    for (uint32_t k = 0; !mbar_wait(bar, parity, 4); k += 4) {
+      if (*dead) return;
+      if (k >= T5_WAIT_LIMIT) { *dead = 1; atomicExch(p.err, 1u); return; }
+    }
+  };
+  // tiles of K and V in the order in which they are first used
+  auto ring_k = [&](int i) { return NQT == 2 ? 2 * i : i ? 2 * i - 1 : 0; };
+  auto ring_v = [&](int i) { return NQT == 2 ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2; };
+
+  if (warp < C::SOFT) {
+    // ---- softmax: a thread a query ----
+    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = qi < NQ ? s.e0 + qi / a.G : -1, lw = a.window ? e - a.window + 1 : 0;
+    const uint32_t lq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    {
+      const uint16_t *src = a.q + (long long)(s.first + qi / a.G) * a.qs + (long long)(g * a.G + qi % a.G) * HD;
+#pragma unroll
+      for (int d0 = 0; d0 < HD; d0 += 64) {
+        uint32_t v[32];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const uint4 w = qi < NQ ? __ldg((const uint4 *)(src + d0) + i) : make_uint4(0, 0, 0, 0);
+          v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
+        }
+        if constexpr (HD == 256) t5_st32(lq + C::Q + d0 / 2, v);
+        else {
+          const int r = tid & 127;
+          uint8_t *d = smem + 1024 + x0 * (128 * HD * 2) + (d0 >> 6) * (128 * 128) + r * 128;
+#pragma unroll
+          for (int i = 0; i < 8; i++) *(uint4 *)(d + ((i ^ (r & 7)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      }
+      if constexpr (HD == 256) { t5_wait_st(); t5_fence_before(); }
+      else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    float m = -INFINITY, l = 0.0f;
+    // slots of this query tile's first and last row: a tile between what they see is seen whole by every row
+    const int qa = q0 + 128 * x0, ra = s.e0 + qa / a.G, rz = s.e0 + min(qa + 127, NQ - 1) / a.G;
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+      const int x = NQT == 2 ? x0 : i & 1, slot = slot_of(i);
+      const uint32_t S = lq + C::S + C::SC * (uint32_t)x;
+      float v[TILE];
+      wait(s_full(x), (uint32_t)(NQT == 2 ? i : i >> 1) & 1u);
+      __syncwarp();
+      t5_fence_after();
+#pragma unroll
+      for (int k = 0; k < TILE; k += 32) kp_ld32(S + k, v + k);
+      t5_wait_ld();
+      const uint32_t bm = badm[i & 7];
+      if (bm || slot + TILE - 1 > ra || (a.window && slot <= rz - a.window && slot + TILE - 1 >= a.sinks) || qa + 127 >= NQ) {
+#pragma unroll
+        for (int k = 0; k < TILE; k++) {
+          const int j = slot + k;
+          if (j > e || (j < lw && j >= a.sinks) || (bm >> (k >> 4) & 1)) v[k] = -INFINITY;
+        }
+      }
+      float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+      for (int k = 4; k < TILE; k += 8) {
+#pragma unroll
+        for (int w = 0; w < 4; w++) mx[w] = k + 4 + w < TILE ? fmaxf(mx[w], fmaxf(v[k + w], v[k + 4 + w])) : fmaxf(mx[w], v[k + w]);
+      }
+      const float t = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
+      const bool grow = t > m + 8.0f;                      // (from minus infinity at once)
+      if (__any_sync(0xffffffffu, grow)) {
+        const float mn = grow ? t : m, cf = mn == -INFINITY ? 1.0f : kv_exp2(m - mn);
+        m = mn;
+        l *= cf;
+        if (i) {
+          if (NQT == 1) { wait(pv_done(0), (uint32_t)(i - 1) & 1u); __syncwarp(); t5_fence_after(); }   // (else S came behind the last product into O)
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 32) {
+            float o[32];
+            const uint32_t at = lq + C::O + (uint32_t)(x0 * HD + d);
+            kp_ld32(at, o);
+            t5_wait_ld();
+            uint32_t w[32];
+#pragma unroll
+            for (int k = 0; k < 32; k++) w[k] = __float_as_uint(o[k] * cf);
+            t5_st32(at, w);
+          }
+          t5_wait_st();
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : -m;
+      const f32x2 sc2 = x2_pack(a.scale2, a.scale2), rf2 = x2_pack(ref, ref);
+      f32x2 sum[2] = {0, 0};
+#pragma unroll
+      for (int k0 = 0; k0 < TILE; k0 += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+          float y0, y1;
+          x2_unpack(x2_fma(x2_pack(v[k0 + 2 * k], v[k0 + 2 * k + 1]), sc2, rf2), y0, y1);
+          y0 = kv_exp2(y0); y1 = kv_exp2(y1);
+          sum[k & 1] = x2_add(sum[k & 1], x2_pack(y0, y1));
+          w[k] = KvEl<T>::of2(y0, y1);
+        }
+        t5_st32(S + k0 / 2, w);
+      }
+      float a0, a1;
+      x2_unpack(x2_add(sum[0], sum[1]), a0, a1);
+      l += a0 + a1;
+      t5_wait_st();
+      t5_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(x));
+    }
+    // ---- the rows' results ----
+    const int pd = NQT == 2 ? x0 : 0;
+    if (NQT == 1 && n > 1) wait(pv_done(0), (uint32_t)(n - 2) & 1u);   // (the last two products may both be under way: one phase after the other)
+    wait(pv_done(pd), (uint32_t)(n - 1) & 1u);
+    __syncwarp();
+    t5_fence_after();
+    const int row = qi / a.G, h = g * a.G + qi % a.G;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float chk = l;
+    const long long at = (long long)(s.first + row) * a.os + (long long)h * HD;
+    const size_t part = p.splits > 1 && qi < NQ ? part_of(qi) : 0;
+    if (p.splits > 1 && qi < NQ) { p.pm[part] = m; p.pl[part] = l; }
+#pragma unroll 1
+    for (int d = 0; d < HD; d += 32) {
+      float o[32];
+      __syncwarp();
+      kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d), o);
+      t5_wait_ld();
+      if (qi >= NQ) continue;
+      if (p.splits > 1) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) *(float4 *)(p.po + part * HD + d + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < 32; k++) { chk += o[k] * 0.0f; o[k] *= inv; }
+      if (a.out32) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) *(float4 *)((float *)a.out + at + d + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+          *(uint4 *)((uint16_t *)a.out + at + d + k) = make_uint4(KvEl<T>::of2(o[k], o[k + 1]), KvEl<T>::of2(o[k + 2], o[k + 3]), KvEl<T>::of2(o[k + 4], o[k + 5]), KvEl<T>::of2(o[k + 6], o[k + 7]));
+      }
+    }
+    // rows whose result is no number once more, by themselves (kv_attn_row says why)
+    unsigned redo = __ballot_sync(0xffffffffu, p.splits == 1 && qi < NQ && !(fabsf(chk) < INFINITY));
+    while (redo) {
+      const int k = __ffs(redo) - 1, qk = q0 + 128 * x0 + 32 * (warp & 3) + k, rk = qk / a.G;
+      redo &= redo - 1;
+      float o[HD / 32], mk, lk;
+      kv_attn_row<T, HD>(c, a, b, s.first + rk, g * a.G + qk % a.G, s.e0 + rk, lane, o, mk, lk);
+      kv_store<T, HD>(a, s.first + rk, g * a.G + qk % a.G, lane, o, lk);
+    }
+  } else if (warp == C::SOFT) {
+    // ---- K and V: a lane a page's part of a tile ----
+    const int bs = min(c.page_sh, SH), boxes = TILE >> bs;
+    auto page_at = [&](int i) {                            // the lane's page of tile i; -2: nothing that a row sees
+      if (lane >= boxes || i >= n) return -2;
+      const int j = slot_of(i) + (lane << bs);
+      bool any = false;                                    // (what is seen is one run of slots and the first ones)
+      if (j <= ez) any = !a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks;
+      return any ? __ldcg(c.table + (size_t)b * c.tstride + (j >> c.page_sh)) : -2;
+    };
+    auto load = [&](const CUtensorMap *map, int t, int i, int id, bool isk) {
+      const int slot = t % NS;
+      if (t >= NS) wait(empty(slot), (uint32_t)(t / NS - 1) & 1u);
+      __syncwarp();
+      const bool in = (unsigned)id < (unsigned)c.n_pages, wrong = !in && id != -2;
+      const unsigned have = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, wrong);
+      if (wrong) atomicOr(c.err, KV_ERR_PAGE);
+      if (lane == 0) {
+        if (isk) {
+          uint32_t bm = 0;
+          for (int k = 0; k < boxes; k++) if (lost >> k & 1) bm |= ((1u << (1 << (bs - 4))) - 1) << (k << (bs - 4));
+          badm[i & 7] = bm;
+        }
+        if (!*dead && have) kv_expect(full(slot), (uint32_t)__popc(have) * (HD / 64) * (128u << bs));
+        else mbar_arrive(full(slot));
+      }
+      __syncwarp();
+      if (in && !*dead) {
+        const int j = slot_of(i) + (lane << bs);
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) kv_tma(ring_s + slot * GB + d * BLK + (lane << bs) * 128, map, 64 * d, j & ((1 << c.page_sh) - 1), g, id, full(slot));
+      }
+      __syncwarp();
+    };
+    int now = page_at(0), next = page_at(1), t = 0;
+    load(&km, t++, 0, now, true);
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+      const int later = page_at(i + 2);
+      if (NQT == 1 && i + 1 < n) load(&km, t++, i + 1, next, true);
+      load(&vm, t++, i, now, false);
+      if (NQT == 2 && i + 1 < n) load(&km, t++, i + 1, next, true);
+      now = next; next = later;
+    }
+  } else {
+    // ---- the tensor core: the whole warp walks, an elected lane issues ----
+    const bool el = t5_elect();
+    constexpr uint32_t ids = kp_idesc<T>(TILE, false), ido = kp_idesc<T>(HD, true);
+    const int steps = NQT * n;
+    wait(q_full, 0);
+    __syncwarp();
+    t5_fence_after();
+    auto score = [&](int k) {
+      const int i = NQT == 2 ? k >> 1 : k, x = k & 1, slot = ring_k(i) % NS;
+      if (NQT == 1 || !x) { wait(full(slot), (uint32_t)(ring_k(i) / NS) & 1u); __syncwarp(); }
+      t5_fence_after();
+      const uint32_t D = tmem + C::S + C::SC * (uint32_t)x;
+      const uint64_t kd = kp_desc(ring_s + slot * GB, 16), qd = kp_desc(q_s + x * (128 * HD * 2), 16);
+      if (el) {
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+          const uint64_t kk = kd + (uint64_t)((d >> 2) * (BLK / 16) + 2 * (d & 3));
+          if constexpr (HD == 256) t5_mma_f16_ts(D, tmem + C::Q + 8 * d, kk, ids, d != 0);
+          else kp_ss(D, qd + (uint64_t)((d >> 2) * (128 * 128 / 16) + 2 * (d & 3)), kk, ids, d != 0);
+        }
+        t5_commit(s_full(x));
+        if (NQT == 1 || x) t5_commit(empty(slot));
+      }
+      __syncwarp();
+    };
+    auto value = [&](int k) {
+      const int i = NQT == 2 ? k >> 1 : k, x = k & 1, slot = ring_v(i) % NS;
+      if (NQT == 1 || !x) {
+        wait(full(slot), (uint32_t)(ring_v(i) / NS) & 1u);
+        __syncwarp();
+        const int j0 = slot_of(i);
+        const uint32_t bm = badm[i & 7];
+        if (bm || j0 + TILE - 1 > ez || (a.window && j0 <= ea - a.window && j0 + TILE - 1 >= a.sinks)) {
+          uint8_t *d = smem + 1024 + C::QB + slot * GB;
+          for (int r = 0; r < TILE; r++) {
+            if (seen(j0 + r) && !(bm >> (r >> 4) & 1)) continue;
+            for (int w = lane; w < HD / 8; w += 32) *(uint4 *)(d + (w >> 3) * BLK + r * 128 + (w & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+      }
+      wait(p_full(x), (uint32_t)(k >> 1) & 1u);
+      __syncwarp();
+      t5_fence_after();
+      const uint64_t vd = kp_desc(ring_s + slot * GB, BLK);
+      const uint32_t P = tmem + C::S + C::SC * (uint32_t)x, D = tmem + C::O + (NQT == 2 ? (uint32_t)(x * HD) : 0u);
+      if (el) {
+#pragma unroll
+        for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(D, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
+        t5_commit(pv_done(NQT == 2 ? x : 0));
+        if (NQT == 1 || x) t5_commit(empty(slot));
+      }
+      __syncwarp();
+    };
+    score(0);
+    if (steps > 1) score(1);
+#pragma unroll 1
+    for (int k = 0; k < steps; k++) {
+      value(k);
+      if (k + 2 < steps) score(k + 2);
+    }
+  }
+  // after a wait ran out nothing is requested any more, but copies may be on their way
+  if (*dead) for (int i = 0; i < 64; i++) __nanosleep(1000);
+  __syncwarp();
+  t5_fence_before();
+  __syncthreads();
+  if (warp == C::SOFT + 1) {
+    t5_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// the splits of a row and head put together, in their order: a warp each
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) k_kv_pf_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p) {
+  constexpr int E = HD / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), r = blockIdx.x;
+  const int b = kv_find(rw, c.seqs, r, lane);
+  if (b < 0 || h >= a.H) return;
+  int first;
+  const int n = kv_rows(c, rw, b, first), i = r - first;
+  if (i >= rw.max_rows) return;
+  const int g = h / a.G;
+  const size_t at = (((size_t)b * c.KV + g) * ((size_t)a.G * rw.max_rows) + (size_t)i * a.G + h % a.G) * p.splits;
+  float M = -INFINITY;
+  for (int w = lane; w < p.splits; w += 32) M = fmaxf(M, __ldcg(p.pm + at + w));
+#pragma unroll
+  for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+  float o[E], l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < E; k++) o[k] = 0.0f;
+#pragma unroll 4
+  for (int w = 0; w < p.splits; w++) {
+    const float pm = __ldcg(p.pm + at + w);
+    if (pm == -INFINITY) continue;                         // (nothing seen there: no sums)
+    const float f = exp2f(pm - M);
+    l += __ldcg(p.pl + at + w) * f;
+#pragma unroll
+    for (int k = 0; k < E; k += 2) { const float2 v = __ldcg((const float2 *)(p.po + (at + w) * HD + lane * E + k)); o[k] += v.x * f; o[k + 1] += v.y * f; }
+  }
+  kv_finish<T, HD>(c, a, b, r, h, kv_len(c, b) - n + i, lane, o, M, l);
+}
