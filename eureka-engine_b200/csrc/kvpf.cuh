@@ -1,10 +1,10 @@
 // kvpf.cuh -- attention of many rows (prompts and pieces of them) over the paged cache, on tcgen05: bound by the matrix products.
 //
-// A block has 128 queries of one kv head (query i G + h is row i, head h of the kv head's G) at head dimension 256, two times 128 below, and
-// the slots that they see, KP_TILE at a time.  Two streams of steps take turns on the tensor core, so that one's softmax runs beside the
-// other's products: the two query tiles where there are two, else the even and the odd tiles of slots of the one.
-//   S[query][slot] = Q K^T     into the stream's S columns; Q in shared memory, or in tensor memory at head dimension 256, where reading it from shared
-//                              memory beside 64 slots of K would take longer than the product
+// A block has 128 queries of one kv head (query i G + h is row i, head h of the kv head's G) at head dimension 256, two times 128 below (two
+// streams), and the slots that they see, 64 at a time.  A stream has the scores of two tiles of slots in tensor memory, so that the tensor core works
+// on the next tile's while the softmax of one runs.
+//   S[query][slot] = Q K^T     Q in shared memory, or in tensor memory at head dimension 256, where reading it from shared memory beside 64 slots of K
+//                              would take longer than the product
 //   P = exp(S - m)             a thread a query; in 16 bits over S's columns
 //   O[query][dim] += P V       V as it lies in the cache (MN-major)
 // m is the maximum of a query's scores as of the last step in which it grew by more than 2^8: O and the sum are only then rescaled, and P stays below 2^8.
@@ -16,15 +16,14 @@
 #include "kvatt.cuh"
 
 template <int HD> struct Kp {
-  static constexpr int NQT = HD == 256 ? 1 : 2;            // query tiles
-  static constexpr int TILE = HD == 256 ? 64 : 128;        // slots
-  static constexpr int SH = HD == 256 ? 6 : 7;
+  static constexpr int NQT = HD == 256 ? 1 : 2;            // query tiles: streams
+  static constexpr int TILE = 64, SH = 6;                  // slots
   static constexpr int GB = TILE * HD * 2;                 // bytes of a tile of K or V
   static constexpr int QB = HD == 256 ? 0 : NQT * 128 * HD * 2;
-  static constexpr int NS = HD == 256 ? 7 : HD == 128 ? 5 : 6;
+  static constexpr int NS = HD == 256 ? 7 : HD == 128 ? 10 : 12;
   static constexpr int SMEM = 1024 + QB + NS * GB;
   static constexpr int SOFT = 4 * NQT, THREADS = 32 * (SOFT + 2);
-  static constexpr uint32_t O = 0, S = HD == 256 ? 384 : 256, SC = TILE, Q = 256;   // tensor memory's columns; S: two times SC
+  static constexpr uint32_t O = 0, S = HD == 256 ? 384 : 256, Q = 256;   // tensor memory's columns; S: two tiles a stream
 };
 static_assert(Kp<256>::SMEM <= 232448 && Kp<128>::SMEM <= 232448 && Kp<64>::SMEM <= 232448, "shared memory");
 
@@ -67,6 +66,8 @@ __device__ __forceinline__ void kp_ld32(uint32_t taddr, float *v) {
   for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }   // the n lowest bits
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p, int tiles, const __grid_constant__ CUtensorMap km,
                                                               const __grid_constant__ CUtensorMap vm) {
@@ -76,14 +77,14 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t bar_s = smem_u32(smem), q_s = bar_s + 1024, ring_s = q_s + C::QB;
   auto full = [&](int s) { return bar_s + 8u * (uint32_t)s; };
-  auto empty = [&](int s) { return bar_s + 64u + 8u * (uint32_t)s; };
-  auto s_full = [&](int x) { return bar_s + 128u + 8u * (uint32_t)x; };
-  auto p_full = [&](int x) { return bar_s + 144u + 8u * (uint32_t)x; };
-  auto pv_done = [&](int x) { return bar_s + 160u + 8u * (uint32_t)x; };
-  const uint32_t q_full = bar_s + 176u;
-  uint32_t *tmem_slot = (uint32_t *)(smem + 192);
-  volatile uint32_t *dead = (volatile uint32_t *)(smem + 196);
-  volatile uint32_t *badm = (volatile uint32_t *)(smem + 256);   // [tile & 7]: 16-slot groups whose page is no page
+  auto empty = [&](int s) { return bar_s + 96u + 8u * (uint32_t)s; };
+  auto s_full = [&](int x, int i) { return bar_s + 192u + 8u * (uint32_t)(2 * x + (i & 1)); };
+  auto p_full = [&](int x, int i) { return bar_s + 224u + 8u * (uint32_t)(2 * x + (i & 1)); };
+  auto pv_done = [&](int x) { return bar_s + 256u + 8u * (uint32_t)x; };
+  const uint32_t q_full = bar_s + 272u;
+  uint32_t *tmem_slot = (uint32_t *)(smem + 280);
+  volatile uint32_t *dead = (volatile uint32_t *)(smem + 284);
+  volatile uint32_t *badm = (volatile uint32_t *)(smem + 288);   // [tile & 15]: 16-slot groups whose page is no page
   pdl_wait();
   // ---- which unit: the last query tiles first, they see the most ----
   const int split = blockIdx.y, u = blockIdx.x, g = u % c.KV, b = u / c.KV % c.seqs, tile = tiles - 1 - u / c.KV / c.seqs;
@@ -106,8 +107,9 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   }
   if (tid == 0) {
     for (int i = 0; i < NS; i++) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
-    for (int x = 0; x < 2; x++) { mbar_init(s_full(x), 1); mbar_init(p_full(x), 4); mbar_init(pv_done(x), 1); }
-    mbar_init(q_full, C::SOFT);
+    for (int x = 0; x < 4; x++) { mbar_init(s_full(x >> 1, x), 1); mbar_init(p_full(x >> 1, x), 4); }
+    mbar_init(pv_done(0), 1); mbar_init(pv_done(1), 1);
+    mbar_init(q_full, NQT == 2 && q0 + 128 < NQ ? 8 : 4);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -127,12 +129,13 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     }
   };
   // tiles of K and V in the order in which they are first used
-  auto ring_k = [&](int i) { return NQT == 2 ? 2 * i : i ? 2 * i - 1 : 0; };
-  auto ring_v = [&](int i) { return NQT == 2 ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2; };
+  auto ring_k = [&](int i) { return i ? 2 * i - 1 : 0; };
+  auto ring_v = [&](int i) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; };
+  const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
 
-  if (warp < C::SOFT) {
+  if (warp < 4 * streams) {
     // ---- softmax: a thread a query ----
-    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = qi < NQ ? s.e0 + qi / a.G : -1, lw = a.window ? e - a.window + 1 : 0;
+    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = s.e0 + min(qi, NQ - 1) / a.G, lw = a.window ? e - a.window + 1 : 0;
     const uint32_t lq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     {
       const uint16_t *src = a.q + (long long)(s.first + qi / a.G) * a.qs + (long long)(g * a.G + qi % a.G) * HD;
@@ -162,21 +165,26 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     const int qa = q0 + 128 * x0, ra = s.e0 + qa / a.G, rz = s.e0 + min(qa + 127, NQ - 1) / a.G;
 #pragma unroll 1
     for (int i = 0; i < n; i++) {
-      const int x = NQT == 2 ? x0 : i & 1, slot = slot_of(i);
-      const uint32_t S = lq + C::S + C::SC * (uint32_t)x;
+      const int slot = slot_of(i);
+      const uint32_t S = lq + C::S + (uint32_t)(TILE * (2 * x0 + (i & 1)));
       float v[TILE];
-      wait(s_full(x), (uint32_t)(NQT == 2 ? i : i >> 1) & 1u);
+      wait(s_full(x0, i), (uint32_t)(i >> 1) & 1u);
       __syncwarp();
       t5_fence_after();
 #pragma unroll
       for (int k = 0; k < TILE; k += 32) kp_ld32(S + k, v + k);
       t5_wait_ld();
-      const uint32_t bm = badm[i & 7];
-      if (bm || slot + TILE - 1 > ra || (a.window && slot <= rz - a.window && slot + TILE - 1 >= a.sinks) || qa + 127 >= NQ) {
+      const uint32_t bm = badm[i & 15];
+      if (bm || slot + TILE - 1 > ra || (a.window && slot <= rz - a.window && slot + TILE - 1 >= a.sinks)) {
 #pragma unroll
-        for (int k = 0; k < TILE; k++) {
-          const int j = slot + k;
-          if (j > e || (j < lw && j >= a.sinks) || (bm >> (k >> 4) & 1)) v[k] = -INFINITY;
+        for (int k0 = 0; k0 < TILE; k0 += 32) {            // a bit a slot: seen
+          const int j = slot + k0;
+          uint32_t on = kp_below(e + 1 - j) & (~kp_below(lw - j) | kp_below(a.sinks - j));
+          if (bm >> (k0 >> 4) & 1) on &= 0xffff0000u;
+          if (bm >> (k0 >> 4) & 2) on &= 0x0000ffffu;
+          if (!__any_sync(0xffffffffu, on != 0xffffffffu)) continue;
+#pragma unroll
+          for (int k = 0; k < 32; k++) v[k0 + k] = on & (1u << k) ? v[k0 + k] : -INFINITY;
         }
       }
       float mx[4] = {v[0], v[1], v[2], v[3]};
@@ -192,7 +200,9 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         m = mn;
         l *= cf;
         if (i) {
-          if (NQT == 1) { wait(pv_done(0), (uint32_t)(i - 1) & 1u); __syncwarp(); t5_fence_after(); }   // (else S came behind the last product into O)
+          wait(pv_done(x0), (uint32_t)(i - 1) & 1u);       // the last product into O is done
+          __syncwarp();
+          t5_fence_after();
 #pragma unroll 1
           for (int d = 0; d < HD; d += 32) {
             float o[32];
@@ -226,44 +236,86 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       float a0, a1;
       x2_unpack(x2_add(sum[0], sum[1]), a0, a1);
       l += a0 + a1;
+      // slots that no row of the block sees: their V is taken out, whatever the page holds, before the first product with the tile
+      if (x0 == 0 && (bm || slot + TILE - 1 > ez || (a.window && slot <= ea - a.window && slot + TILE - 1 >= a.sinks))) {
+        const int rs = ring_v(i) % NS;
+        wait(full(rs), (uint32_t)(ring_v(i) / NS) & 1u);
+        const uint32_t at = ring_s + rs * GB;
+        auto clear = [&](int ra, int rz) {                 // rows ra .. rz - 1 of the tile
+#pragma unroll 1
+          for (int w = ra * (HD / 8) + tid; w < rz * (HD / 8); w += 128) {
+            const int r = w / (HD / 8), d = w % (HD / 8);  // a row's 16 bytes, in the order in which they lie
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (d >> 3) * BLK + r * 128 + ((d & 7) << 4)), "r"(0) : "memory");
+          }
+        };
+        clear(max(0, ez + 1 - slot), TILE);
+        if (a.window) clear(max(0, a.sinks - slot), min(TILE, ea - a.window + 1 - slot));
+#pragma unroll 1
+        for (int r = 0; bm && r < TILE; r += 16)
+          if (bm >> (r >> 4) & 1) clear(r, r + 16);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
       t5_wait_st();
       t5_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(x));
+      if (lane == 0) mbar_arrive(p_full(x0, i));
     }
     // ---- the rows' results ----
-    const int pd = NQT == 2 ? x0 : 0;
-    if (NQT == 1 && n > 1) wait(pv_done(0), (uint32_t)(n - 2) & 1u);   // (the last two products may both be under way: one phase after the other)
-    wait(pv_done(pd), (uint32_t)(n - 1) & 1u);
+    if (n > 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);  // (the last two products may both be under way: one phase after the other)
+    wait(pv_done(x0), (uint32_t)(n - 1) & 1u);
     __syncwarp();
     t5_fence_after();
-    const int row = qi / a.G, h = g * a.G + qi % a.G;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float chk = l;
-    const long long at = (long long)(s.first + row) * a.os + (long long)h * HD;
-    const size_t part = p.splits > 1 && qi < NQ ? part_of(qi) : 0;
-    if (p.splits > 1 && qi < NQ) { p.pm[part] = m; p.pl[part] = l; }
-#pragma unroll 1
-    for (int d = 0; d < HD; d += 32) {
-      float o[32];
+    if (p.splits > 1 && qi < NQ) { const size_t part = part_of(qi); p.pm[part] = m; p.pl[part] = l; }
+    // whole 128-byte pieces of rows, turned in the ring's memory: every product is done
+    const bool wide = p.splits > 1 || a.out32;             // 32 dims a piece, or 64
+    const uint32_t st = ring_s + (uint32_t)warp * 4096u;
+    uint8_t *dst[8];                                       // rows 4 k + lane / 8 of the warp's
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int qk = q0 + 128 * x0 + 32 * (warp & 3) + 4 * k + (lane >> 3);
+      dst[k] = nullptr;
+      if (qk >= NQ) continue;
+      if (p.splits > 1) dst[k] = (uint8_t *)(p.po + part_of(qk) * HD);
+      else dst[k] = (uint8_t *)a.out + ((long long)(s.first + qk / a.G) * a.os + (long long)(g * a.G + qk % a.G) * HD) * (a.out32 ? 4 : 2);
+      dst[k] += 16 * (lane & 7);
+    }
+    auto piece = [&](int at) {
       __syncwarp();
-      kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d), o);
-      t5_wait_ld();
-      if (qi >= NQ) continue;
-      if (p.splits > 1) {
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) *(float4 *)(p.po + part * HD + d + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-        continue;
+      for (int k = 0; k < 8; k++) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(st + (4 * k + (lane >> 3)) * 128 + (((lane & 7) ^ ((4 * k + (lane >> 3)) & 7)) << 4)) : "memory");
+        if (dst[k]) *(uint4 *)(dst[k] + at) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      __syncwarp();
+    };
+    auto put = [&](int k, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(st + lane * 128 + ((k ^ (lane & 7)) << 4)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
+    };
+#pragma unroll 1
+    for (int d = 0; d < HD; d += 64) {
 #pragma unroll
-      for (int k = 0; k < 32; k++) { chk += o[k] * 0.0f; o[k] *= inv; }
-      if (a.out32) {
+      for (int half = 0; half < 2; half++) {
+        float o[32];
+        kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d + 32 * half), o);
+        t5_wait_ld();
+        if (p.splits == 1) {
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) *(float4 *)((float *)a.out + at + d + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-      } else {
+          for (int k = 0; k < 32; k++) { chk += o[k] * 0.0f; o[k] *= inv; }
+        }
+        if (wide) {
 #pragma unroll
-        for (int k = 0; k < 32; k += 8)
-          *(uint4 *)((uint16_t *)a.out + at + d + k) = make_uint4(KvEl<T>::of2(o[k], o[k + 1]), KvEl<T>::of2(o[k + 2], o[k + 3]), KvEl<T>::of2(o[k + 4], o[k + 5]), KvEl<T>::of2(o[k + 6], o[k + 7]));
+          for (int k = 0; k < 8; k++) put(k, __float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
+          piece(4 * (d + 32 * half));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            put(4 * half + k, KvEl<T>::of2(o[8 * k], o[8 * k + 1]), KvEl<T>::of2(o[8 * k + 2], o[8 * k + 3]), KvEl<T>::of2(o[8 * k + 4], o[8 * k + 5]), KvEl<T>::of2(o[8 * k + 6], o[8 * k + 7]));
+          if (half) piece(2 * d);
+        }
       }
     }
     // rows whose result is no number once more, by themselves (kv_attn_row says why)
@@ -275,16 +327,23 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       kv_attn_row<T, HD>(c, a, b, s.first + rk, g * a.G + qk % a.G, s.e0 + rk, lane, o, mk, lk);
       kv_store<T, HD>(a, s.first + rk, g * a.G + qk % a.G, lane, o, lk);
     }
+  } else if (warp < C::SOFT) {
+    // (the second query tile is behind the last query)
   } else if (warp == C::SOFT) {
     // ---- K and V: a lane a page's part of a tile ----
     const int bs = min(c.page_sh, SH), boxes = TILE >> bs;
-    auto page_at = [&](int i) {                            // the lane's page of tile i; -2: nothing that a row sees
-      if (lane >= boxes || i >= n) return -2;
-      const int j = slot_of(i) + (lane << bs);
-      bool any = false;                                    // (what is seen is one run of slots and the first ones)
-      if (j <= ez) any = !a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks;
-      return any ? __ldcg(c.table + (size_t)b * c.tstride + (j >> c.page_sh)) : -2;
+    // the lane's entry of tile i's pages, asked for two tiles before its use; -2: nothing that a row sees
+    struct Entry { int id; bool on; };
+    auto entry = [&](int i) {
+      Entry x = {-2, false};
+      if (lane < boxes && i < n) {
+        const int j = slot_of(i) + (lane << bs);
+        x.on = j <= ez && (!a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks);   // (what is seen is one run of slots and the first ones)
+        if (x.on) asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(x.id) : "l"(c.table + (size_t)b * c.tstride + (j >> c.page_sh)));
+      }
+      return x;
     };
+    auto use = [&](Entry x) { asm volatile("" : "+r"(x.id)); return x.on ? x.id : -2; };     // (the load is not waited for before)
     auto load = [&](const CUtensorMap *map, int t, int i, int id, bool isk) {
       const int slot = t % NS;
       if (t >= NS) wait(empty(slot), (uint32_t)(t / NS - 1) & 1u);
@@ -296,7 +355,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         if (isk) {
           uint32_t bm = 0;
           for (int k = 0; k < boxes; k++) if (lost >> k & 1) bm |= ((1u << (1 << (bs - 4))) - 1) << (k << (bs - 4));
-          badm[i & 7] = bm;
+          badm[i & 15] = bm;
         }
         if (!*dead && have) kv_expect(full(slot), (uint32_t)__popc(have) * (HD / 64) * (128u << bs));
         else mbar_arrive(full(slot));
@@ -309,29 +368,29 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       }
       __syncwarp();
     };
-    int now = page_at(0), next = page_at(1), t = 0;
+    Entry next = entry(1);
+    int now = use(entry(0)), t = 0;
     load(&km, t++, 0, now, true);
 #pragma unroll 1
     for (int i = 0; i < n; i++) {
-      const int later = page_at(i + 2);
-      if (NQT == 1 && i + 1 < n) load(&km, t++, i + 1, next, true);
+      const Entry later = entry(i + 2);
+      const int then = use(next);
+      if (i + 1 < n) load(&km, t++, i + 1, then, true);
       load(&vm, t++, i, now, false);
-      if (NQT == 2 && i + 1 < n) load(&km, t++, i + 1, next, true);
-      now = next; next = later;
+      now = then; next = later;
     }
   } else {
     // ---- the tensor core: the whole warp walks, an elected lane issues ----
     const bool el = t5_elect();
     constexpr uint32_t ids = kp_idesc<T>(TILE, false), ido = kp_idesc<T>(HD, true);
-    const int steps = NQT * n;
     wait(q_full, 0);
     __syncwarp();
     t5_fence_after();
-    auto score = [&](int k) {
-      const int i = NQT == 2 ? k >> 1 : k, x = k & 1, slot = ring_k(i) % NS;
-      if (NQT == 1 || !x) { wait(full(slot), (uint32_t)(ring_k(i) / NS) & 1u); __syncwarp(); }
+    auto score = [&](int i, int x) {
+      const int slot = ring_k(i) % NS;
+      if (!x) { wait(full(slot), (uint32_t)(ring_k(i) / NS) & 1u); __syncwarp(); }
       t5_fence_after();
-      const uint32_t D = tmem + C::S + C::SC * (uint32_t)x;
+      const uint32_t D = tmem + C::S + (uint32_t)(TILE * (2 * x + (i & 1)));
       const uint64_t kd = kp_desc(ring_s + slot * GB, 16), qd = kp_desc(q_s + x * (128 * HD * 2), 16);
       if (el) {
 #pragma unroll
@@ -340,48 +399,39 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
           if constexpr (HD == 256) t5_mma_f16_ts(D, tmem + C::Q + 8 * d, kk, ids, d != 0);
           else kp_ss(D, qd + (uint64_t)((d >> 2) * (128 * 128 / 16) + 2 * (d & 3)), kk, ids, d != 0);
         }
-        t5_commit(s_full(x));
-        if (NQT == 1 || x) t5_commit(empty(slot));
+        t5_commit(s_full(x, i));
+        if (x == streams - 1) t5_commit(empty(slot));
       }
       __syncwarp();
     };
-    auto value = [&](int k) {
-      const int i = NQT == 2 ? k >> 1 : k, x = k & 1, slot = ring_v(i) % NS;
-      if (NQT == 1 || !x) {
-        wait(full(slot), (uint32_t)(ring_v(i) / NS) & 1u);
-        __syncwarp();
-        const int j0 = slot_of(i);
-        const uint32_t bm = badm[i & 7];
-        if (bm || j0 + TILE - 1 > ez || (a.window && j0 <= ea - a.window && j0 + TILE - 1 >= a.sinks)) {
-          uint8_t *d = smem + 1024 + C::QB + slot * GB;
-          for (int r = 0; r < TILE; r++) {
-            if (seen(j0 + r) && !(bm >> (r >> 4) & 1)) continue;
-            for (int w = lane; w < HD / 8; w += 32) *(uint4 *)(d + (w >> 3) * BLK + r * 128 + (w & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-      }
-      wait(p_full(x), (uint32_t)(k >> 1) & 1u);
+    auto value = [&](int i, int x) {
+      const int slot = ring_v(i) % NS;
+      if (!x) { wait(full(slot), (uint32_t)(ring_v(i) / NS) & 1u); __syncwarp(); }
+      wait(p_full(x, i), (uint32_t)(i >> 1) & 1u);         // (V's rows that nobody sees are zero by then, too)
       __syncwarp();
       t5_fence_after();
       const uint64_t vd = kp_desc(ring_s + slot * GB, BLK);
-      const uint32_t P = tmem + C::S + C::SC * (uint32_t)x, D = tmem + C::O + (NQT == 2 ? (uint32_t)(x * HD) : 0u);
+      const uint32_t P = tmem + C::S + (uint32_t)(TILE * (2 * x + (i & 1))), D = tmem + C::O + (uint32_t)(x * HD);
       if (el) {
 #pragma unroll
         for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(D, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
-        t5_commit(pv_done(NQT == 2 ? x : 0));
-        if (NQT == 1 || x) t5_commit(empty(slot));
+        t5_commit(pv_done(x));
+        if (x == streams - 1) t5_commit(empty(slot));
       }
       __syncwarp();
     };
-    score(0);
-    if (steps > 1) score(1);
+    // a stream's next scores go into the columns of the probabilities that the product in front of them has used
 #pragma unroll 1
-    for (int k = 0; k < steps; k++) {
-      value(k);
-      if (k + 2 < steps) score(k + 2);
-    }
+    for (int i = 0; i < min(n, 2); i++)
+#pragma unroll 1
+      for (int x = 0; x < streams; x++) score(i, x);
+#pragma unroll 1
+    for (int i = 0; i < n; i++)
+#pragma unroll 1
+      for (int x = 0; x < streams; x++) {
+        value(i, x);
+        if (i + 2 < n) score(i + 2, x);
+      }
   }
   // after a wait ran out nothing is requested any more, but copies may be on their way
   if (*dead) for (int i = 0; i < 64; i++) __nanosleep(1000);
