@@ -254,12 +254,13 @@ template <typename T, typename X> static int append_go(const KvDev &c, const KvR
   else CU_OK(llb_launch(k_kv_append<T, X, 256>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
   return 0;
 }
-// pages as [page][kv head][slot][dims], in boxes of 64 dims of `slots` slots of a kv head of a page
-static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int slots) {
+// pages as [page][kv head][64 dims][slot][dim], in boxes of `slots` slots and `blocks` times 64 dims of a kv head of a page
+static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int slots, int blocks) {
   const cuuint64_t row = (cuuint64_t)kv->head_dim * 2;
-  const cuuint64_t dim[4] = {(cuuint64_t)kv->head_dim, (cuuint64_t)kv->page, (cuuint64_t)kv->kv_heads, (cuuint64_t)kv->n_pages}, step[3] = {row, row * kv->page, row * kv->page * kv->kv_heads};
-  const cuuint32_t box[4] = {64, (cuuint32_t)slots, 1, 1}, one[4] = {1, 1, 1, 1};
-  const CUresult r = g_kv_map(map, kv->el == LLB_EL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)(uintptr_t)base, dim, step, box, one,
+  const cuuint64_t dim[5] = {64, (cuuint64_t)kv->page, (cuuint64_t)kv->head_dim / 64, (cuuint64_t)kv->kv_heads, (cuuint64_t)kv->n_pages};
+  const cuuint64_t step[4] = {row, 128, row * kv->page, row * kv->page * kv->kv_heads};
+  const cuuint32_t box[5] = {64, (cuuint32_t)slots, (cuuint32_t)blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = g_kv_map(map, kv->el == LLB_EL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, (void *)(uintptr_t)base, dim, step, box, one,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : llb_fail("kv: tensor map of %d pages: error %d", kv->n_pages, (int)r);
 }
@@ -289,7 +290,7 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   few_plan(kv, call, (uintptr_t)call->ws, &p);
   p.err = gemm_err_word();
   CUtensorMap km, vm;
-  if (pool_map(&km, kv, kv->k, KF_SLOTS) || pool_map(&vm, kv, kv->v, KF_SLOTS)) return -1;
+  if (pool_map(&km, kv, kv->k, KF_SLOTS, HD / 64) || pool_map(&vm, kv, kv->v, KF_SLOTS, HD / 64)) return -1;
   const dim3 grid(few_grid(kv)), block(32 * KF_WARPS);
   const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + 511) / 512;   // (attn_check: they fit)
   if (a.w_out) {
@@ -323,9 +324,9 @@ template <typename T, int HD> static int attn_go(const llb_kv *kv, const llb_kv_
   KvPfPlan p;
   pf_plan(kv, call, (uintptr_t)call->ws, &p);
   p.err = gemm_err_word();
-  const int slots = std::min(kv->page, Kp<HD>::TILE), tiles = pf_tiles(kv, call);
+  const int slots = std::min(kv->page, Kp<HD>::TILE), blocks = slots == Kp<HD>::TILE ? HD / 64 : 1, tiles = pf_tiles(kv, call);
   CUtensorMap km, vm;
-  if (pool_map(&km, kv, kv->k, slots) || pool_map(&vm, kv, kv->v, slots)) return -1;
+  if (pool_map(&km, kv, kv->k, slots, blocks) || pool_map(&vm, kv, kv->v, slots, blocks)) return -1;
   CU_OK(llb_launch(k_kv_pf<T, HD>, dim3(tiles * c.KV * c.seqs, p.splits), dim3(Kp<HD>::THREADS), (size_t)Kp<HD>::SMEM, g_llb.stream, c, rw, a, p, tiles, km, vm));
   if (p.splits > 1) CU_OK(llb_launch(k_kv_pf_join<T, HD>, dim3(rw.rows, (a.H + 3) / 4), dim3(128), (size_t)0, g_llb.stream, c, rw, a, p));
   return 0;
@@ -349,7 +350,7 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");
   if (a->w_in && !a->w_out) return llb_fail("kv_attn: w_in without w_out");
   const long long queries = (long long)a->heads / kv->kv_heads * most_rows(a), pairs = (long long)kv->seqs * kv->kv_heads;
-  if (queries > INT_MAX / 2 || pairs * (std::min(queries, (queries + 127) / 128 + KV_FEW) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
+  if (queries >= 1 << 26 || pairs * (std::min(queries, (queries + 127) / 128 + KV_FEW) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
     return llb_fail("kv_attn: %d sequences of %d kv heads, %d rows, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, most_rows(a), a->max_len);
   if (a->w_out) {
     if (off(a->w_in, 4) || off(a->w_out, 4)) return llb_fail("kv_attn: weights are f32 on the device");
@@ -447,7 +448,7 @@ int llb_b200_kv_attn(const llb_kv *kv, const llb_kv_attn *a) {
   const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, most_rows(a)};
   KvAttn k;
   k.q = (const uint16_t *)(uintptr_t)a->q; k.out = (void *)(uintptr_t)a->out;
-  k.qs = a->q_stride; k.os = a->out_stride; k.H = a->heads; k.G = a->heads / kv->kv_heads; k.window = a->window; k.sinks = a->sinks; k.out32 = a->el_out == LLB_EL_F32;
+  k.qs = a->q_stride; k.os = a->out_stride; k.H = a->heads; k.G = a->heads / kv->kv_heads; k.inv = (unsigned)(((1ull << 32) + k.G - 1) / k.G); k.window = a->window; k.sinks = a->sinks; k.out32 = a->el_out == LLB_EL_F32;
   k.scale2 = (float)((a->scale > 0.0f ? (double)a->scale : 1.0 / sqrt((double)kv->head_dim)) * 1.4426950408889634);
   k.w_in = (const float *)(uintptr_t)a->w_in; k.w_out = (float *)(uintptr_t)a->w_out; k.wstride = a->w_stride;
   if (kv->el == LLB_EL_F16) return kv->head_dim == 64 ? attn_go<__half, 64>(kv, a, c, rw, k) : kv->head_dim == 128 ? attn_go<__half, 128>(kv, a, c, rw, k) : attn_go<__half, 256>(kv, a, c, rw, k);

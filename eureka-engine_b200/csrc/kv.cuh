@@ -89,11 +89,14 @@ struct KvAttn {
   void *out;
   long long qs, os;            // elements between rows
   int H, G, window, sinks, out32;   // G: query heads a kv head
+  unsigned inv;                // 2^32 / G, rounded up
   float scale2;                // times log2(e): probabilities are powers of two
   const float *w_in;
   float *w_out;
   int wstride;
 };
+// row of a query i G + h: exact for fewer than 2^26 queries (kv_attn_check), G at most 64
+__device__ __forceinline__ int kv_row_of(const KvAttn &a, int q) { return a.G == 1 ? q : (int)__umulhi((unsigned)q, a.inv); }
 // one sequence's share of a call.  What its rows see is cut into chunks of `1 << sh` slots: cs of first tokens, then those from slot lo's on.
 struct KvSeq {
   int first, n, len;           // first row, rows; slots

@@ -57,9 +57,10 @@ __device__ __forceinline__ void kf_ldsm_t(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ float kv_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ void kv_tma(uint32_t dst_s, const CUtensorMap *map, int x, int slot, int g, int page, uint32_t bar_s) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst_s), "l"(map), "r"(x), "r"(slot),
-               "r"(g), "r"(page), "r"(bar_s)
+// a box of pool_map's: from 64 dims number d of kv head g's slot `slot` of a page on
+__device__ __forceinline__ void kv_tma(uint32_t dst_s, const CUtensorMap *map, int x, int slot, int d, int g, int page, uint32_t bar_s) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst_s), "l"(map), "r"(x), "r"(slot),
+               "r"(d), "r"(g), "r"(page), "r"(bar_s)
                : "memory");
 }
 __device__ __forceinline__ void kv_expect(uint32_t bar_s, uint32_t bytes) {
@@ -172,11 +173,8 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
       hd.bad[warp][st] = !in;
       if (in) {
         kv_expect(full, SB);
-#pragma unroll
-        for (int d = 0; d < HD / 64; d++) {
-          kv_tma(ring_s + st * SB + d * (KF_SLOTS * 128), &km, 64 * d, slot & ((1 << c.page_sh) - 1), get.g, gid_page, full);
-          kv_tma(ring_s + st * SB + KB + d * (KF_SLOTS * 128), &vm, 64 * d, slot & ((1 << c.page_sh) - 1), get.g, gid_page, full);
-        }
+        kv_tma(ring_s + st * SB, &km, 0, slot & ((1 << c.page_sh) - 1), 0, get.g, gid_page, full);
+        kv_tma(ring_s + st * SB + KB, &vm, 0, slot & ((1 << c.page_sh) - 1), 0, get.g, gid_page, full);
       } else {
         if (get.s.e0 + get.s.nc > 0) atomicOr(c.err, KV_ERR_PAGE);
         mbar_arrive(full);

@@ -11,7 +11,9 @@
 // K and V come by TMA, a page's part of a tile each, in rows of 128 swizzled bytes.  A slot that no row of the block sees is zeroed in V before
 // the product (whatever the page holds there, 0 times it has to be 0).
 //
-// Warps: softmax (4 a query tile), one that loads, one that issues the MMAs.  Every wait is bounded.
+// Warps: softmax (4 a query tile), one that loads K, one that loads V, one a stream that issues its MMAs: an MMA is issued when the one before has
+// begun, so that a warp's time between two products (its waits, its commits) is the tensor core's too, unless the other stream's warp has
+// products in line.  Every wait is bounded.
 #pragma once
 #include "kvatt.cuh"
 
@@ -20,9 +22,9 @@ template <int HD> struct Kp {
   static constexpr int TILE = 64, SH = 6;                  // slots
   static constexpr int GB = TILE * HD * 2;                 // bytes of a tile of K or V
   static constexpr int QB = HD == 256 ? 0 : NQT * 128 * HD * 2;
-  static constexpr int NS = HD == 256 ? 7 : HD == 128 ? 10 : 12;
-  static constexpr int SMEM = 1024 + QB + NS * GB;
-  static constexpr int SOFT = 4 * NQT, THREADS = 32 * (SOFT + 2);
+  static constexpr int NK = HD == 256 ? 3 : HD == 128 ? 5 : 6, NV = HD == 256 ? 4 : NK;   // tiles of K and of V that have room
+  static constexpr int SMEM = 1024 + QB + (NK + NV) * GB;
+  static constexpr int SOFT = 4 * NQT, THREADS = 32 * (SOFT + 2 + NQT);
   static constexpr uint32_t O = 0, S = HD == 256 ? 384 : 256, Q = 256;   // tensor memory's columns; S: two tiles a stream
 };
 static_assert(Kp<256>::SMEM <= 232448 && Kp<128>::SMEM <= 232448 && Kp<64>::SMEM <= 232448, "shared memory");
@@ -68,16 +70,36 @@ __device__ __forceinline__ void kp_ld32(uint32_t taddr, float *v) {
 
 __device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }   // the n lowest bits
 
+// 2^y of two numbers by the FMA pipe (y <= 127): the whole part into the exponent, 2^f on [-1/2, 1/2] by the polynomial of degree four whose largest relative
+// error is smallest (2.7e-6 in f32; coefficients by Remez's exchange).  The special function unit takes a warp's 32 in eight cycles.
+__device__ __forceinline__ void kp_exp2_fma(f32x2 y, float &r0, float &r1) {
+  float a, b;
+  x2_unpack(y, a, b);
+  y = x2_pack(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const f32x2 big = x2_pack(12582912.0f, 12582912.0f), one = x2_pack(-1.0f, -1.0f);
+  const f32x2 t = x2_add(y, big), f = x2_add(y, x2_fma(t, one, big));      // (t's low bits: the whole part)
+  f32x2 v = x2_fma(x2_pack(0.009570102207362652f, 0.009570102207362652f), f, x2_pack(0.05591785907745361f, 0.05591785907745361f));
+  v = x2_fma(v, f, x2_pack(0.240247443318367f, 0.240247443318367f));
+  v = x2_fma(v, f, x2_pack(0.6931217908859253f, 0.6931217908859253f));
+  v = x2_fma(v, f, x2_pack(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1;
+  x2_unpack(t, t0, t1);
+  x2_unpack(v, a, b);
+  r0 = __int_as_float(__float_as_int(a) + (__float_as_int(t0) << 23));
+  r1 = __int_as_float(__float_as_int(b) + (__float_as_int(t1) << 23));
+}
+#define KP_FMA_EVERY 4         // every fourth pair of probabilities goes that way
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p, int tiles, const __grid_constant__ CUtensorMap km,
                                                               const __grid_constant__ CUtensorMap vm) {
   using C = Kp<HD>;
-  constexpr int NQT = C::NQT, TILE = C::TILE, SH = C::SH, GB = C::GB, NS = C::NS, QT = 128 * NQT, BLK = TILE * 128;   // BLK: 64 dims of a tile
+  constexpr int NQT = C::NQT, TILE = C::TILE, SH = C::SH, GB = C::GB, NK = C::NK, NV = C::NV, QT = 128 * NQT, BLK = TILE * 128;   // BLK: 64 dims of a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t bar_s = smem_u32(smem), q_s = bar_s + 1024, ring_s = q_s + C::QB;
-  auto full = [&](int s) { return bar_s + 8u * (uint32_t)s; };
-  auto empty = [&](int s) { return bar_s + 96u + 8u * (uint32_t)s; };
+  const uint32_t bar_s = smem_u32(smem), q_s = bar_s + 1024, ring_s = q_s + C::QB, ringv_s = ring_s + NK * GB;
+  auto full = [&](bool v, int s) { return bar_s + (v ? 96u : 0u) + 8u * (uint32_t)s; };
+  auto empty = [&](bool v, int s) { return bar_s + (v ? 144u : 48u) + 8u * (uint32_t)s; };
   auto s_full = [&](int x, int i) { return bar_s + 192u + 8u * (uint32_t)(2 * x + (i & 1)); };
   auto p_full = [&](int x, int i) { return bar_s + 224u + 8u * (uint32_t)(2 * x + (i & 1)); };
   auto pv_done = [&](int x) { return bar_s + 256u + 8u * (uint32_t)x; };
@@ -91,7 +113,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, SH);
   const int NQ = a.G * s.nc, q0 = tile * QT;
   if (q0 >= NQ) return;
-  const int ea = s.e0 + q0 / a.G, ez = s.e0 + min(q0 + QT - 1, NQ - 1) / a.G;   // slots of the first and the last row
+  const int ea = s.e0 + kv_row_of(a, q0), ez = s.e0 + kv_row_of(a, min(q0 + QT - 1, NQ - 1));   // slots of the first and the last row
   const KpTiles kt = kp_tiles<SH>(ea, ez, a.window, a.sinks);
   const int per = (kt.n + p.splits - 1) / p.splits, t0 = min(kt.n, split * per), n = min(kt.n, t0 + per) - t0;
   auto slot_of = [&](int i) { i += t0; return (i < kt.cs ? i : kt.lo + i - kt.cs) << SH; };
@@ -100,20 +122,21 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   if (!n) {
     for (int qi = q0 + tid; qi < min(q0 + QT, NQ); qi += C::THREADS) {
       if (p.splits > 1) { p.pm[part_of(qi)] = -INFINITY; p.pl[part_of(qi)] = 0.0f; continue; }
-      const long long at = (long long)(s.first + qi / a.G) * a.os + (long long)(g * a.G + qi % a.G) * HD;
+      const long long at = (long long)(s.first + kv_row_of(a, qi)) * a.os + (long long)(g * a.G + qi - kv_row_of(a, qi) * a.G) * HD;
       for (int d = 0; d < HD * (a.out32 ? 4 : 2); d += 16) *(uint4 *)((uint8_t *)a.out + at * (a.out32 ? 4 : 2) + d) = make_uint4(0, 0, 0, 0);
     }
     return;
   }
   if (tid == 0) {
-    for (int i = 0; i < NS; i++) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
+    const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
+    for (int i = 0; i < 12; i++) { mbar_init(full(i >= 6, i % 6), 1); mbar_init(empty(i >= 6, i % 6), streams); }
     for (int x = 0; x < 4; x++) { mbar_init(s_full(x >> 1, x), 1); mbar_init(p_full(x >> 1, x), 4); }
     mbar_init(pv_done(0), 1); mbar_init(pv_done(1), 1);
-    mbar_init(q_full, NQT == 2 && q0 + 128 < NQ ? 8 : 4);
+    mbar_init(q_full, 4 * streams);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == C::SOFT + 1) {
+  if (warp == C::SOFT + 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -128,17 +151,14 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       if (k >= T5_WAIT_LIMIT) { *dead = 1; atomicExch(p.err, 1u); return; }
     }
   };
-  // tiles of K and V in the order in which they are first used
-  auto ring_k = [&](int i) { return i ? 2 * i - 1 : 0; };
-  auto ring_v = [&](int i) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; };
   const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
 
   if (warp < 4 * streams) {
     // ---- softmax: a thread a query ----
-    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = s.e0 + min(qi, NQ - 1) / a.G, lw = a.window ? e - a.window + 1 : 0;
+    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = s.e0 + kv_row_of(a, min(qi, NQ - 1)), lw = a.window ? e - a.window + 1 : 0;
     const uint32_t lq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     {
-      const uint16_t *src = a.q + (long long)(s.first + qi / a.G) * a.qs + (long long)(g * a.G + qi % a.G) * HD;
+      const uint16_t *src = a.q + (long long)(s.first + kv_row_of(a, qi)) * a.qs + (long long)(g * a.G + qi - kv_row_of(a, qi) * a.G) * HD;
 #pragma unroll
       for (int d0 = 0; d0 < HD; d0 += 64) {
         uint32_t v[32];
@@ -162,7 +182,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     }
     float m = -INFINITY, l = 0.0f;
     // slots of this query tile's first and last row: a tile between what they see is seen whole by every row
-    const int qa = q0 + 128 * x0, ra = s.e0 + qa / a.G, rz = s.e0 + min(qa + 127, NQ - 1) / a.G;
+    const int qa = q0 + 128 * x0, ra = s.e0 + kv_row_of(a, qa), rz = s.e0 + kv_row_of(a, min(qa + 127, NQ - 1));
 #pragma unroll 1
     for (int i = 0; i < n; i++) {
       const int slot = slot_of(i);
@@ -226,8 +246,9 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
 #pragma unroll
         for (int k = 0; k < 32; k++) {
           float y0, y1;
-          x2_unpack(x2_fma(x2_pack(v[k0 + 2 * k], v[k0 + 2 * k + 1]), sc2, rf2), y0, y1);
-          y0 = kv_exp2(y0); y1 = kv_exp2(y1);
+          const f32x2 y = x2_fma(x2_pack(v[k0 + 2 * k], v[k0 + 2 * k + 1]), sc2, rf2);
+          if (k % KP_FMA_EVERY == KP_FMA_EVERY - 1) kp_exp2_fma(y, y0, y1);
+          else { x2_unpack(y, y0, y1); y0 = kv_exp2(y0); y1 = kv_exp2(y1); }
           sum[k & 1] = x2_add(sum[k & 1], x2_pack(y0, y1));
           w[k] = KvEl<T>::of2(y0, y1);
         }
@@ -237,13 +258,14 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       x2_unpack(x2_add(sum[0], sum[1]), a0, a1);
       l += a0 + a1;
       // slots that no row of the block sees: their V is taken out, whatever the page holds, before the first product with the tile
-      if (x0 == 0 && (bm || slot + TILE - 1 > ez || (a.window && slot <= ea - a.window && slot + TILE - 1 >= a.sinks))) {
-        const int rs = ring_v(i) % NS;
-        wait(full(rs), (uint32_t)(ring_v(i) / NS) & 1u);
-        const uint32_t at = ring_s + rs * GB;
+      // (every stream's warps do it: what is zero is written as zero again)
+      if (bm || slot + TILE - 1 > ez || (a.window && slot <= ea - a.window && slot + TILE - 1 >= a.sinks)) {
+        const int rs = i % NV;
+        wait(full(true, rs), (uint32_t)(i / NV) & 1u);
+        const uint32_t at = ringv_s + rs * GB;
         auto clear = [&](int ra, int rz) {                 // rows ra .. rz - 1 of the tile
 #pragma unroll 1
-          for (int w = ra * (HD / 8) + tid; w < rz * (HD / 8); w += 128) {
+          for (int w = ra * (HD / 8) + (tid & 127); w < rz * (HD / 8); w += 128) {
             const int r = w / (HD / 8), d = w % (HD / 8);  // a row's 16 bytes, in the order in which they lie
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (d >> 3) * BLK + r * 128 + ((d & 7) << 4)), "r"(0) : "memory");
           }
@@ -266,11 +288,11 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     __syncwarp();
     t5_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float chk = l;
+    float chk[4] = {l, 0.0f, 0.0f, 0.0f};
     if (p.splits > 1 && qi < NQ) { const size_t part = part_of(qi); p.pm[part] = m; p.pl[part] = l; }
-    // whole 128-byte pieces of rows, turned in the ring's memory: every product is done
+    // whole 128-byte pieces of rows, turned in memory that no product reads any more: the stream's queries', or the rings where it is the only stream
     const bool wide = p.splits > 1 || a.out32;             // 32 dims a piece, or 64
-    const uint32_t st = ring_s + (uint32_t)warp * 4096u;
+    const uint32_t st = (HD == 256 ? ring_s : q_s + x0 * (128 * HD * 2)) + (uint32_t)(warp & 3) * 4096u;
     uint8_t *dst[8];                                       // rows 4 k + lane / 8 of the warp's
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -278,18 +300,19 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       dst[k] = nullptr;
       if (qk >= NQ) continue;
       if (p.splits > 1) dst[k] = (uint8_t *)(p.po + part_of(qk) * HD);
-      else dst[k] = (uint8_t *)a.out + ((long long)(s.first + qk / a.G) * a.os + (long long)(g * a.G + qk % a.G) * HD) * (a.out32 ? 4 : 2);
+      else dst[k] = (uint8_t *)a.out + ((long long)(s.first + kv_row_of(a, qk)) * a.os + (long long)(g * a.G + qk - kv_row_of(a, qk) * a.G) * HD) * (a.out32 ? 4 : 2);
       dst[k] += 16 * (lane & 7);
     }
     auto piece = [&](int at) {
+      uint32_t w[8][4];
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+      for (int k = 0; k < 8; k++)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
                      : "r"(st + (4 * k + (lane >> 3)) * 128 + (((lane & 7) ^ ((4 * k + (lane >> 3)) & 7)) << 4)) : "memory");
-        if (dst[k]) *(uint4 *)(dst[k] + at) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (dst[k]) *(uint4 *)(dst[k] + at) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
       __syncwarp();
     };
     auto put = [&](int k, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
@@ -304,7 +327,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         t5_wait_ld();
         if (p.splits == 1) {
 #pragma unroll
-          for (int k = 0; k < 32; k++) { chk += o[k] * 0.0f; o[k] *= inv; }
+          for (int k = 0; k < 32; k++) { chk[k & 3] += o[k] * 0.0f; o[k] *= inv; }
         }
         if (wide) {
 #pragma unroll
@@ -319,7 +342,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       }
     }
     // rows whose result is no number once more, by themselves (kv_attn_row says why)
-    unsigned redo = __ballot_sync(0xffffffffu, p.splits == 1 && qi < NQ && !(fabsf(chk) < INFINITY));
+    unsigned redo = __ballot_sync(0xffffffffu, p.splits == 1 && qi < NQ && !(fabsf((chk[0] + chk[1]) + (chk[2] + chk[3])) < INFINITY));
     while (redo) {
       const int k = __ffs(redo) - 1, qk = q0 + 128 * x0 + 32 * (warp & 3) + k, rk = qk / a.G;
       redo &= redo - 1;
@@ -329,10 +352,13 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     }
   } else if (warp < C::SOFT) {
     // (the second query tile is behind the last query)
-  } else if (warp == C::SOFT) {
-    // ---- K and V: a lane a page's part of a tile ----
-    const int bs = min(c.page_sh, SH), boxes = TILE >> bs;
-    // the lane's entry of tile i's pages, asked for two tiles before its use; -2: nothing that a row sees
+  } else if (warp < C::SOFT + 2) {
+    // ---- K, or V: the pages' parts of a tile ----
+    const bool isv = warp == C::SOFT + 1;
+    const CUtensorMap *map = isv ? &vm : &km;
+    const int bs = min(c.page_sh, SH), boxes = TILE >> bs, N = isv ? NV : NK;
+    const uint32_t ring = isv ? ringv_s : ring_s;
+    // the lane's entry of tile i's pages, asked for a tile before its use; -2: nothing that a row sees
     struct Entry { int id; bool on; };
     auto entry = [&](int i) {
       Entry x = {-2, false};
@@ -343,55 +369,57 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       }
       return x;
     };
-    auto use = [&](Entry x) { asm volatile("" : "+r"(x.id)); return x.on ? x.id : -2; };     // (the load is not waited for before)
-    auto load = [&](const CUtensorMap *map, int t, int i, int id, bool isk) {
-      const int slot = t % NS;
-      if (t >= NS) wait(empty(slot), (uint32_t)(t / NS - 1) & 1u);
-      __syncwarp();
-      const bool in = (unsigned)id < (unsigned)c.n_pages, wrong = !in && id != -2;
-      const unsigned have = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, wrong);
-      if (wrong) atomicOr(c.err, KV_ERR_PAGE);
-      if (lane == 0) {
-        if (isk) {
-          uint32_t bm = 0;
-          for (int k = 0; k < boxes; k++) if (lost >> k & 1) bm |= ((1u << (1 << (bs - 4))) - 1) << (k << (bs - 4));
-          badm[i & 15] = bm;
-        }
-        if (!*dead && have) kv_expect(full(slot), (uint32_t)__popc(have) * (HD / 64) * (128u << bs));
-        else mbar_arrive(full(slot));
-      }
-      __syncwarp();
-      if (in && !*dead) {
-        const int j = slot_of(i) + (lane << bs);
-#pragma unroll
-        for (int d = 0; d < HD / 64; d++) kv_tma(ring_s + slot * GB + d * BLK + (lane << bs) * 128, map, 64 * d, j & ((1 << c.page_sh) - 1), g, id, full(slot));
-      }
-      __syncwarp();
-    };
-    Entry next = entry(1);
-    int now = use(entry(0)), t = 0;
-    load(&km, t++, 0, now, true);
+    Entry next = entry(0);
+    int slot = 0;
+    uint32_t round = 0;
 #pragma unroll 1
     for (int i = 0; i < n; i++) {
-      const Entry later = entry(i + 2);
-      const int then = use(next);
-      if (i + 1 < n) load(&km, t++, i + 1, then, true);
-      load(&vm, t++, i, now, false);
-      now = then; next = later;
+      asm volatile("" : "+r"(next.id));                    // (the load is not waited for before)
+      const int id = next.on ? next.id : -2;
+      next = entry(i + 1);
+      if (round) wait(empty(isv, slot), (round - 1) & 1u);
+      __syncwarp();
+      const bool in = (unsigned)id < (unsigned)c.n_pages;
+      const unsigned have = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, !in && id != -2);
+      const uint32_t bar = full(isv, slot), at = ring + slot * GB;
+      const int j = slot_of(i) & ((1 << c.page_sh) - 1);   // (where a tile has several pages, the first slot of each)
+      if (lane == 0) {
+        if (lost) atomicOr(c.err, KV_ERR_PAGE);
+        if (!isv) {
+          uint32_t bm = 0;
+          for (int k = 0; lost && k < boxes; k++) if (lost >> k & 1) bm |= ((1u << (1 << (bs - 4))) - 1) << (k << (bs - 4));
+          badm[i & 15] = bm;
+        }
+        if (!*dead && have) kv_expect(bar, (uint32_t)__popc(have) * (HD / 64) * (128u << bs));
+        else mbar_arrive(bar);
+        if (!*dead && boxes == 1 && have) kv_tma(at, map, 0, j, 0, g, id, bar);              // one box of all dims
+      }
+      if (boxes > 1) {
+        __syncwarp();
+        if (in && !*dead) {
+#pragma unroll
+          for (int d = 0; d < HD / 64; d++) kv_tma(at + d * BLK + (lane << bs) * 128, map, 0, j, d, g, id, bar);
+        }
+      }
+      __syncwarp();
+      if (++slot == N) { slot = 0; round++; }
     }
-  } else {
-    // ---- the tensor core: the whole warp walks, an elected lane issues ----
+  } else if (warp < C::SOFT + 2 + streams) {
+    // ---- the tensor core, a warp a stream: the whole warp walks, an elected lane issues ----
     const bool el = t5_elect();
+    const int x = warp - C::SOFT - 2;
     constexpr uint32_t ids = kp_idesc<T>(TILE, false), ido = kp_idesc<T>(HD, true);
+    const uint64_t k0 = kp_desc(ring_s, 16), v0 = kp_desc(ringv_s, BLK), qd = kp_desc(q_s + x * (128 * HD * 2), 16);
+    const uint32_t S0 = tmem + C::S + (uint32_t)(2 * TILE * x), O = tmem + C::O + (uint32_t)(x * HD);
+    int ks = 0, vs = 0;
+    uint32_t kp = 0, vp = 0;                               // ring places and their phases
     wait(q_full, 0);
     __syncwarp();
-    t5_fence_after();
-    auto score = [&](int i, int x) {
-      const int slot = ring_k(i) % NS;
-      if (!x) { wait(full(slot), (uint32_t)(ring_k(i) / NS) & 1u); __syncwarp(); }
+    auto score = [&](int i) {                              // (its K is there)
+      __syncwarp();
       t5_fence_after();
-      const uint32_t D = tmem + C::S + (uint32_t)(TILE * (2 * x + (i & 1)));
-      const uint64_t kd = kp_desc(ring_s + slot * GB, 16), qd = kp_desc(q_s + x * (128 * HD * 2), 16);
+      const uint32_t D = S0 + (uint32_t)(TILE * (i & 1));
+      const uint64_t kd = k0 + (uint64_t)(ks * (GB / 16));
       if (el) {
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) {
@@ -400,45 +428,41 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
           else kp_ss(D, qd + (uint64_t)((d >> 2) * (128 * 128 / 16) + 2 * (d & 3)), kk, ids, d != 0);
         }
         t5_commit(s_full(x, i));
-        if (x == streams - 1) t5_commit(empty(slot));
+        t5_commit(empty(false, ks));
       }
       __syncwarp();
+      if (++ks == NK) { ks = 0; kp ^= 1u; }
     };
-    auto value = [&](int i, int x) {
-      const int slot = ring_v(i) % NS;
-      if (!x) { wait(full(slot), (uint32_t)(ring_v(i) / NS) & 1u); __syncwarp(); }
+    wait(full(false, 0), 0);
+    score(0);
+    if (n > 1) { wait(full(false, ks), kp); score(1); }
+    wait(full(true, 0), 0);
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
       wait(p_full(x, i), (uint32_t)(i >> 1) & 1u);         // (V's rows that nobody sees are zero by then, too)
       __syncwarp();
       t5_fence_after();
-      const uint64_t vd = kp_desc(ring_s + slot * GB, BLK);
-      const uint32_t P = tmem + C::S + (uint32_t)(TILE * (2 * x + (i & 1))), D = tmem + C::O + (uint32_t)(x * HD);
+      const uint64_t vd = v0 + (uint64_t)(vs * (GB / 16));
+      const uint32_t P = S0 + (uint32_t)(TILE * (i & 1));
       if (el) {
 #pragma unroll
-        for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(D, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
+        for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(O, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
         t5_commit(pv_done(x));
-        if (x == streams - 1) t5_commit(empty(slot));
+        t5_commit(empty(true, vs));
       }
       __syncwarp();
-    };
-    // a stream's next scores go into the columns of the probabilities that the product in front of them has used
-#pragma unroll 1
-    for (int i = 0; i < min(n, 2); i++)
-#pragma unroll 1
-      for (int x = 0; x < streams; x++) score(i, x);
-#pragma unroll 1
-    for (int i = 0; i < n; i++)
-#pragma unroll 1
-      for (int x = 0; x < streams; x++) {
-        value(i, x);
-        if (i + 2 < n) score(i + 2, x);
-      }
+      if (++vs == NV) { vs = 0; vp ^= 1u; }
+      // what comes next is waited for while this product runs
+      if (i + 1 < n) wait(full(true, vs), vp);
+      if (i + 2 < n) { wait(full(false, ks), kp); score(i + 2); }   // into the columns of the probabilities that have just been used
+    }
   }
   // after a wait ran out nothing is requested any more, but copies may be on their way
   if (*dead) for (int i = 0; i < 64; i++) __nanosleep(1000);
   __syncwarp();
   t5_fence_before();
   __syncthreads();
-  if (warp == C::SOFT + 1) {
+  if (warp == C::SOFT + 2) {
     t5_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
