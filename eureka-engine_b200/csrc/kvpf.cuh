@@ -127,8 +127,37 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     }
     return;
   }
+  const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
+  // a softmax warp's 32 queries are asked for before the block meets: four rows of 128 bytes a load
+  uint4 qw[HD / 64][8];
+  if (warp < 4 * streams) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int qk = q0 + 32 * warp + 4 * k + (lane >> 3);
+      const uint16_t *src = a.q + (long long)(s.first + kv_row_of(a, qk)) * a.qs + (long long)(g * a.G + qk - kv_row_of(a, qk) * a.G) * HD + 8 * (lane & 7);
+#pragma unroll
+      for (int d = 0; d < HD / 64; d++) {
+        qw[d][k] = make_uint4(0, 0, 0, 0);                 // (a choice between the load and zeros would wait for the load)
+        if (qk < NQ)
+          asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(qw[d][k].x), "=r"(qw[d][k].y), "=r"(qw[d][k].z), "=r"(qw[d][k].w) : "l"(src + 64 * d));
+      }
+    }
+  }
+  const int bs = min(c.page_sh, SH), boxes = TILE >> bs;   // slots of a page's part of a tile, and how many parts
+  // a loading lane's entry of tile i's pages, asked for a tile before its use; -2: nothing that a row sees
+  struct Entry { int id; bool on; };
+  auto entry = [&](int i) {
+    Entry x = {-2, false};
+    if (lane < boxes && i < n) {
+      const int j = slot_of(i) + (lane << bs);
+      x.on = j <= ez && (!a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks);   // (what is seen is one run of slots and the first ones)
+      if (x.on) asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(x.id) : "l"(c.table + (size_t)b * c.tstride + (j >> c.page_sh)));
+    }
+    return x;
+  };
+  Entry first = {-2, false};
+  if (warp == C::SOFT || warp == C::SOFT + 1) first = entry(0);
   if (tid == 0) {
-    const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
     for (int i = 0; i < 12; i++) { mbar_init(full(i >= 6, i % 6), 1); mbar_init(empty(i >= 6, i % 6), streams); }
     for (int x = 0; x < 4; x++) { mbar_init(s_full(x >> 1, x), 1); mbar_init(p_full(x >> 1, x), 4); }
     mbar_init(pv_done(0), 1); mbar_init(pv_done(1), 1);
@@ -151,32 +180,43 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       if (k >= T5_WAIT_LIMIT) { *dead = 1; atomicExch(p.err, 1u); return; }
     }
   };
-  const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
 
   if (warp < 4 * streams) {
     // ---- softmax: a thread a query ----
     const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = s.e0 + kv_row_of(a, min(qi, NQ - 1)), lw = a.window ? e - a.window + 1 : 0;
     const uint32_t lq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    // the queries: into shared memory as the product reads them, or through the last place of V's ring into tensor memory, 128 dims at a time
     {
-      const uint16_t *src = a.q + (long long)(s.first + kv_row_of(a, qi)) * a.qs + (long long)(g * a.G + qi - kv_row_of(a, qi) * a.G) * HD;
+      constexpr int PART = HD == 256 ? 2 : HD / 64;        // 64 dims at a time
+      const uint32_t to = HD == 256 ? ringv_s + (NV - 1) * GB + (uint32_t)warp * 8192u : q_s + x0 * (128 * HD * 2) + (uint32_t)(warp & 3) * 4096u;
 #pragma unroll
-      for (int d0 = 0; d0 < HD; d0 += 64) {
-        uint32_t v[32];
+      for (int d0 = 0; d0 < HD / 64; d0 += PART) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const uint4 w = qi < NQ ? __ldg((const uint4 *)(src + d0) + i) : make_uint4(0, 0, 0, 0);
-          v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
-        }
-        if constexpr (HD == 256) t5_st32(lq + C::Q + d0 / 2, v);
-        else {
-          const int r = tid & 127;
-          uint8_t *d = smem + 1024 + x0 * (128 * HD * 2) + (d0 >> 6) * (128 * 128) + r * 128;
+        for (int d = 0; d < PART; d++)
 #pragma unroll
-          for (int i = 0; i < 8; i++) *(uint4 *)(d + ((i ^ (r & 7)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          for (int k = 0; k < 8; k++) {
+            const int r = 4 * k + (lane >> 3);
+            const uint4 w = qw[d0 + d][k];
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + d * (HD == 256 ? 4096 : 128 * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), "r"(w.x), "r"(w.y), "r"(w.z),
+                         "r"(w.w)
+                         : "memory");
+          }
+        if constexpr (HD == 256) {
+          __syncwarp();
+#pragma unroll
+          for (int d = 0; d < 2; d++) {
+            uint32_t v[32];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4 * i]), "=r"(v[4 * i + 1]), "=r"(v[4 * i + 2]), "=r"(v[4 * i + 3])
+                           : "r"(to + d * 4096 + lane * 128 + ((i ^ (lane & 7)) << 4)) : "memory");
+            t5_st32(lq + C::Q + 32 * (d0 + d), v);
+          }
+          __syncwarp();
         }
       }
       if constexpr (HD == 256) { t5_wait_st(); t5_fence_before(); }
-      else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
@@ -320,25 +360,31 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     };
 #pragma unroll 1
     for (int d = 0; d < HD; d += 64) {
+      float o[64];
+      kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d), o);
+      kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d + 32), o + 32);
+      t5_wait_ld();
+      if (p.splits == 1) {
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        float o[32];
-        kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d + 32 * half), o);
-        t5_wait_ld();
-        if (p.splits == 1) {
+        for (int k = 0; k < 64; k++) { chk[k & 3] += o[k] * 0.0f; o[k] *= inv; }
+      }
+      if (wide) {
 #pragma unroll
-          for (int k = 0; k < 32; k++) { chk[k & 3] += o[k] * 0.0f; o[k] *= inv; }
-        }
-        if (wide) {
+        for (int half = 0; half < 2; half++) {
 #pragma unroll
-          for (int k = 0; k < 8; k++) put(k, __float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
+          for (int k = 0; k < 8; k++) {
+            const float *w = o + 32 * half + 4 * k;
+            put(k, __float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
+          }
           piece(4 * (d + 32 * half));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            put(4 * half + k, KvEl<T>::of2(o[8 * k], o[8 * k + 1]), KvEl<T>::of2(o[8 * k + 2], o[8 * k + 3]), KvEl<T>::of2(o[8 * k + 4], o[8 * k + 5]), KvEl<T>::of2(o[8 * k + 6], o[8 * k + 7]));
-          if (half) piece(2 * d);
         }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const float *w = o + 8 * k;
+          put(k, KvEl<T>::of2(w[0], w[1]), KvEl<T>::of2(w[2], w[3]), KvEl<T>::of2(w[4], w[5]), KvEl<T>::of2(w[6], w[7]));
+        }
+        piece(2 * d);
       }
     }
     // rows whose result is no number once more, by themselves (kv_attn_row says why)
@@ -356,20 +402,9 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     // ---- K, or V: the pages' parts of a tile ----
     const bool isv = warp == C::SOFT + 1;
     const CUtensorMap *map = isv ? &vm : &km;
-    const int bs = min(c.page_sh, SH), boxes = TILE >> bs, N = isv ? NV : NK;
+    const int N = isv ? NV : NK;
     const uint32_t ring = isv ? ringv_s : ring_s;
-    // the lane's entry of tile i's pages, asked for a tile before its use; -2: nothing that a row sees
-    struct Entry { int id; bool on; };
-    auto entry = [&](int i) {
-      Entry x = {-2, false};
-      if (lane < boxes && i < n) {
-        const int j = slot_of(i) + (lane << bs);
-        x.on = j <= ez && (!a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks);   // (what is seen is one run of slots and the first ones)
-        if (x.on) asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(x.id) : "l"(c.table + (size_t)b * c.tstride + (j >> c.page_sh)));
-      }
-      return x;
-    };
-    Entry next = entry(0);
+    Entry next = first;
     int slot = 0;
     uint32_t round = 0;
 #pragma unroll 1
@@ -378,6 +413,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       const int id = next.on ? next.id : -2;
       next = entry(i + 1);
       if (round) wait(empty(isv, slot), (round - 1) & 1u);
+      else if (HD == 256 && isv && slot == NV - 1) wait(q_full, 0);   // (the queries come through it)
       __syncwarp();
       const bool in = (unsigned)id < (unsigned)c.n_pages;
       const unsigned have = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, !in && id != -2);
@@ -405,56 +441,59 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       if (++slot == N) { slot = 0; round++; }
     }
   } else if (warp < C::SOFT + 2 + streams) {
-    // ---- the tensor core, a warp a stream: the whole warp walks, an elected lane issues ----
-    const bool el = t5_elect();
-    const int x = warp - C::SOFT - 2;
-    constexpr uint32_t ids = kp_idesc<T>(TILE, false), ido = kp_idesc<T>(HD, true);
-    const uint64_t k0 = kp_desc(ring_s, 16), v0 = kp_desc(ringv_s, BLK), qd = kp_desc(q_s + x * (128 * HD * 2), 16);
-    const uint32_t S0 = tmem + C::S + (uint32_t)(2 * TILE * x), O = tmem + C::O + (uint32_t)(x * HD);
-    int ks = 0, vs = 0;
-    uint32_t kp = 0, vp = 0;                               // ring places and their phases
-    wait(q_full, 0);
-    __syncwarp();
-    auto score = [&](int i) {                              // (its K is there)
-      __syncwarp();
-      t5_fence_after();
-      const uint32_t D = S0 + (uint32_t)(TILE * (i & 1));
-      const uint64_t kd = k0 + (uint64_t)(ks * (GB / 16));
-      if (el) {
+    // ---- the tensor core, a thread a stream ----
+    if (t5_elect()) {
+      const int x = warp - C::SOFT - 2;
+      constexpr uint32_t ids = kp_idesc<T>(TILE, false), ido = kp_idesc<T>(HD, true);
+      const uint64_t k0 = kp_desc(ring_s, 16), v0 = kp_desc(ringv_s, BLK), qd = kp_desc(q_s + x * (128 * HD * 2), 16);
+      const uint32_t S0 = tmem + C::S + (uint32_t)(2 * TILE * x), O = tmem + C::O + (uint32_t)(x * HD);
+      int ks = 0, vs = 0;
+      uint32_t kp = 0, vp = 0;                             // ring places and their phases
+      auto score = [&](int i, uint32_t look, uint32_t phase) {   // (its K is there); looks at a barrier on the way
+        const uint32_t D = S0 + (uint32_t)(TILE * (i & 1));
+        const uint64_t kd = k0 + (uint64_t)(ks * (GB / 16));
+        bool seen = false;
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) {
           const uint64_t kk = kd + (uint64_t)((d >> 2) * (BLK / 16) + 2 * (d & 3));
+          // (an issue waits until the MMA two in front of it is done: the look fits between the last ones)
+          if (d == HD / 16 - 2 && look) seen = mbar_wait(look, phase, 1);
           if constexpr (HD == 256) t5_mma_f16_ts(D, tmem + C::Q + 8 * d, kk, ids, d != 0);
           else kp_ss(D, qd + (uint64_t)((d >> 2) * (128 * 128 / 16) + 2 * (d & 3)), kk, ids, d != 0);
         }
         t5_commit(s_full(x, i));
         t5_commit(empty(false, ks));
-      }
-      __syncwarp();
-      if (++ks == NK) { ks = 0; kp ^= 1u; }
-    };
-    wait(full(false, 0), 0);
-    score(0);
-    if (n > 1) { wait(full(false, ks), kp); score(1); }
-    wait(full(true, 0), 0);
-#pragma unroll 1
-    for (int i = 0; i < n; i++) {
-      wait(p_full(x, i), (uint32_t)(i >> 1) & 1u);         // (V's rows that nobody sees are zero by then, too)
-      __syncwarp();
+        if (++ks == NK) { ks = 0; kp ^= 1u; }
+        return seen;
+      };
+      wait(q_full, 0);
+      wait(full(false, 0), 0);
       t5_fence_after();
-      const uint64_t vd = v0 + (uint64_t)(vs * (GB / 16));
-      const uint32_t P = S0 + (uint32_t)(TILE * (i & 1));
-      if (el) {
+      score(0, 0, 0);
+      if (n > 1) { wait(full(false, ks), kp); t5_fence_after(); score(1, 0, 0); }
+      wait(full(true, 0), 0);
+      bool seen = false;
+#pragma unroll 1
+      for (int i = 0; i < n; i++) {
+        if (!seen) wait(p_full(x, i), (uint32_t)(i >> 1) & 1u);   // (V's rows that nobody sees are zero by then, too)
+        t5_fence_after();
+        const uint64_t vd = v0 + (uint64_t)(vs * (GB / 16));
+        const uint32_t P = S0 + (uint32_t)(TILE * (i & 1));
 #pragma unroll
         for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(O, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
         t5_commit(pv_done(x));
         t5_commit(empty(true, vs));
+        if (++vs == NV) { vs = 0; vp ^= 1u; }
+        // what comes next is waited for while this product runs; the next scores go into the columns of the probabilities that it uses
+        seen = false;
+        if (i + 2 < n) {
+          const bool vk = mbar_wait(full(true, vs), vp, 1), kk = mbar_wait(full(false, ks), kp, 1);
+          if (!vk) wait(full(true, vs), vp);
+          if (!kk) wait(full(false, ks), kp);
+          t5_fence_after();
+          seen = score(i + 2, p_full(x, i + 1), (uint32_t)((i + 1) >> 1) & 1u);
+        } else if (i + 1 < n) wait(full(true, vs), vp);
       }
-      __syncwarp();
-      if (++vs == NV) { vs = 0; vp ^= 1u; }
-      // what comes next is waited for while this product runs
-      if (i + 1 < n) wait(full(true, vs), vp);
-      if (i + 2 < n) { wait(full(false, ks), kp); score(i + 2); }   // into the columns of the probabilities that have just been used
     }
   }
   // after a wait ran out nothing is requested any more, but copies may be on their way
