@@ -13,8 +13,9 @@ static unsigned int *g_kv_err = nullptr;   // what the kernels met (KV_ERR_*)
 static decltype(&cuTensorMapEncodeTiled) g_kv_map = nullptr;
 
 // ---- rows in ------------------------------------------------------------------------------------
-// A warp a head of a row, eight of them a block, whose threads make the row's sines first.  Angles in 64 bits: at position
-// 200,000 a 32-bit product is 0.008 off; what is left of whole turns, taken off in 64 bits too, fits a float.  Bound by bytes.
+// A warp a row, or a head of one where there are few: it finds the row's place, makes its sines, and takes the heads, the next ones on their way.  A lane
+// has head_dim / 32 dimensions of a head and reads their partners of the rotation too (the line is there), so that nothing but the sum of squares
+// crosses lanes.  Angles in turns and 64 bits: at position 200,000 a 32-bit product is 0.008 off; what is left of whole turns fits a float.
 struct KvAppend {
   const void *q, *k, *v;
   long long qs, ks, vs;
@@ -28,61 +29,140 @@ struct KvAppend {
   float eps;
   int wide;                    // q, k, v and q_out: a lane's elements lie on a multiple of their size
 };
-template <typename T, typename X, int HD>
-__global__ void __launch_bounds__(256) k_kv_append(const KvDev c, const KvRows rw, const KvAppend a) {
-  constexpr int E = HD / 32;
-  __shared__ float2 turn[HD / 2];
+template <typename X, int E> struct KaIn { uint32_t w[E * sizeof(X) / 4]; };
+template <typename X, int E> __device__ __forceinline__ KaIn<X, E> ka_load(const X *p, bool wide) {
+  constexpr int W = E * sizeof(X) / 4;
+  KaIn<X, E> r;
+  if (wide) {
+    if constexpr (W == 1) r.w[0] = __ldcs((const uint32_t *)p);
+    else if constexpr (W == 2) { const uint2 t = __ldcs((const uint2 *)p); r.w[0] = t.x; r.w[1] = t.y; }
+    else
+#pragma unroll
+      for (int i = 0; i < W; i += 4) { const uint4 t = __ldcs((const uint4 *)p + i / 4); r.w[i] = t.x; r.w[i + 1] = t.y; r.w[i + 2] = t.z; r.w[i + 3] = t.w; }
+  } else if constexpr (sizeof(X) == 4) {
+#pragma unroll
+    for (int i = 0; i < W; i++) r.w[i] = __ldcs((const uint32_t *)p + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i++) r.w[i] = (uint32_t)__ldcs((const uint16_t *)p + 2 * i) | ((uint32_t)__ldcs((const uint16_t *)p + 2 * i + 1) << 16);
+  }
+  return r;
+}
+template <typename X, int E> __device__ __forceinline__ void ka_values(const KaIn<X, E> &r, float (&x)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; i += 2) {
+    if constexpr (sizeof(X) == 4) { x[i] = __uint_as_float(r.w[i]); x[i + 1] = __uint_as_float(r.w[i + 1]); }
+    else { const float2 f = KvEl<X>::to2(r.w[i / 2]); x[i] = f.x; x[i + 1] = f.y; }
+  }
+}
+template <typename T, typename X, int HD, bool ROW>
+__global__ void __launch_bounds__(256, ROW ? 3 : 1) k_kv_append(const KvDev c, const KvRows rw, const KvAppend a) {
+  constexpr int E = HD / 32, FLY = !ROW ? 1 : E * sizeof(X) > 16 ? 1 : 2;
+  __shared__ float2 turn[8][HD / 2];
   __shared__ float ys[8][HD];
   pdl_trigger();
   pdl_wait();
-  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope >> 1;
-  const int b = kv_find(rw, c.seqs, r, lane);
   if (!blockIdx.x && !blockIdx.y) kv_check_rows(c, rw);
-  if (b < 0) return;           // behind the last row, or row_start is not what it should be
-  const int i = r - __ldcg(rw.start + b), slot = kv_len(c, b) - (__ldcg(rw.start + b + 1) - __ldcg(rw.start + b)) + i;
-  const int pos = a.pos ? __ldcg(a.pos + b) + i : slot;
-  for (int p = threadIdx.x; p < half; p += blockDim.x) {
-    const double th = (double)pos * __ldg(a.invfreq + p), t = th - 6.283185307179586476925 * rint(th * 0.15915494309189533577);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope >> 1, r = ROW ? blockIdx.x * 8 + warp : blockIdx.x;
+  const int b = r < rw.rows ? kv_find(rw, c.seqs, r, lane) : -1;
+  if (b < 0) return;                           // behind the last row, or row_start is not what it should be
+  const int slot = kv_len(c, b) - __ldcg(rw.start + b + 1) + r, pos = a.pos ? __ldcg(a.pos + b) + r - __ldcg(rw.start + b) : slot;
+  const int id = slot >= 0 ? kv_page(c, b, slot >> c.page_sh) : -1;
+#pragma unroll 1
+  for (int p = lane; p < half; p += 32) {
+    const double n = (double)pos * __ldg(a.invfreq + p) * 0.15915494309189533577;   // turns
     float s, co;
-    sincosf((float)t, &s, &co);
-    turn[p] = make_float2(co, s);
+    sincospif((float)(2.0 * (n - rint(n))), &s, &co);
+    turn[warp][p] = make_float2(co, s);
   }
-  __syncthreads();
-  const int u = blockIdx.y * 8 + warp;         // query heads, then kv heads of keys, then of values
-  if (u >= a.H + 2 * c.KV) return;
-  const bool isq = u < a.H, isv = u >= a.H + c.KV;
-  const int g = isq ? u : isv ? u - a.H - c.KV : u - a.H;
-  if (isq && !a.q) return;
-  const X *src = isq ? (const X *)a.q + r * a.qs + (long long)g * a.qhs : isv ? (const X *)a.v + r * a.vs + (long long)g * HD : (const X *)a.k + r * a.ks + (long long)g * HD;
-  float x[E];
-  kv_row_in<X, E>(src + lane * E, a.wide, x);
-  if (!isv) {
-    const float *w = isq ? a.qn : a.kn;
-    if (w) {
-      float ss = 0.0f;
+  __syncwarp();
+  const bool lanes = half % E == 0;            // a lane's partners lie side by side
+  const int d0 = lane * E, other = d0 < half ? d0 + half : d0 - half;
+  const size_t at = id < 0 ? 0 : kv_at(c, id, 0, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD + d0, head_step = (size_t)HD << c.page_sh;
+  auto heads = [&](const X *src, long long step, int n, const float *norm, uint16_t *dst, size_t dstep, bool wide, bool turns) {   // of one kind
+    const bool roll = turns && half;
+    float A[E], B[E];                          // a dimension becomes x A + partner B, divided by the root of the mean square
 #pragma unroll
-      for (int j = 0; j < E; j++) ss += x[j] * x[j];
-      const float sc = 1.0f / sqrtf(kv_warp_sum(ss) / (float)HD + a.eps);
-#pragma unroll
-      for (int j = 0; j < E; j++) x[j] = x[j] * sc * __ldg(w + lane * E + j);
+    for (int j = 0; j < E; j++) {
+      const int d = d0 + j;
+      const bool low = d < half, in = roll && d < a.rope;
+      const float2 t = in ? turn[warp][low ? d : d - half] : make_float2(1.0f, 0.0f);
+      A[j] = (norm ? __ldg(norm + d) : 1.0f) * t.x;
+      B[j] = (norm ? __ldg(norm + (!in ? d : low ? d + half : d - half)) : 1.0f) * (low ? -t.y : t.y);
     }
-    if (half) {
+    src += d0;
+    KaIn<X, E> nin[FLY], npr[FLY];             // the next heads, on their way while these are worked on
+    auto ask = [&](int h0) {
 #pragma unroll
-      for (int j = 0; j < E; j++) ys[warp][lane * E + j] = x[j];
-      __syncwarp();
+      for (int f = 0; f < FLY; f++) {
+        const X *q = src + min(h0 + f, n - 1) * step;
+        nin[f] = ka_load<X, E>(q, a.wide);
+        if (roll && lanes && d0 < a.rope) npr[f] = ka_load<X, E>(q + (other - d0), a.wide);
+      }
+    };
+    ask(0);
+#pragma unroll 1
+    for (int h0 = 0; h0 < n; h0 += FLY) {
+      KaIn<X, E> in[FLY], pr[FLY];
 #pragma unroll
-      for (int j = 0; j < E; j++) {
-        const int d = lane * E + j;
-        if (d < half) x[j] = x[j] * turn[d].x - ys[warp][d + half] * turn[d].y;
-        else if (d < a.rope) x[j] = ys[warp][d - half] * turn[d - half].y + x[j] * turn[d - half].x;
+      for (int f = 0; f < FLY; f++) { in[f] = nin[f]; pr[f] = roll && lanes && d0 < a.rope ? npr[f] : nin[f]; }
+      if (ROW && h0 + FLY < n) ask(h0 + FLY);
+      float ss[FLY];
+#pragma unroll
+      for (int f = 0; f < FLY; f++) {
+        float x[E];
+        ka_values<X, E>(in[f], x);
+        ss[f] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; j++) ss[f] += x[j] * x[j];
+      }
+      if (norm) {
+#pragma unroll
+        for (int m = 16; m; m >>= 1)
+#pragma unroll
+          for (int f = 0; f < FLY; f++) ss[f] += __shfl_xor_sync(0xffffffffu, ss[f], m);
+      }
+#pragma unroll
+      for (int f = 0; f < FLY; f++) {
+        const float sc = norm ? rsqrtf(ss[f] * (1.0f / HD) + a.eps) : 1.0f;
+        float x[E];
+        ka_values<X, E>(in[f], x);
+        if (roll) {
+          float y[E];
+          if (lanes) ka_values<X, E>(pr[f], y);
+          else {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < E; j++) ys[warp][d0 + j] = x[j];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < E; j++) { const int d = d0 + j; y[j] = ys[warp][d < half ? d + half : d < a.rope ? d - half : d]; }
+          }
+#pragma unroll
+          for (int j = 0; j < E; j++) x[j] = (x[j] * A[j] + y[j] * B[j]) * sc;
+        } else if (turns) {
+#pragma unroll
+          for (int j = 0; j < E; j++) x[j] = x[j] * A[j] * sc;
+        }
+        if (h0 + f < n) kv_row_out<T, E>(dst + (h0 + f) * dstep, wide, x);
       }
     }
+  };
+  // query heads, then keys, then values; ROW: all of them, else the warp's one
+  const int u = blockIdx.y * 8 + warp, kh = u - a.H, vh = kh - c.KV;
+  if (a.q && (ROW || u < a.H)) {
+    const int h = ROW ? 0 : u;
+    heads((const X *)a.q + r * a.qs + (long long)h * a.qhs, a.qhs, ROW ? a.H : 1, a.qn, a.qo + r * a.qos + (long long)h * HD + d0, HD, a.wide, true);
   }
-  if (isq) { kv_row_out<T, E>(a.qo + r * a.qos + (long long)g * HD + lane * E, a.wide, x); return; }
-  if (slot < 0) return;
-  const int id = kv_page(c, b, slot >> c.page_sh);
   if (id < 0) return;
-  kv_row_out<T, E>((isv ? c.v : c.k) + kv_at(c, id, g, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD + lane * E, true, x);
+  if (ROW || (kh >= 0 && kh < c.KV)) {
+    const int h = ROW ? 0 : kh;
+    heads((const X *)a.k + r * a.ks + (long long)h * HD, HD, ROW ? c.KV : 1, a.kn, c.k + at + h * head_step, head_step, true, true);
+  }
+  if (ROW || (vh >= 0 && vh < c.KV)) {
+    const int h = ROW ? 0 : vh;
+    heads((const X *)a.v + r * a.vs + (long long)h * HD, HD, ROW ? c.KV : 1, nullptr, c.v + at + h * head_step, head_step, true, false);
+  }
 }
 
 // ---- eviction -------------------------------------------------------------------------------------
@@ -247,12 +327,15 @@ static int heads_check(const llb_kv *kv, int heads, const char *what) {
   return 0;
 }
 
-template <typename T, typename X> static int append_go(const KvDev &c, const KvRows &rw, const KvAppend &a, int hd) {
-  const dim3 grid(rw.rows, (a.H + 2 * c.KV + 7) / 8);
-  if (hd == 64) CU_OK(llb_launch(k_kv_append<T, X, 64>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
-  else if (hd == 128) CU_OK(llb_launch(k_kv_append<T, X, 128>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
-  else CU_OK(llb_launch(k_kv_append<T, X, 256>, grid, dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+// A warp a head where that leaves SMs free (a step of a few tokens is as long as a warp's chain of latencies: place, sines, a head), else a warp a row.
+template <typename T, typename X, int HD> static int append_hd(const KvDev &c, const KvRows &rw, const KvAppend &a) {
+  const int groups = (a.H + 2 * c.KV + 7) / 8;
+  if ((long long)rw.rows * groups <= 8LL * g_llb.sms) CU_OK(llb_launch(k_kv_append<T, X, HD, false>, dim3(rw.rows, groups), dim3(256), (size_t)0, g_llb.stream, c, rw, a));
+  else CU_OK(llb_launch(k_kv_append<T, X, HD, true>, dim3((unsigned)(((long long)rw.rows + 7) / 8)), dim3(256), (size_t)0, g_llb.stream, c, rw, a));
   return 0;
+}
+template <typename T, typename X> static int append_go(const KvDev &c, const KvRows &rw, const KvAppend &a, int hd) {
+  return hd == 64 ? append_hd<T, X, 64>(c, rw, a) : hd == 128 ? append_hd<T, X, 128>(c, rw, a) : append_hd<T, X, 256>(c, rw, a);
 }
 // pages as [page][kv head][64 dims][slot][dim], in boxes of `slots` slots and `blocks` times 64 dims of a kv head of a page
 static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int slots, int blocks) {
@@ -424,7 +507,7 @@ int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a) {
   k.H = a->heads; k.rope = a->rope_dim; k.eps = a->eps;
   // a lane's head_dim / 32 elements in wide words, where all of q, k, v and q_out have them there
   const int E = hd / 32;
-  const unsigned in = es == 4 ? 8 : 2 * E;
+  const unsigned in = std::min(16u, E * es);
   k.wide = !off(a->q, in) && !off(a->k, in) && !off(a->v, in) && a->q_stride % E == 0 && a->k_stride % E == 0 && a->v_stride % E == 0 && a->q_head_stride % E == 0 &&
            !off(a->q_out, 2 * E) && a->q_out_stride % E == 0;
   if (kv->el == LLB_EL_F16) {
