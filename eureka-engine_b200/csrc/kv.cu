@@ -13,9 +13,10 @@ static unsigned int *g_kv_err = nullptr;   // what the kernels met (KV_ERR_*)
 static decltype(&cuTensorMapEncodeTiled) g_kv_map = nullptr;
 
 // ---- rows in ------------------------------------------------------------------------------------
-// A warp a row, or a head of one where there are few: it finds the row's place, makes its sines, and takes the heads, the next ones on their way.  A lane
-// has head_dim / 32 dimensions of a head and reads their partners of the rotation too (the line is there), so that nothing but the sum of squares
-// crosses lanes.  Angles in turns and 64 bits: at position 200,000 a 32-bit product is 0.008 off; what is left of whole turns fits a float.
+// A warp a row, or a few heads of one where there are few rows: it finds the row's place, makes its sines, and takes the heads, 512 / head_dim at a
+// time and the next ones on their way.  A lane has eight dimensions in each half of a head and reads their partners of the rotation too (the line is
+// there), so that nothing but the sum of squares crosses lanes.  Angles in turns and 64 bits: at position 200,000 a 32-bit product is 0.008
+// off; what is left of whole turns fits a float.  Bound by bytes and by the instructions a head takes.
 struct KvAppend {
   const void *q, *k, *v;
   long long qs, ks, vs;
@@ -27,18 +28,16 @@ struct KvAppend {
   long long qos;
   int H, rope;
   float eps;
-  int wide;                    // q, k, v and q_out: a lane's elements lie on a multiple of their size
+  int wide;                    // q, k, v and q_out: eight elements lie on a multiple of 16 bytes
 };
-template <typename X, int E> struct KaIn { uint32_t w[E * sizeof(X) / 4]; };
-template <typename X, int E> __device__ __forceinline__ KaIn<X, E> ka_load(const X *p, bool wide) {
-  constexpr int W = E * sizeof(X) / 4;
-  KaIn<X, E> r;
+// eight values of a row of the caller's, as they lie there
+template <typename X> struct KaIn { uint32_t w[2 * sizeof(X)]; };
+template <typename X> __device__ __forceinline__ KaIn<X> ka_load(const X *p, bool wide) {
+  constexpr int W = 2 * sizeof(X);
+  KaIn<X> r;
   if (wide) {
-    if constexpr (W == 1) r.w[0] = __ldcs((const uint32_t *)p);
-    else if constexpr (W == 2) { const uint2 t = __ldcs((const uint2 *)p); r.w[0] = t.x; r.w[1] = t.y; }
-    else
 #pragma unroll
-      for (int i = 0; i < W; i += 4) { const uint4 t = __ldcs((const uint4 *)p + i / 4); r.w[i] = t.x; r.w[i + 1] = t.y; r.w[i + 2] = t.z; r.w[i + 3] = t.w; }
+    for (int i = 0; i < W; i += 4) { const uint4 t = __ldcs((const uint4 *)p + i / 4); r.w[i] = t.x; r.w[i + 1] = t.y; r.w[i + 2] = t.z; r.w[i + 3] = t.w; }
   } else if constexpr (sizeof(X) == 4) {
 #pragma unroll
     for (int i = 0; i < W; i++) r.w[i] = __ldcs((const uint32_t *)p + i);
@@ -48,18 +47,18 @@ template <typename X, int E> __device__ __forceinline__ KaIn<X, E> ka_load(const
   }
   return r;
 }
-template <typename X, int E> __device__ __forceinline__ void ka_values(const KaIn<X, E> &r, float (&x)[E]) {
+// as pairs
+template <typename X> __device__ __forceinline__ void ka_values(const KaIn<X> &r, f32x2 (&x)[4]) {
 #pragma unroll
-  for (int i = 0; i < E; i += 2) {
-    if constexpr (sizeof(X) == 4) { x[i] = __uint_as_float(r.w[i]); x[i + 1] = __uint_as_float(r.w[i + 1]); }
-    else { const float2 f = KvEl<X>::to2(r.w[i / 2]); x[i] = f.x; x[i + 1] = f.y; }
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(X) == 4) x[i] = x2_pack(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else { const float2 f = KvEl<X>::to2(r.w[i]); x[i] = x2_pack(f.x, f.y); }
   }
 }
 template <typename T, typename X, int HD, bool ROW>
-__global__ void __launch_bounds__(256, ROW ? 3 : 1) k_kv_append(const KvDev c, const KvRows rw, const KvAppend a) {
-  constexpr int E = HD / 32, FLY = !ROW ? 1 : E * sizeof(X) > 16 ? 1 : 2;
-  __shared__ float2 turn[8][HD / 2];
-  __shared__ float ys[8][HD];
+__global__ void __launch_bounds__(256, ROW ? 2 : 1) k_kv_append(const KvDev c, const KvRows rw, const KvAppend a) {
+  constexpr int LPH = HD / 16, HPW = 32 / LPH, H2 = HD / 2;   // lanes a head, heads a warp
+  __shared__ float2 turn[8][H2];
   pdl_trigger();
   pdl_wait();
   if (!blockIdx.x && !blockIdx.y) kv_check_rows(c, rw);
@@ -76,93 +75,101 @@ __global__ void __launch_bounds__(256, ROW ? 3 : 1) k_kv_append(const KvDev c, c
     turn[warp][p] = make_float2(co, s);
   }
   __syncwarp();
-  const bool lanes = half % E == 0;            // a lane's partners lie side by side
-  const int d0 = lane * E, other = d0 < half ? d0 + half : d0 - half;
-  const size_t at = id < 0 ? 0 : kv_at(c, id, 0, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD + d0, head_step = (size_t)HD << c.page_sh;
-  auto heads = [&](const X *src, long long step, int n, const float *norm, uint16_t *dst, size_t dstep, bool wide, bool turns) {   // of one kind
-    const bool roll = turns && half;
-    float A[E], B[E];                          // a dimension becomes x A + partner B, divided by the root of the mean square
+  const int sub = lane / LPH, l8 = 8 * (lane % LPH);   // the lane's head of the warp's; its dimensions l8 .. and HD / 2 + l8 ..
+  const bool lanes = half % 8 == 0;                    // eight dimensions' partners lie side by side
+  const size_t at = id < 0 ? 0 : kv_at(c, id, 0, HD) + (size_t)(slot & ((1 << c.page_sh) - 1)) * HD, head_step = (size_t)HD << c.page_sh;
+  // heads ha .. n - 1 of one kind (the warp's first HPW of them where the warp has no row of its own)
+  auto heads = [&](const X *src, long long step, int ha, int n, const float *norm, uint16_t *dst, size_t dstep, bool wide, bool turns) {
+    f32x2 A[2][4], B[2][4];                    // a dimension becomes x A + partner B, divided by the root of the mean square
+    bool roll[2];                              // the warp: this half of the heads has turned dimensions
 #pragma unroll
-    for (int j = 0; j < E; j++) {
-      const int d = d0 + j;
-      const bool low = d < half, in = roll && d < a.rope;
-      const float2 t = in ? turn[warp][low ? d : d - half] : make_float2(1.0f, 0.0f);
-      A[j] = (norm ? __ldg(norm + d) : 1.0f) * t.x;
-      B[j] = (norm ? __ldg(norm + (!in ? d : low ? d + half : d - half)) : 1.0f) * (low ? -t.y : t.y);
+    for (int h = 0; h < 2; h++) {
+      roll[h] = turns && a.rope > h * H2;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        float p[2], q[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int d = h * H2 + l8 + j + k;
+          const bool low = d < half, in = roll[h] && d < a.rope;
+          const float2 t = in ? turn[warp][low ? d : d - half] : make_float2(1.0f, 0.0f);
+          p[k] = (norm ? __ldg(norm + d) : 1.0f) * t.x;
+          q[k] = (norm && in ? __ldg(norm + (low ? d + half : d - half)) : 1.0f) * (low ? -t.y : t.y);
+        }
+        A[h][j / 2] = x2_pack(p[0], p[1]); B[h][j / 2] = x2_pack(q[0], q[1]);
+      }
     }
-    src += d0;
-    KaIn<X, E> nin[FLY], npr[FLY];             // the next heads, on their way while these are worked on
+    KaIn<X> nin[2], npr[2];                    // the next heads, on their way while these are worked on
     auto ask = [&](int h0) {
+      const X *q = src + min(h0 + sub, n - 1) * step + l8;
 #pragma unroll
-      for (int f = 0; f < FLY; f++) {
-        const X *q = src + min(h0 + f, n - 1) * step;
-        nin[f] = ka_load<X, E>(q, a.wide);
-        if (roll && lanes && d0 < a.rope) npr[f] = ka_load<X, E>(q + (other - d0), a.wide);
+      for (int h = 0; h < 2; h++) {
+        nin[h] = ka_load<X>(q + h * H2, a.wide);
+        if (!roll[h]) continue;
+        const int d = h * H2 + l8;
+        if (lanes) npr[h] = ka_load<X>(d < a.rope ? q + h * H2 + (d < half ? half : -half) : q + h * H2, a.wide);
+        else if constexpr (sizeof(X) == 4) {
+#pragma unroll
+          for (int j = 0; j < 8; j++) npr[h].w[j] = __ldcs((const uint32_t *)(q + h * H2) + j + (d + j < half ? half : d + j < a.rope ? -half : 0));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            uint32_t v[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) v[k] = __ldcs((const uint16_t *)(q + h * H2) + j + k + (d + j + k < half ? half : d + j + k < a.rope ? -half : 0));
+            npr[h].w[j / 2] = v[0] | v[1] << 16;
+          }
+        }
       }
     };
-    ask(0);
+    ask(ha);
 #pragma unroll 1
-    for (int h0 = 0; h0 < n; h0 += FLY) {
-      KaIn<X, E> in[FLY], pr[FLY];
+    for (int h0 = ha; h0 < n; h0 += HPW) {
+      f32x2 x[2][4], y[2][4];
 #pragma unroll
-      for (int f = 0; f < FLY; f++) { in[f] = nin[f]; pr[f] = roll && lanes && d0 < a.rope ? npr[f] : nin[f]; }
-      if (ROW && h0 + FLY < n) ask(h0 + FLY);
-      float ss[FLY];
-#pragma unroll
-      for (int f = 0; f < FLY; f++) {
-        float x[E];
-        ka_values<X, E>(in[f], x);
-        ss[f] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < E; j++) ss[f] += x[j] * x[j];
+      for (int h = 0; h < 2; h++) {
+        ka_values<X>(nin[h], x[h]);
+        if (roll[h]) ka_values<X>(npr[h], y[h]);
       }
+      if (ROW && h0 + HPW < n) ask(h0 + HPW);
+      float sc = 1.0f;
       if (norm) {
+        f32x2 q = x2_mul(x[0][0], x[0][0]), q2 = x2_mul(x[1][0], x[1][0]);
 #pragma unroll
-        for (int m = 16; m; m >>= 1)
+        for (int j = 1; j < 4; j++) { q = x2_fma(x[0][j], x[0][j], q); q2 = x2_fma(x[1][j], x[1][j], q2); }
+        float q0, q1;
+        x2_unpack(x2_add(q, q2), q0, q1);
+        float ss = q0 + q1;
 #pragma unroll
-          for (int f = 0; f < FLY; f++) ss[f] += __shfl_xor_sync(0xffffffffu, ss[f], m);
+        for (int m = LPH / 2; m; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        sc = rsqrtf(ss * (1.0f / HD) + a.eps);
       }
+      const f32x2 sc2 = x2_pack(sc, sc);
+      uint16_t *to = dst + (h0 + sub) * dstep + l8;
 #pragma unroll
-      for (int f = 0; f < FLY; f++) {
-        const float sc = norm ? rsqrtf(ss[f] * (1.0f / HD) + a.eps) : 1.0f;
-        float x[E];
-        ka_values<X, E>(in[f], x);
-        if (roll) {
-          float y[E];
-          if (lanes) ka_values<X, E>(pr[f], y);
-          else {
-            __syncwarp();
+      for (int h = 0; h < 2; h++) {
+        float o[8];
 #pragma unroll
-            for (int j = 0; j < E; j++) ys[warp][d0 + j] = x[j];
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < E; j++) { const int d = d0 + j; y[j] = ys[warp][d < half ? d + half : d < a.rope ? d - half : d]; }
+        for (int j = 0; j < 4; j++) {
+          f32x2 v = x[h][j];
+          if (turns) {
+            if (roll[h]) v = x2_fma(v, A[h][j], x2_mul(y[h][j], B[h][j]));
+            else v = x2_mul(v, A[h][j]);
+            v = x2_mul(v, sc2);
           }
-#pragma unroll
-          for (int j = 0; j < E; j++) x[j] = (x[j] * A[j] + y[j] * B[j]) * sc;
-        } else if (turns) {
-#pragma unroll
-          for (int j = 0; j < E; j++) x[j] = x[j] * A[j] * sc;
+          x2_unpack(v, o[2 * j], o[2 * j + 1]);
         }
-        if (h0 + f < n) kv_row_out<T, E>(dst + (h0 + f) * dstep, wide, x);
+        if (h0 + sub < n) kv_row_out<T, 8>(to + h * H2, wide, o);
       }
+      if (!ROW) break;
     }
   };
-  // query heads, then keys, then values; ROW: all of them, else the warp's one
-  const int u = blockIdx.y * 8 + warp, kh = u - a.H, vh = kh - c.KV;
-  if (a.q && (ROW || u < a.H)) {
-    const int h = ROW ? 0 : u;
-    heads((const X *)a.q + r * a.qs + (long long)h * a.qhs, a.qhs, ROW ? a.H : 1, a.qn, a.qo + r * a.qos + (long long)h * HD + d0, HD, a.wide, true);
-  }
+  // query heads, then keys, then values; where the warp has no row of its own, its HPW of one of them
+  const int u = blockIdx.y * 8 + warp, qu = (a.H + HPW - 1) / HPW, ku = (c.KV + HPW - 1) / HPW, kh = u - qu, vh = kh - ku;
+  if (a.q && (ROW || u < qu)) heads((const X *)a.q + r * a.qs, a.qhs, ROW ? 0 : u * HPW, a.H, a.qn, a.qo + r * a.qos, HD, a.wide, true);
   if (id < 0) return;
-  if (ROW || (kh >= 0 && kh < c.KV)) {
-    const int h = ROW ? 0 : kh;
-    heads((const X *)a.k + r * a.ks + (long long)h * HD, HD, ROW ? c.KV : 1, a.kn, c.k + at + h * head_step, head_step, true, true);
-  }
-  if (ROW || (vh >= 0 && vh < c.KV)) {
-    const int h = ROW ? 0 : vh;
-    heads((const X *)a.v + r * a.vs + (long long)h * HD, HD, ROW ? c.KV : 1, nullptr, c.v + at + h * head_step, head_step, true, false);
-  }
+  if (ROW || (kh >= 0 && kh < ku)) heads((const X *)a.k + r * a.ks, HD, ROW ? 0 : kh * HPW, c.KV, a.kn, c.k + at, head_step, true, true);
+  if (ROW || (vh >= 0 && vh < ku)) heads((const X *)a.v + r * a.vs, HD, ROW ? 0 : vh * HPW, c.KV, nullptr, c.v + at, head_step, true, false);
 }
 
 // ---- eviction -------------------------------------------------------------------------------------
@@ -327,9 +334,10 @@ static int heads_check(const llb_kv *kv, int heads, const char *what) {
   return 0;
 }
 
-// A warp a head where that leaves SMs free (a step of a few tokens is as long as a warp's chain of latencies: place, sines, a head), else a warp a row.
+// A warp 512 / head_dim heads where that leaves SMs free (a step of a few tokens is as long as a warp's chain of latencies: place, sines, a head), else a warp a row.
 template <typename T, typename X, int HD> static int append_hd(const KvDev &c, const KvRows &rw, const KvAppend &a) {
-  const int groups = (a.H + 2 * c.KV + 7) / 8;
+  constexpr int HPW = 512 / HD;
+  const int groups = ((a.H + HPW - 1) / HPW + 2 * ((c.KV + HPW - 1) / HPW) + 7) / 8;
   if ((long long)rw.rows * groups <= 8LL * g_llb.sms) CU_OK(llb_launch(k_kv_append<T, X, HD, false>, dim3(rw.rows, groups), dim3(256), (size_t)0, g_llb.stream, c, rw, a));
   else CU_OK(llb_launch(k_kv_append<T, X, HD, true>, dim3((unsigned)(((long long)rw.rows + 7) / 8)), dim3(256), (size_t)0, g_llb.stream, c, rw, a));
   return 0;
@@ -505,11 +513,9 @@ int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a) {
   k.invfreq = (const double *)(uintptr_t)a->invfreq; k.pos = (const int *)(uintptr_t)a->pos;
   k.qo = (uint16_t *)(uintptr_t)a->q_out; k.qos = a->q_out_stride;
   k.H = a->heads; k.rope = a->rope_dim; k.eps = a->eps;
-  // a lane's head_dim / 32 elements in wide words, where all of q, k, v and q_out have them there
-  const int E = hd / 32;
-  const unsigned in = std::min(16u, E * es);
-  k.wide = !off(a->q, in) && !off(a->k, in) && !off(a->v, in) && a->q_stride % E == 0 && a->k_stride % E == 0 && a->v_stride % E == 0 && a->q_head_stride % E == 0 &&
-           !off(a->q_out, 2 * E) && a->q_out_stride % E == 0;
+  // eight elements as 16-byte words, where all of q, k, v and q_out have them there
+  k.wide = !off(a->q, 16) && !off(a->k, 16) && !off(a->v, 16) && !off(a->q_out, 16) && a->q_stride % 8 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0 && a->q_head_stride % 8 == 0 &&
+           a->q_out_stride % 8 == 0;
   if (kv->el == LLB_EL_F16) {
     if (a->el_in == LLB_EL_F32) return append_go<__half, float>(c, rw, k, hd);
     if (a->el_in == LLB_EL_F16) return append_go<__half, __half>(c, rw, k, hd);
