@@ -360,10 +360,10 @@ static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int 
 #define KF_LEAST 8             // fewest chunks of a block's stretch: two a warp
 static int most_rows(const llb_kv_attn *a) { return std::min(a->max_rows, std::max(a->rows, 1)); }
 static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * most_rows(a) <= KV_FEW; }
-static int few_grid(const llb_kv *kv) { return (g_llb.sms ? g_llb.sms : 148) * (kv->head_dim == 256 ? 1 : 2); }
+static int few_grid(void) { return g_llb.sms ? g_llb.sms : 148; }
 // its parts, one behind the other; the size where `base` is 0
 static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, KvPlan *p) {
-  const size_t blocks = few_grid(kv), queries = (size_t)kv->seqs * a->heads * most_rows(a);
+  const size_t blocks = few_grid(), queries = (size_t)kv->seqs * a->heads * most_rows(a);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
   p->least = KF_LEAST;
@@ -382,7 +382,7 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   p.err = gemm_err_word();
   CUtensorMap km, vm;
   if (pool_map(&km, kv, kv->k, KF_SLOTS, HD / 64) || pool_map(&vm, kv, kv->v, KF_SLOTS, HD / 64)) return -1;
-  const dim3 grid(few_grid(kv)), block(32 * KF_WARPS);
+  const dim3 grid(few_grid()), block(32 * (kf_warps(HD) + 1));
   const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + 511) / 512;   // (attn_check: they fit)
   if (a.w_out) {
     CU_OK(llb_launch(k_kv_few<T, HD, true>, grid, block, (size_t)kf_smem(HD), g_llb.stream, c, rw, a, p, km, vm));

@@ -2,36 +2,38 @@
 //
 // A unit is (sequence, kv head, 16 queries); its queries are the rows' heads side by side, query i G + h is row i, head h of the kv head's
 // G.  What a unit sees is cut into chunks of 16 slots, a page's part each, and the chunks of all units, one after the other, into as many
-// equal stretches as there are blocks, so that sequences of any lengths keep every SM busy to the end; a block's stretch may begin and end inside a unit.  The four warps of a
-// block take its chunks in turn, each with a ring of stages of its own that TMA fills (rows of 128 swizzled bytes) and that runs ahead over
-// the ends of units: no barrier between warps but where a unit ends and their sums are joined.
+// equal stretches as there are blocks, so that sequences of any lengths keep every SM busy to the end; a block's stretch may begin and end inside a unit.
+// A warp of the block brings the chunks by TMA (rows of 128 swizzled bytes) into a ring, on over the ends of units; the others take them in turn.
 //   S[query][slot] = Q K^T      m16n8k16, 16 queries x 16 slots
 //   O[query][dim] += P V        P from the registers of S, rounded to the cache's type (the second product takes 16-bit operands)
-// with the maximum and the sum of every query kept in f32.  A unit that one block has wholly is finished there; the others' sums go to the workspace,
-// and k_kv_join, the second launch, puts them together in the order of the blocks.
+// with the maximum and the sum of every query kept in f32.  Where a unit ends the warps' sums are put together, 32 dims at a time.  A unit that one
+// block has wholly is finished there; the others' sums go to the workspace, and k_kv_join, the second launch, puts them together in the order of the blocks.
+//
+// A chunk is a chain of some 2000 to 4000 cycles for its warp (two products with the softmax between), which is why so many warps work on chunks of their own.
 #pragma once
 #include <cuda.h>
 
 #include "kv.cuh"
 #include "tc5.cuh"
 
-#define KF_WARPS 4
 #define KF_SLOTS 16
 #define KF_SH 4
-__host__ __device__ constexpr int kf_stages(int HD) { return HD == 64 ? 5 : HD == 128 ? 3 : 3; }
-__host__ __device__ constexpr int kf_stage_bytes(int HD) { return 2 * KF_SLOTS * HD * 2; }       // K, then V
-__host__ __device__ constexpr int kf_ring(int HD) { return KF_WARPS * kf_stages(HD) * kf_stage_bytes(HD); }
-__host__ __device__ constexpr int kf_row(int HD) { return HD + 8; }                              // floats of a row of a warp's sums
-__host__ __device__ constexpr int kf_sums(int HD) { return HD == 64 ? 2 : 1; }                  // sums of so many warps have room
-__host__ __device__ constexpr int kf_smem(int HD) { return 1024 + kf_ring(HD) + kf_sums(HD) * 16 * kf_row(HD) * 4 + 16 * HD * 2; }
-static_assert(kf_smem(256) <= 232448 && 2 * (kf_smem(128) + 1024) <= 233472 && 2 * (kf_smem(64) + 1024) <= 233472, "one block an SM, or two");
-struct KfHead {                // before the rings
-  uint64_t full[KF_WARPS][5];
-  long long sum[KF_WARPS], rem;
-  int b, bad[KF_WARPS][5];
-  float m[2][16], l[2][16];
+__host__ __device__ constexpr int kf_warps(int HD) { return HD == 256 ? 6 : 11; }   // that compute
+__host__ __device__ constexpr int kf_ring(int HD) { return HD == 256 ? 12 : 22; }    // chunks that have room
+__host__ __device__ constexpr int kf_bytes(int HD) { return 2 * KF_SLOTS * HD * 2; }                  // of a chunk: K, then V
+#define KF_ROW 40              // floats from a row of the warps' sums to the next: 32 dims, and eight banks on
+struct KfHead {                // before the ring
+  uint64_t full[32], empty[32];
+  long long sum[16], rem;
+  int b, bad[32], odd[16];
+  float m[11][16], l[11][16], M[16], L[16];
 };
-static_assert(sizeof(KfHead) <= 1024, "the rings begin 1024 bytes on");
+#define KF_HEAD 3072
+// A place of the ring is one warp's: a warp that came to it after another would take the phase before the other's for its own where that one's copy is late.
+static_assert(kf_ring(256) % kf_warps(256) == 0 && kf_ring(128) % kf_warps(128) == 0 && kf_ring(64) % kf_warps(64) == 0 && kf_ring(64) <= 32, "a place of the ring is one warp's");
+static_assert(sizeof(KfHead) <= KF_HEAD, "the ring begins after it");
+__host__ __device__ constexpr int kf_smem(int HD) { return KF_HEAD + kf_ring(HD) * kf_bytes(HD) + kf_warps(HD) * 16 * KF_ROW * 4 + 16 * HD * 2; }
+static_assert(kf_smem(256) <= 232448 && kf_smem(128) <= 232448 && kf_smem(64) <= 232448, "shared memory");
 
 struct KvPlan {
   int least;                   // chunks of a block's stretch, at least
@@ -95,23 +97,22 @@ struct KfWalk {
 };
 
 template <typename T, int HD, bool WT>
-__global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
-                                                                             const __grid_constant__ CUtensorMap vm) {
-  constexpr int NS = kf_stages(HD), SB = kf_stage_bytes(HD), KB = SB / 2, ROW = kf_row(HD), E = HD / 32, NT = HD / 8, NB = kf_sums(HD);
-  static_assert(NS <= 5, "KfHead");
+__global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
+                                                                      const __grid_constant__ CUtensorMap vm) {
+  constexpr int CW = kf_warps(HD), NT = 32 * (CW + 1), NS = kf_ring(HD), SB = kf_bytes(HD), KB = SB / 2, TD = HD / 8;   // TD: tiles of eight dims
   extern __shared__ __align__(1024) uint8_t smem[];
   KfHead &hd = *(KfHead *)smem;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, j2 = 2 * (lane & 3), lr = lane & 7, mi = lane >> 3;
-  const uint32_t bar_s = smem_u32(smem), ring_s = bar_s + 1024 + warp * NS * SB;
-  float *sums = (float *)(smem + 1024 + kf_ring(HD));                    // [NB][16][ROW]
-  const uint32_t q_s = bar_s + 1024 + kf_ring(HD) + NB * 16 * ROW * 4;   // the unit's queries: a core matrix's rows of 16 bytes, [dims / 8][16]
-  uint8_t *q_m = smem + 1024 + kf_ring(HD) + NB * 16 * ROW * 4;
-  if (tid < KF_WARPS * 5) mbar_init(bar_s + 8 * tid, 1);
+  const uint32_t bar_s = smem_u32(smem), ring_s = bar_s + KF_HEAD, q_s = ring_s + NS * SB + CW * 16 * KF_ROW * 4;   // queries: rows of 16 bytes, [dims / 8][16]
+  float *sums = (float *)(smem + KF_HEAD + NS * SB);                     // [warp][16][KF_ROW]
+  uint8_t *q_m = smem + (q_s - bar_s);
+  if (tid < 32) { mbar_init(bar_s + 8 * tid, 1); mbar_init(bar_s + 256 + 8 * tid, 1); }
   if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (tid < 16) hd.odd[tid] = 0;
   pdl_trigger();
   pdl_wait();
   // ---- the block's stretch: chunks of every sequence, summed over the threads' runs of sequences ----
-  const int run = (c.seqs + 32 * KF_WARPS - 1) / (32 * KF_WARPS), ba = min(c.seqs, tid * run), bz = min(c.seqs, ba + run);
+  const int run = (c.seqs + NT - 1) / NT, ba = min(c.seqs, tid * run), bz = min(c.seqs, ba + run);
   auto work = [&](int b) {
     const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
     return (long long)s.chunks * c.KV * ((a.G * s.nc + 15) >> 4);
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
   __syncthreads();
   long long all = 0;
 #pragma unroll
-  for (int w = 0; w < KF_WARPS; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
+  for (int w = 0; w <= CW; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
   const long long per = max((long long)p.least, (all + gridDim.x - 1) / gridDim.x), start = per * blockIdx.x;
   if (blockIdx.x == 0) {
     long long at = to - mine;
@@ -152,57 +153,70 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
     use.left = min(per, all - start);
     use.take();
   }
-  // ---- the warp's requests: a chunk behind the other, over the ends of units ----
-  KfWalk get = use;
-  int gch = use.c0 + warp, gid_page = -1, issued = 0;
-  bool more = true, dead = false;
-  auto find = [&]() {          // the page of the next chunk, or that there is none
-    while (gch >= get.c1) {
-      if (!get.next(c, rw, a)) { more = false; return; }
-      gch = get.c0 + warp;
-    }
-    const int slot = kv_chunk_slot(get.s, gch, KF_SH);
-    gid_page = get.s.e0 + get.s.nc > 0 ? __ldcg(c.table + (size_t)get.b * c.tstride + (slot >> c.page_sh)) : -1;
+  bool dead = false;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!dead && !mbar_wait(bar, parity)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
   };
-  auto issue = [&]() {
-    if (!more) return;
-    const int st = issued % NS, slot = kv_chunk_slot(get.s, gch, KF_SH);
-    const uint32_t full = bar_s + 8 * (warp * 5 + st);
-    const bool in = (unsigned)gid_page < (unsigned)c.n_pages;
-    if (lane == 0) {
-      hd.bad[warp][st] = !in;
-      if (in) {
-        kv_expect(full, SB);
-        kv_tma(ring_s + st * SB, &km, 0, slot & ((1 << c.page_sh) - 1), 0, get.g, gid_page, full);
-        kv_tma(ring_s + st * SB + KB, &vm, 0, slot & ((1 << c.page_sh) - 1), 0, get.g, gid_page, full);
-      } else {
-        if (get.s.e0 + get.s.nc > 0) atomicOr(c.err, KV_ERR_PAGE);
-        mbar_arrive(full);
-      }
-    }
-    issued++;
-    gch += KF_WARPS;
-    find();
-  };
-  find();
+  if (warp == CW) {
+    // ---- the chunks, one behind the other, over the ends of units; the pages of 32 chunks are asked for at once, and those of the next 32 while these are requested ----
+    int st = 0;
+    uint32_t round = 0;
+    const int pm = (1 << c.page_sh) - 1;
+    do {
+      const bool seen = use.s.e0 + use.s.nc > 0;           // (or the unit's rows see nothing)
+      auto pages = [&](int ch) {
+        int id = -1;
+        if (seen && ch + lane < use.c1)
+          asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(id) : "l"(c.table + (size_t)use.b * c.tstride + (kv_chunk_slot(use.s, ch + lane, KF_SH) >> c.page_sh)));
+        return id;
+      };
+      int next = pages(use.c0);
 #pragma unroll 1
-  for (int i = 0; i < NS; i++) issue();
-  int done = 0;
+      for (int c0 = use.c0; c0 < use.c1; c0 += 32) {
+        asm volatile("" : "+r"(next));
+        const int ids = next, n = min(32, use.c1 - c0);
+        next = pages(c0 + 32);
+#pragma unroll 1
+        for (int k = 0; k < n; k++) {
+          const int id = __shfl_sync(0xffffffffu, ids, k), slot = kv_chunk_slot(use.s, c0 + k, KF_SH) & pm;
+          if (round) wait(bar_s + 256 + 8 * st, (round - 1) & 1u);
+          if (lane == 0) {
+            const uint32_t full = bar_s + 8 * st;
+            const bool in = (unsigned)id < (unsigned)c.n_pages && !dead;
+            hd.bad[st] = !in;
+            if (in) {
+              kv_expect(full, SB);
+              kv_tma(ring_s + st * SB, &km, 0, slot, 0, use.g, id, full);
+              kv_tma(ring_s + st * SB + KB, &vm, 0, slot, 0, use.g, id, full);
+            } else {
+              if (seen && !dead) atomicOr(c.err, KV_ERR_PAGE);
+              mbar_arrive(full);
+            }
+          }
+          __syncwarp();
+          if (++st == NS) { st = 0; round++; }
+        }
+      }
+    } while (use.next(c, rw, a));
+    if (dead) for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies may be on their way
+    return;
+  }
+  auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory"); };   // the warps that compute
+  int n0 = 0;                                              // chunks of the stretch before this unit's
 #pragma unroll 1
   for (;;) {
     const KvSeq &s = use.s;
     const int NQ = a.G * s.nc, q0 = 16 * use.qt, last = s.e0 + s.nc - 1;
-    // the queries: rows of 16 bytes, [dims / 8][query]
-    for (int i = tid; i < 16 * NT; i += 32 * KF_WARPS) {
-      const int qi = q0 + (i & 15), d = i >> 4;
+    for (int i = tid; i < 16 * TD; i += 32 * CW) {
+      const int qi = q0 + (i & 15), d = i >> 4, row = kv_row_of(a, qi);
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (qi < NQ) v = __ldcg((const uint4 *)(a.q + (long long)(s.first + qi / a.G) * a.qs + (long long)(use.g * a.G + qi % a.G) * HD + 8 * d));
+      if (qi < NQ) v = __ldcg((const uint4 *)(a.q + (long long)(s.first + row) * a.qs + (long long)(use.g * a.G + qi - row * a.G) * HD + 8 * d));
       *(uint4 *)(q_m + i * 16) = v;
     }
-    __syncthreads();
-    float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    meet();
+    float o[TD][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+    for (int i = 0; i < TD; i++)
 #pragma unroll
       for (int k = 0; k < 4; k++) o[i][k] = 0.0f;
     // the slots that the thread's two queries see: from lw to e, and below the first tokens' end
@@ -210,27 +224,32 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const int qi = q0 + gid + 8 * k;
-      e[k] = qi < NQ ? s.e0 + qi / a.G : -1;
+      e[k] = qi < NQ ? s.e0 + kv_row_of(a, qi) : -1;
       lw[k] = a.window ? e[k] - a.window + 1 : 0;
     }
-    const int ea = s.e0 + q0 / a.G, ez = s.e0 + min(q0 + 15, NQ - 1) / a.G;      // slots of the unit's first and last row
+    const int ea = s.e0 + kv_row_of(a, q0), ez = s.e0 + kv_row_of(a, min(q0 + 15, NQ - 1));      // slots of the unit's first and last row
+    int skip = (warp - n0) % CW;
+    if (skip < 0) skip += CW;
 #pragma unroll 1
-    for (int ch = use.c0 + warp; ch < use.c1; ch += KF_WARPS, done++) {
-      const int st = done % NS, slot = kv_chunk_slot(s, ch, KF_SH);
+    for (int ch = use.c0 + skip; ch < use.c1; ch += CW) {
+      const int n = n0 + ch - use.c0, st = n % NS, slot = kv_chunk_slot(s, ch, KF_SH);
       const uint32_t k_s = ring_s + st * SB, v_s = k_s + KB;
-      if (!dead && !mbar_wait(bar_s + 8 * (warp * 5 + st), (uint32_t)(done / NS) & 1u)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
-      const bool none = hd.bad[warp][st] || dead;
-      float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      wait(bar_s + 8 * st, (uint32_t)(n / NS) & 1u);
+      const bool none = hd.bad[st] || dead;
+      float x[2][4];
       if (!none) {
         // slots that no row sees: their V is taken out, whatever it holds (0 times NaN is NaN)
         if (slot + 15 > last || (a.window && slot <= s.e0 - a.window && slot + 15 >= a.sinks)) {
-          for (int i = lane; i < KF_SLOTS * NT; i += 32) {
+          for (int i = lane; i < KF_SLOTS * TD; i += 32) {
             const int r = i & 15;
             if (!kv_any_sees(s, slot + r, a.window, a.sinks)) *(uint4 *)(smem + (v_s - bar_s) + (i >> 7) * (KF_SLOTS * 128) + r * 128 + ((i >> 4) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
+        float y[2][2][4];                                  // even and odd steps: shorter chains
+#pragma unroll
+        for (int i = 0; i < 16; i++) y[i >> 3][(i >> 2) & 1][i & 3] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ks++) {
           uint32_t qa[4], kb[4];
@@ -238,19 +257,22 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
           kf_ldsm(qa, q_s + (2 * ks + (mi >> 1)) * 256 + (lr + 8 * (mi & 1)) * 16);
           const int unit = 2 * ks + (mi & 1), row = lr + 8 * (mi >> 1);
           kf_ldsm(kb, k_s + (unit >> 3) * (KF_SLOTS * 128) + row * 128 + (((unit & 7) ^ lr) << 4));
-          kf_mma<T>(x[0], qa, kb[0], kb[1]);
-          kf_mma<T>(x[1], qa, kb[2], kb[3]);
+          kf_mma<T>(y[ks & 1][0], qa, kb[0], kb[1]);
+          kf_mma<T>(y[ks & 1][1], qa, kb[2], kb[3]);
         }
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = (y[0][i >> 2][i & 3] + y[1][i >> 2][i & 3]) * a.scale2;
       }
       const bool whole = !none && slot + 15 <= ea && (!a.window || slot > ez - a.window || slot + 15 < a.sinks) && q0 + 15 < NQ;
+      if (!whole) {
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int j = slot + 8 * t + j2 + (k & 1), w = k >> 1;
-          x[t][k] *= a.scale2;
-          if (!whole && (none || j > e[w] || (j < lw[w] && j >= a.sinks))) x[t][k] = -INFINITY;
-        }
+          for (int k = 0; k < 4; k++) {
+            const int j = slot + 8 * t + j2 + (k & 1), w = k >> 1;
+            if (none | (j > e[w]) | ((j < lw[w]) & (j >= a.sinks))) x[t][k] = -INFINITY;
+          }
+      }
       if constexpr (WT) {
 #pragma unroll
         for (int w = 0; w < 2; w++)
@@ -277,11 +299,11 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
       if (!none) {
         if (__any_sync(0xffffffffu, cf[0] != 1.0f || cf[1] != 1.0f)) {
 #pragma unroll
-          for (int i = 0; i < NT; i++) { o[i][0] *= cf[0]; o[i][1] *= cf[0]; o[i][2] *= cf[1]; o[i][3] *= cf[1]; }
+          for (int i = 0; i < TD; i++) { o[i][0] *= cf[0]; o[i][1] *= cf[0]; o[i][2] *= cf[1]; o[i][3] *= cf[1]; }
         }
         const uint32_t pa[4] = {KvEl<T>::of2(x[0][0], x[0][1]), KvEl<T>::of2(x[0][2], x[0][3]), KvEl<T>::of2(x[1][0], x[1][1]), KvEl<T>::of2(x[1][2], x[1][3])};
 #pragma unroll
-        for (int i = 0; i < NT; i += 2) {
+        for (int i = 0; i < TD; i += 2) {
           uint32_t vb[4];                                  // matrix mi: slots 8 (mi & 1) .., dims 8 (i + mi / 2) ..
           const int unit = i + (mi >> 1), row = lr + 8 * (mi & 1);
           kf_ldsm_t(vb, v_s + (unit >> 3) * (KF_SLOTS * 128) + row * 128 + (((unit & 7) ^ lr) << 4));
@@ -289,73 +311,77 @@ __global__ void __launch_bounds__(32 * KF_WARPS, HD == 256 ? 1 : 2) k_kv_few(con
           kf_mma<T>(o[i + 1], pa, vb[2], vb[3]);
         }
       }
-      __syncwarp();                                        // the stage has been read
-      if (!dead) issue();
+      __syncwarp();                                        // the chunk has been read
+      if (lane == 0) mbar_arrive(bar_s + 256 + 8 * st);
     }
-    // ---- the warps' sums put together: a tree where two have room (2 and 3 to 0 and 1, 1 to 0), else 3, 2 and 1 to 0 ----
+    n0 += use.c1 - use.c0;
+    // ---- the warps' sums put together: everything relative to the largest maximum, then 32 dims at a time ----
 #pragma unroll
-    for (int w = 0; w < 2; w++) { l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1); l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2); }
-    auto leave = [&](int at) {
-      float *d = sums + at * 16 * ROW;
-#pragma unroll
-      for (int i = 0; i < NT; i++) {
-        *(float2 *)(d + gid * ROW + 8 * i + j2) = make_float2(o[i][0], o[i][1]);
-        *(float2 *)(d + (gid + 8) * ROW + 8 * i + j2) = make_float2(o[i][2], o[i][3]);
-      }
-      if (j2 == 0) { hd.m[at][gid] = m[0]; hd.m[at][gid + 8] = m[1]; hd.l[at][gid] = l[0]; hd.l[at][gid + 8] = l[1]; }
-    };
-    auto add = [&](int at) {
-      const float *d = sums + at * 16 * ROW;
-      float fa[2], fb[2];
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        const float mb = hd.m[at][gid + 8 * w], t = fmaxf(m[w], mb), ref = t == -INFINITY ? 0.0f : t;
-        fa[w] = kv_exp2(m[w] - ref); fb[w] = kv_exp2(mb - ref);
-        l[w] = l[w] * fa[w] + hd.l[at][gid + 8 * w] * fb[w];
-        m[w] = t;
-      }
-#pragma unroll
-      for (int i = 0; i < NT; i++) {
-        const float2 u = *(const float2 *)(d + gid * ROW + 8 * i + j2), v = *(const float2 *)(d + (gid + 8) * ROW + 8 * i + j2);
-        o[i][0] = o[i][0] * fa[0] + u.x * fb[0]; o[i][1] = o[i][1] * fa[0] + u.y * fb[0];
-        o[i][2] = o[i][2] * fa[1] + v.x * fb[1]; o[i][3] = o[i][3] * fa[1] + v.y * fb[1];
-      }
-    };
-    const int used = min(KF_WARPS, use.c1 - use.c0);       // warps that had a chunk
-#pragma unroll 1
-    for (int src = KF_WARPS - 1; src > 0; src = NB == 2 ? src >> 1 : src - 1) {   // NB 2: 3 (with 2), then 1
-      if (NB == 2 ? src == 3 && used < 3 : src >= used) continue;
-      if (src == 1 && used < 2) continue;
-      if (NB == 2 && src == 3) { if (warp >= 2) leave(warp - 2); }
-      else if (warp == src) leave(0);
-      __syncthreads();
-      if (NB == 2 && src == 3) { if (warp < 2) add(warp); }
-      else if (warp == 0) add(0);
-      __syncthreads();
+    for (int w = 0; w < 2; w++) {
+      l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1); l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
+      if (j2 == 0) { hd.m[warp][gid + 8 * w] = m[w]; hd.l[warp][gid + 8 * w] = l[w]; }
     }
-    if (warp == 0) leave(0);
-    __syncthreads();
+    meet();
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      float M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int k = 0; k < CW; k++) M = fmaxf(M, hd.m[k][gid + 8 * w]);
+      const float ref = M == -INFINITY ? 0.0f : M, f = kv_exp2(m[w] - ref);
+      if (warp == 0) {
+#pragma unroll
+        for (int k = 0; k < CW; k++) L += hd.l[k][gid + 8 * w] * kv_exp2(hd.m[k][gid + 8 * w] - ref);
+        if (j2 == 0) { hd.M[gid + 8 * w] = M; hd.L[gid + 8 * w] = L; }
+      }
+#pragma unroll
+      for (int i = 0; i < TD; i++) { o[i][2 * w] *= f; o[i][2 * w + 1] *= f; }
+    }
     const bool wholly = use.c0 == 0 && use.c1 == s.chunks;
     const size_t part = ((size_t)blockIdx.x * 2 + (use.c0 == 0)) * 16;
-#pragma unroll 1
-    for (int r = warp; r < 16 && q0 + r < NQ; r += KF_WARPS) {
-      float v[E];
 #pragma unroll
-      for (int k = 0; k < E; k++) v[k] = sums[r * ROW + lane * E + k];
-      const int row = (q0 + r) / a.G, h = use.g * a.G + (q0 + r) % a.G;
-      if (wholly) {
-        if (WT && lane == 0) p.lse[((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + r] = hd.l[0][r] > 0.0f ? hd.m[0][r] + log2f(hd.l[0][r]) : INFINITY;
-        kv_finish<T, HD>(c, a, use.b, s.first + row, h, s.e0 + row, lane, v, hd.m[0][r], hd.l[0][r]);
-      } else {
-        if (lane == 0) { p.pm[part + r] = hd.m[0][r]; p.pl[part + r] = hd.l[0][r]; }
+    for (int d0 = 0; d0 < HD; d0 += 32) {
+      float *d = sums + warp * 16 * KF_ROW;
 #pragma unroll
-        for (int k = 0; k < E; k += 2) *(float2 *)(p.po + (part + r) * HD + lane * E + k) = make_float2(v[k], v[k + 1]);
+      for (int i = 0; i < 4; i++) {
+        *(float2 *)(d + gid * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][0], o[d0 / 8 + i][1]);
+        *(float2 *)(d + (gid + 8) * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][2], o[d0 / 8 + i][3]);
       }
+      meet();
+#pragma unroll 1
+      for (int it = tid; it < 256; it += 32 * CW) {        // a row, two dims of the 32
+        const int r = it >> 4, dd = 2 * (it & 15), qi = q0 + r;
+        if (qi >= NQ) break;
+        float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < CW; k++) { const float2 t = *(const float2 *)(sums + (k * 16 + r) * KF_ROW + dd); v.x += t.x; v.y += t.y; }
+        if (!wholly) { *(float2 *)(p.po + (part + r) * HD + d0 + dd) = v; continue; }
+        const int row = kv_row_of(a, qi), h = use.g * a.G + qi - row * a.G;
+        const float L = hd.L[r], inv = L == 0.0f ? 0.0f : 1.0f / L;   // (nothing seen: zeros)
+        if (!(fabsf(v.x) + fabsf(v.y) + L < INFINITY)) hd.odd[r] = 1;
+        const long long at = (long long)(s.first + row) * a.os + (long long)h * HD + d0 + dd;
+        if (a.out32) *(float2 *)((float *)a.out + at) = make_float2(v.x * inv, v.y * inv);
+        else *(uint32_t *)((uint16_t *)a.out + at) = KvEl<T>::of2(v.x * inv, v.y * inv);
+      }
+      meet();
+    }
+    if (tid < 16 && q0 + tid < NQ) {
+      if (!wholly) { p.pm[part + tid] = hd.M[tid]; p.pl[part + tid] = hd.L[tid]; }
+      else if (WT) p.lse[((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + tid] = hd.L[tid] > 0.0f ? hd.M[tid] + log2f(hd.L[tid]) : INFINITY;
+    }
+    // rows whose result is no number once more, by themselves (kv_attn_row says why)
+#pragma unroll 1
+    for (int k = warp; wholly && k < 16; k += CW) {
+      if (!hd.odd[k]) continue;
+      const int rk = kv_row_of(a, q0 + k), hk = use.g * a.G + q0 + k - rk * a.G;
+      float v[HD / 32], mk, lk;
+      kv_attn_row<T, HD>(c, a, use.b, s.first + rk, hk, s.e0 + rk, lane, v, mk, lk);
+      kv_store<T, HD>(a, s.first + rk, hk, lane, v, lk);
+      __syncwarp();
+      if (lane == 0) hd.odd[k] = 0;
     }
     if (!use.next(c, rw, a)) break;
-    __syncthreads();                                       // (the queries' and sums' memory is free again)
+    meet();                                                // (the queries' and sums' memory is free again)
   }
-  if (dead) for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies may be on their way
 }
 
 // blocks that have a part of the unit that begins `at` chunks into the call: first, last

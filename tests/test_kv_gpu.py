@@ -346,6 +346,19 @@ def test_a_long_sequence_beside_short_ones(llb, window, sinks):
     _clean(llb)
 
 
+@pytest.mark.parametrize("form", [(16, 4, 256), (8, 2, 128), (4, 2, 64)])
+def test_stretches_that_go_round_the_ring_many_times(llb, form):
+    """Sequences enough for blocks that bring a few hundred chunks through their rings, over the ends of units, twice with the same bits."""
+    H, KV, hd = form
+    lens = [16000, 900, 12345, 16, 9000, 15999, 1, 7000, 11111, 14000]
+    c = Cache(llb, "bf16", KV, hd, 64, lens, seed=63)
+    one = _attn(llb, c, H, [1] * len(lens), seed=64)
+    _check_attn(c, one)
+    for _ in range(5):
+        assert torch.equal(one["out"], _attn(llb, c, H, [1] * len(lens), seed=64)["out"])
+    _clean(llb)
+
+
 def test_weights_in_place_and_from_nothing(llb):
     c = Cache(llb, "bf16", 2, 128, 16, [400, 90], seed=25)
     r = _attn(llb, c, 8, [2, 1], weights=True, seed=26)
