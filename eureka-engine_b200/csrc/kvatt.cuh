@@ -25,7 +25,7 @@ __host__ __device__ constexpr int kf_bytes(int HD) { return 2 * KF_SLOTS * HD * 
 struct KfHead {                // before the ring
   uint64_t full[32], empty[32];
   long long sum[16], rem;
-  int b, bad[32], odd[16];
+  int b, bad[32], odd[16], ids[32];
   float m[11][16], l[11][16], M[16], L[16];
 };
 #define KF_HEAD 3072
@@ -37,7 +37,7 @@ static_assert(kf_smem(256) <= 232448 && kf_smem(128) <= 232448 && kf_smem(64) <=
 
 struct KvPlan {
   int least;                   // chunks of a block's stretch, at least
-  long long *before;           // [seqs + 2]: chunks of the sequences before; all; chunks of a stretch
+  int *unit;                   // [seqs][KV][16-query tiles][2]: the first and the last block that had a part of the unit
   float *pm, *pl, *po;         // [2 blocks][16](, [hd])
   float *sc;                   // [seqs][KV][G max_rows][sstride]: scores, where weights are wanted
   float *lse;                  // [seqs][KV][G max_rows]: of units that one block has wholly
@@ -129,12 +129,6 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
 #pragma unroll
   for (int w = 0; w <= CW; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
   const long long per = max((long long)p.least, (all + gridDim.x - 1) / gridDim.x), start = per * blockIdx.x;
-  if (blockIdx.x == 0) {
-    long long at = to - mine;
-#pragma unroll 1
-    for (int b = ba; b < bz; b++) { p.before[b] = at; at += work(b); }
-    if (tid == 0) { p.before[c.seqs] = all; p.before[c.seqs + 1] = per; }
-  }
   if (start >= all) return;
   if (to - mine <= start && start < to) {
     long long at = to - mine;
@@ -173,15 +167,17 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       int next = pages(use.c0);
 #pragma unroll 1
       for (int c0 = use.c0; c0 < use.c1; c0 += 32) {
-        asm volatile("" : "+r"(next));
-        const int ids = next, n = min(32, use.c1 - c0);
+        const int n = min(32, use.c1 - c0);
+        __syncwarp();
+        hd.ids[lane] = next;
+        __syncwarp();
         next = pages(c0 + 32);
+        if (lane == 0) {                                   // one thread: a warp that walks together takes three times as long a request
 #pragma unroll 1
-        for (int k = 0; k < n; k++) {
-          const int id = __shfl_sync(0xffffffffu, ids, k), slot = kv_chunk_slot(use.s, c0 + k, KF_SH) & pm;
-          if (round) wait(bar_s + 256 + 8 * st, (round - 1) & 1u);
-          if (lane == 0) {
+          for (int k = 0; k < n; k++) {
+            const int id = hd.ids[k], slot = kv_chunk_slot(use.s, c0 + k, KF_SH) & pm;
             const uint32_t full = bar_s + 8 * st;
+            if (round && !dead && !mbar_wait(full + 256, (round - 1) & 1u)) { dead = true; atomicExch(p.err, 1u); }
             const bool in = (unsigned)id < (unsigned)c.n_pages && !dead;
             hd.bad[st] = !in;
             if (in) {
@@ -192,10 +188,10 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
               if (seen && !dead) atomicOr(c.err, KV_ERR_PAGE);
               mbar_arrive(full);
             }
+            if (++st == NS) { st = 0; round++; }
           }
-          __syncwarp();
-          if (++st == NS) { st = 0; round++; }
         }
+        __syncwarp();
       }
     } while (use.next(c, rw, a));
     if (dead) for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies may be on their way
@@ -337,6 +333,11 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       for (int i = 0; i < TD; i++) { o[i][2 * w] *= f; o[i][2 * w + 1] *= f; }
     }
     const bool wholly = use.c0 == 0 && use.c1 == s.chunks;
+    if (tid == 0) {
+      int *u = p.unit + (((size_t)use.b * c.KV + use.g) * ((a.G * rw.max_rows + 15) >> 4) + use.qt) * 2;
+      if (use.c0 == 0) u[0] = blockIdx.x;
+      if (use.c1 == s.chunks) u[1] = blockIdx.x;
+    }
     const size_t part = ((size_t)blockIdx.x * 2 + (use.c0 == 0)) * 16;
 #pragma unroll
     for (int d0 = 0; d0 < HD; d0 += 32) {
@@ -384,91 +385,95 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
   }
 }
 
-// blocks that have a part of the unit that begins `at` chunks into the call: first, last
-__device__ __forceinline__ void kf_parts(const KvPlan &p, long long at, int chunks, long long per, int &w0, int &w1) {
-  w0 = (int)(at / per); w1 = (int)((at + chunks - 1) / per);
-}
-__device__ __forceinline__ size_t kf_part(long long at, long long per, int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }   // (only the first begins with the unit's first chunk)
+// the part of a unit that block w had, of blocks w0 .. (only the first begins with the unit's first chunk)
+__device__ __forceinline__ size_t kf_part(int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }
 
-// Units that several blocks had: a block a query, its four warps the parts in turn.  Blocks from `joins` on: what every slot got, 512 slots of a kv head each.
+// Units that several blocks had: a block a query, its four warps the parts in turn, each with what it needs of them asked for at once.  Blocks from
+// `joins` on: what every slot got, 512 slots of a kv head each.
 template <typename T, int HD, bool WT>
 __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
   constexpr int E = HD / 32;
   __shared__ float sm[4], sl[4], so[4][HD], lse[64];
   pdl_trigger();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NQM = a.G * rw.max_rows;
-  const long long per = __ldcg(p.before + c.seqs + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NQM = a.G * rw.max_rows, QTM = (NQM + 15) >> 4;
   if (!WT || blockIdx.x < joins) {
-    const int qi = blockIdx.x % NQM, g = blockIdx.x / NQM % c.KV, b = blockIdx.x / NQM / c.KV;
+    const int qi = blockIdx.x % NQM, gb = blockIdx.x / NQM, g = gb % c.KV, b = gb / c.KV;
+    const int2 w = __ldcg((const int2 *)p.unit + (size_t)gb * QTM + (qi >> 4));
     const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
-    if (qi >= a.G * s.nc) return;
-    const int qts = (a.G * s.nc + 15) >> 4;
-    int w0, w1;
-    const long long at = __ldcg(p.before + b) + ((long long)g * qts + (qi >> 4)) * s.chunks;
-    kf_parts(p, at, s.chunks, per, w0, w1);
-    if (w0 == w1) return;
-    float M = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, __ldcg(p.pm + kf_part(at, per, w, w0) + (qi & 15)));
-#pragma unroll
-    for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float o[E], l = 0.0f;
+    if (qi >= a.G * s.nc || w.x == w.y) return;
+    float o[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; k++) o[k] = 0.0f;
-#pragma unroll 4
-    for (int w = w0 + warp; w <= w1; w += 4) {
-      const size_t i = kf_part(at, per, w, w0) + (qi & 15);
-      const float f = exp2f(__ldcg(p.pm + i) - ref);
-      l += __ldcg(p.pl + i) * f;
+#pragma unroll 2
+    for (int i = w.x + warp; i <= w.y; i += 4) {
+      const size_t at = kf_part(i, w.x) + (qi & 15);
+      const float pm = __ldcg(p.pm + at), pl = __ldcg(p.pl + at);
+      float2 v[E / 2];
 #pragma unroll
-      for (int k = 0; k < E; k += 2) { const float2 v = __ldcg((const float2 *)(p.po + i * HD + lane * E + k)); o[k] += v.x * f; o[k + 1] += v.y * f; }
+      for (int k = 0; k < E / 2; k++) v[k] = __ldcg((const float2 *)(p.po + at * HD + lane * E) + k);
+      const float t = fmaxf(m, pm), ref = t == -INFINITY ? 0.0f : t, f = kv_exp2(m - ref), fp = kv_exp2(pm - ref);
+      l = l * f + pl * fp;
+      m = t;
+#pragma unroll
+      for (int k = 0; k < E / 2; k++) { o[2 * k] = o[2 * k] * f + v[k].x * fp; o[2 * k + 1] = o[2 * k + 1] * f + v[k].y * fp; }
     }
-    if (lane == 0) sl[warp] = l;
+    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
 #pragma unroll
-    for (int k = 0; k < E; k++) so[warp][lane * E + k] = o[k];
+    for (int k = 0; k < E; k += 2) *(float2 *)&so[warp][lane * E + k] = make_float2(o[k], o[k + 1]);
     __syncthreads();
     if (warp) return;
-    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), ref = M == -INFINITY ? 0.0f : M;
+    float f[4];
+    l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < E; k++) o[k] = (so[0][lane * E + k] + so[1][lane * E + k]) + (so[2][lane * E + k] + so[3][lane * E + k]);
-    const int row = qi / a.G;
-    kv_finish<T, HD>(c, a, b, s.first + row, g * a.G + qi % a.G, s.e0 + row, lane, o, M, l);
+    for (int i = 0; i < 4; i++) { f[i] = kv_exp2(sm[i] - ref); l += sl[i] * f[i]; }
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+      o[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[k] += so[i][lane * E + k] * f[i];
+    }
+    const int row = kv_row_of(a, qi);
+    kv_finish<T, HD>(c, a, b, s.first + row, g * a.G + qi - row * a.G, s.e0 + row, lane, o, M, l);
     return;
   }
   if constexpr (WT) {
-    const int u = blockIdx.x - joins, wb = u % wblocks, g = u / wblocks % c.KV, b = u / wblocks / c.KV;
+    const int u = blockIdx.x - joins, wb = u % wblocks, gb = u / wblocks, b = gb / c.KV;
     const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
     if (wb * 512 >= s.len) return;
-    const int qts = (a.G * s.nc + 15) >> 4, NQ = a.G * s.nc;
-    const size_t ug = (size_t)b * c.KV + g;
+    const int NQ = a.G * s.nc;
+    const size_t ug = gb;
     if (tid < NQ) {
-      int w0, w1;
-      const long long at = __ldcg(p.before + b) + ((long long)g * qts + (tid >> 4)) * s.chunks;
-      kf_parts(p, at, s.chunks, per, w0, w1);
-      if (w0 == w1) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
+      const int2 w = __ldcg((const int2 *)p.unit + ug * QTM + (tid >> 4));
+      if (w.x == w.y) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
       else {
         float M = -INFINITY, l = 0.0f;
 #pragma unroll 4
-        for (int w = w0; w <= w1; w++) M = fmaxf(M, __ldcg(p.pm + kf_part(at, per, w, w0) + (tid & 15)));
+        for (int i = w.x; i <= w.y; i++) M = fmaxf(M, __ldcg(p.pm + kf_part(i, w.x) + (tid & 15)));
         const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll 4
-        for (int w = w0; w <= w1; w++) { const size_t i = kf_part(at, per, w, w0) + (tid & 15); l += __ldcg(p.pl + i) * exp2f(__ldcg(p.pm + i) - ref); }
+        for (int i = w.x; i <= w.y; i++) { const size_t at = kf_part(i, w.x) + (tid & 15); l += __ldcg(p.pl + at) * exp2f(__ldcg(p.pm + at) - ref); }
         lse[tid] = l > 0.0f ? M + log2f(l) : INFINITY;
       }
     }
     __syncthreads();
+    float sum[4] = {0.f, 0.f, 0.f, 0.f}, in[4] = {0.f, 0.f, 0.f, 0.f};
+    const float *x = p.sc + ug * NQM * p.sstride + wb * 512 + tid;
+    bool on[4], see[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const int j = wb * 512 + k * 128 + tid;
-      if (j >= s.len) return;
-      float sum = 0.0f;
-      if (NQ && kv_any_sees(s, j, a.window, a.sinks)) {
-        const float *x = p.sc + ug * NQM * p.sstride + j;
-#pragma unroll 4
-        for (int q = 0; q < NQ; q++) sum += exp2f(__ldcg(x + (size_t)q * p.sstride) - lse[q]);
-      }
-      a.w_out[ug * a.wstride + j] = (a.w_in ? __ldcg(a.w_in + ug * a.wstride + j) : 0.0f) + sum;
+      on[k] = j < s.len; see[k] = on[k] && kv_any_sees(s, j, a.window, a.sinks);
+      if (on[k] && a.w_in) in[k] = __ldcg(a.w_in + ug * a.wstride + j);
     }
+#pragma unroll 4
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (see[k]) sum[k] += kv_exp2(__ldcs(x + (size_t)q * p.sstride + k * 128) - lse[q]);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (on[k]) a.w_out[ug * a.wstride + wb * 512 + k * 128 + tid] = in[k] + sum[k];
   }
 }
