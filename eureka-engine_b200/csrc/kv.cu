@@ -357,7 +357,7 @@ static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int 
 }
 // ---- which kernel, and its workspace ----
 #define KV_FEW 64              // queries a kv head up to which a call goes to k_kv_few
-#define KF_LEAST 8             // fewest chunks of a block's stretch: two a warp
+#define KF_LEAST 2             // fewest groups of a block's stretch
 static int most_rows(const llb_kv_attn *a) { return std::min(a->max_rows, std::max(a->rows, 1)); }
 static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * most_rows(a) <= KV_FEW; }
 static int few_grid(void) { return g_llb.sms ? g_llb.sms : 148; }
@@ -381,7 +381,8 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   few_plan(kv, call, (uintptr_t)call->ws, &p);
   p.err = gemm_err_word();
   CUtensorMap km, vm;
-  if (pool_map(&km, kv, kv->k, KF_SLOTS, HD / 64) || pool_map(&vm, kv, kv->v, KF_SLOTS, HD / 64)) return -1;
+  const int slots = std::min(kv->page, 1 << kf_sh(HD));
+  if (pool_map(&km, kv, kv->k, slots, HD / 64) || pool_map(&vm, kv, kv->v, slots, HD / 64)) return -1;
   const dim3 grid(few_grid()), block(32 * (kf_warps(HD) + 1));
   const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + 511) / 512;   // (attn_check: they fit)
   if (a.w_out) {
@@ -441,6 +442,8 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");
   if (a->w_in && !a->w_out) return llb_fail("kv_attn: w_in without w_out");
   const long long queries = (long long)a->heads / kv->kv_heads * most_rows(a), pairs = (long long)kv->seqs * kv->kv_heads;
+  if (queries <= KV_FEW && pairs * ((queries + 15) / 16) > INT_MAX / 2 / (a->max_len / 32 + 3))
+    return llb_fail("kv_attn: %d sequences of %d kv heads with up to %d slots: more than are counted (max_len bounds it)", kv->seqs, kv->kv_heads, a->max_len);
   if (queries >= 1 << 26 || pairs * (std::min(queries, (queries + 127) / 128 + KV_FEW) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
     return llb_fail("kv_attn: %d sequences of %d kv heads, %d rows, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, most_rows(a), a->max_len);
   if (a->w_out) {

@@ -1,42 +1,46 @@
 // kvatt.cuh -- attention of the few rows of a decode or verify step over the paged cache: bound by the cache's bytes.
 //
 // A unit is (sequence, kv head, 16 queries); its queries are the rows' heads side by side, query i G + h is row i, head h of the kv head's
-// G.  What a unit sees is cut into chunks of 16 slots, a page's part each, and the chunks of all units, one after the other, into as many
-// equal stretches as there are blocks, so that sequences of any lengths keep every SM busy to the end; a block's stretch may begin and end inside a unit.
-// A warp of the block brings the chunks by TMA (rows of 128 swizzled bytes) into a ring, on over the ends of units; the others take them in turn.
+// G.  What a unit sees is cut into groups of 32 or 64 slots, and the groups of all units, one after the other, into as many equal stretches as
+// there are blocks, so that sequences of any lengths keep every SM busy to the end; a block's stretch may begin and end inside a unit.
+// A thread of the block requests the groups (TMA, a box a page, rows of 128 swizzled bytes) and every unit's queries, on over the ends of units; the other
+// warps take 16 slots of a group each.
 //   S[query][slot] = Q K^T      m16n8k16, 16 queries x 16 slots
 //   O[query][dim] += P V        P from the registers of S, rounded to the cache's type (the second product takes 16-bit operands)
-// with the maximum and the sum of every query kept in f32.  Where a unit ends the warps' sums are put together, 32 dims at a time.  A unit that one
+// with the maximum and the sum of every query kept in f32.  Where a unit ends the warps' sums are put together, some dims at a time.  A unit that one
 // block has wholly is finished there; the others' sums go to the workspace, and k_kv_join, the second launch, puts them together in the order of the blocks.
 //
-// A chunk is a chain of some 2000 to 4000 cycles for its warp (two products with the softmax between), which is why so many warps work on chunks of their own.
+// 16 slots are a chain of 1500 to 2000 cycles for their warp (two products with the softmax between), which is why several warps work on slots of their own; a
+// request takes its thread 100 cycles a box whatever the box's size, 500 for 16 slots' K and V with all around them, which is why groups are 32 KB.
 #pragma once
 #include <cuda.h>
 
 #include "kv.cuh"
 #include "tc5.cuh"
 
-#define KF_SLOTS 16
-#define KF_SH 4
-__host__ __device__ constexpr int kf_warps(int HD) { return HD == 256 ? 6 : 11; }   // that compute
-__host__ __device__ constexpr int kf_ring(int HD) { return HD == 256 ? 12 : 22; }    // chunks that have room
-__host__ __device__ constexpr int kf_bytes(int HD) { return 2 * KF_SLOTS * HD * 2; }                  // of a chunk: K, then V
+__host__ __device__ constexpr int kf_sh(int HD) { return HD == 256 ? 5 : 6; }                         // log2 of a group's slots
+__host__ __device__ constexpr int kf_parts(int HD) { return 1 << (kf_sh(HD) - 4); }                   // of 16 slots in it
+__host__ __device__ constexpr int kf_warps(int HD) { return HD == 256 ? 6 : 8; }                      // that compute
+__host__ __device__ constexpr int kf_ring(int HD) { return HD == 64 ? 8 : 6; }                        // groups that have room
+__host__ __device__ constexpr int kf_bytes(int HD) { return 2 * HD * 2 << kf_sh(HD); }                // of a group: K, then V
+__host__ __device__ constexpr int kf_qrow(int HD) { return HD * 2 + 16; }                             // bytes from a query to the next: four banks on
 #define KF_ROW 40              // floats from a row of the warps' sums to the next: 32 dims, and eight banks on
 struct KfHead {                // before the ring
-  uint64_t full[32], empty[32];
-  long long sum[16], rem;
-  int b, bad[32], odd[16], ids[32];
-  float m[11][16], l[11][16], M[16], L[16];
+  uint64_t full[8], empty[8], qfull[2], qempty[2];
+  int sum[16], b, rem;
+  KvSeq s;
+  int bad[8], odd[16], ids[32];   // bad: a bit for 16 slots of a group whose page is no page
+  float m[8][16], l[8][16], M[16], L[16];
 };
-#define KF_HEAD 3072
-// A place of the ring is one warp's: a warp that came to it after another would take the phase before the other's for its own where that one's copy is late.
-static_assert(kf_ring(256) % kf_warps(256) == 0 && kf_ring(128) % kf_warps(128) == 0 && kf_ring(64) % kf_warps(64) == 0 && kf_ring(64) <= 32, "a place of the ring is one warp's");
+#define KF_HEAD 2048
 static_assert(sizeof(KfHead) <= KF_HEAD, "the ring begins after it");
-__host__ __device__ constexpr int kf_smem(int HD) { return KF_HEAD + kf_ring(HD) * kf_bytes(HD) + kf_warps(HD) * 16 * KF_ROW * 4 + 16 * HD * 2; }
+// 16 slots' place in the ring is one warp's: a warp that came to it after another would take the phase before the other's for its own where that one's copy is late.
+static_assert(kf_ring(256) * kf_parts(256) % kf_warps(256) == 0 && kf_ring(128) * kf_parts(128) % kf_warps(128) == 0 && kf_ring(64) * kf_parts(64) % kf_warps(64) == 0, "a place is one warp's");
+__host__ __device__ constexpr int kf_smem(int HD) { return KF_HEAD + kf_ring(HD) * kf_bytes(HD) + kf_warps(HD) * 16 * KF_ROW * 4 + 2 * 16 * kf_qrow(HD); }
 static_assert(kf_smem(256) <= 232448 && kf_smem(128) <= 232448 && kf_smem(64) <= 232448, "shared memory");
 
 struct KvPlan {
-  int least;                   // chunks of a block's stretch, at least
+  int least;                   // groups of a block's stretch, at least
   int *unit;                   // [seqs][KV][16-query tiles][2]: the first and the last block that had a part of the unit
   float *pm, *pl, *po;         // [2 blocks][16](, [hd])
   float *sc;                   // [seqs][KV][G max_rows][sstride]: scores, where weights are wanted
@@ -69,13 +73,17 @@ __device__ __forceinline__ void kv_expect(uint32_t bar_s, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_s), "r"(bytes) : "memory");
 }
 
-// a block's way through its stretch: the unit it is in, and the chunks c0 .. c1 - 1 of it that are the block's
-struct KfWalk {
+// so many bytes from global to shared memory, counted on a barrier
+__device__ __forceinline__ void kv_bulk(uint32_t dst_s, const void *src, uint32_t bytes, uint32_t bar_s) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_s), "l"(src), "r"(bytes), "r"(bar_s) : "memory");
+}
+// a block's way through its stretch: the unit it is in, and the groups c0 .. c1 - 1 of it that are the block's
+template <int SH> struct KfWalk {
   KvSeq s;
   int b, g, qt, c0, c1;
-  long long left;              // chunks of the stretch behind this unit's
+  int left;                    // groups of the stretch behind this unit's
   __device__ __forceinline__ void take() {
-    c1 = (int)min((long long)s.chunks, c0 + left);
+    c1 = min(s.chunks, c0 + left);
     left -= c1 - c0;
   }
   __device__ __forceinline__ bool next(const KvDev &c, const KvRows &r, const KvAttn &a) {
@@ -87,7 +95,7 @@ struct KfWalk {
         g = 0;
         do {
           if (++b >= c.seqs) { left = 0; return false; }
-          s = kv_seq(c, r, b, a.window, a.sinks, KF_SH);
+          s = kv_seq(c, r, b, a.window, a.sinks, SH);
         } while (!s.chunks);
       }
     }
@@ -99,117 +107,140 @@ struct KfWalk {
 template <typename T, int HD, bool WT>
 __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
                                                                       const __grid_constant__ CUtensorMap vm) {
-  constexpr int CW = kf_warps(HD), NT = 32 * (CW + 1), NS = kf_ring(HD), SB = kf_bytes(HD), KB = SB / 2, TD = HD / 8;   // TD: tiles of eight dims
+  constexpr int CW = kf_warps(HD), NT = 32 * (CW + 1), NG = kf_ring(HD), SB = kf_bytes(HD), KB = SB / 2, TD = HD / 8, SH = kf_sh(HD), PG = kf_parts(HD), QR = kf_qrow(HD);   // TD: tiles of eight dims
   extern __shared__ __align__(1024) uint8_t smem[];
   KfHead &hd = *(KfHead *)smem;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, j2 = 2 * (lane & 3), lr = lane & 7, mi = lane >> 3;
-  const uint32_t bar_s = smem_u32(smem), ring_s = bar_s + KF_HEAD, q_s = ring_s + NS * SB + CW * 16 * KF_ROW * 4;   // queries: rows of 16 bytes, [dims / 8][16]
-  float *sums = (float *)(smem + KF_HEAD + NS * SB);                     // [warp][16][KF_ROW]
-  uint8_t *q_m = smem + (q_s - bar_s);
-  if (tid < 32) { mbar_init(bar_s + 8 * tid, 1); mbar_init(bar_s + 256 + 8 * tid, 1); }
+  const uint32_t bar_s = smem_u32(smem), ring_s = bar_s + KF_HEAD, q_s = ring_s + NG * SB + CW * 16 * KF_ROW * 4;   // two units' queries
+  float *sums = (float *)(smem + KF_HEAD + NG * SB);                     // [warp][16][KF_ROW]
+  auto full = [&](int i) { return bar_s + 8u * (uint32_t)i; };
+  auto empty = [&](int i) { return bar_s + 64u + 8u * (uint32_t)i; };
+  auto qfull = [&](int i) { return bar_s + 128u + 8u * (uint32_t)i; };
+  auto qempty = [&](int i) { return bar_s + 144u + 8u * (uint32_t)i; };
+  if (tid < 8) { mbar_init(full(tid), 1); mbar_init(empty(tid), PG); }
+  if (tid < 2) { mbar_init(qfull(tid), 1); mbar_init(qempty(tid), 1); }
   if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   if (tid < 16) hd.odd[tid] = 0;
   pdl_trigger();
   pdl_wait();
-  // ---- the block's stretch: chunks of every sequence, summed over the threads' runs of sequences ----
+  // ---- the block's stretch: groups of every sequence, summed over the threads' runs of sequences ----
   const int run = (c.seqs + NT - 1) / NT, ba = min(c.seqs, tid * run), bz = min(c.seqs, ba + run);
+  KvSeq seq;
   auto work = [&](int b) {
-    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
-    return (long long)s.chunks * c.KV * ((a.G * s.nc + 15) >> 4);
+    seq = kv_seq(c, rw, b, a.window, a.sinks, SH);
+    return seq.chunks * c.KV * ((a.G * seq.nc + 15) >> 4);
   };
-  long long mine = 0;
+  int mine = 0;
 #pragma unroll 1
   for (int b = ba; b < bz; b++) mine += work(b);
-  long long to = mine;
+  int to = mine;
 #pragma unroll
-  for (int m = 1; m < 32; m <<= 1) { const long long o = __shfl_up_sync(0xffffffffu, to, m); if (lane >= m) to += o; }
+  for (int m = 1; m < 32; m <<= 1) { const int o = __shfl_up_sync(0xffffffffu, to, m); if (lane >= m) to += o; }
   if (lane == 31) hd.sum[warp] = to;
   __syncthreads();
-  long long all = 0;
+  int all = 0;
 #pragma unroll
   for (int w = 0; w <= CW; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
-  const long long per = max((long long)p.least, (all + gridDim.x - 1) / gridDim.x), start = per * blockIdx.x;
-  if (start >= all) return;
+  const int per = max(p.least, (all + (int)gridDim.x - 1) / (int)gridDim.x);
+  if (blockIdx.x >= (all + per - 1) / per) return;
+  const int start = per * blockIdx.x;
   if (to - mine <= start && start < to) {
-    long long at = to - mine;
-    int b = ba;
+    int at = to - mine, b = ba;
 #pragma unroll 1
-    for (;; b++) { const long long w = work(b); if (start < at + w) break; at += w; }
-    hd.b = b; hd.rem = start - at;
+    for (;; b++) { const int w = work(b); if (start < at + w) break; at += w; }
+    hd.b = b; hd.rem = start - at; hd.s = seq;
   }
   __syncthreads();
-  KfWalk use;
+  KfWalk<SH> use;
   use.b = hd.b;
-  use.s = kv_seq(c, rw, use.b, a.window, a.sinks, KF_SH);
+  use.s = hd.s;
   {
-    const int qts = (a.G * use.s.nc + 15) >> 4, u = (int)(hd.rem / use.s.chunks);
-    use.g = u / qts; use.qt = u % qts; use.c0 = (int)(hd.rem % use.s.chunks);
+    const int qts = (a.G * use.s.nc + 15) >> 4, u = hd.rem / use.s.chunks;
+    use.g = u / qts; use.qt = u % qts; use.c0 = hd.rem % use.s.chunks;
     use.left = min(per, all - start);
     use.take();
   }
   bool dead = false;
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!dead && !mbar_wait(bar, parity)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
-  };
+  const int bs = min(c.page_sh, SH), bmask = (1 << bs) - 1;   // log2 of a box's slots: a page's part of a group
   if (warp == CW) {
-    // ---- the chunks, one behind the other, over the ends of units; the pages of 32 chunks are asked for at once, and those of the next 32 while these are requested ----
-    int st = 0;
+    // ---- the queries and the groups, over the ends of units.  The pages of 32 boxes are asked for at once, those of the next 32 while these are requested ----
+    const int boxes = 1 << (SH - bs), gb = 5 - (SH - bs), pm = (1 << c.page_sh) - 1;   // of a group; log2 of the groups that 32 boxes are
+    int st = 0, sp = 0;
     uint32_t round = 0;
-    const int pm = (1 << c.page_sh) - 1;
     do {
-      const bool seen = use.s.e0 + use.s.nc > 0;           // (or the unit's rows see nothing)
-      auto pages = [&](int ch) {
-        int id = -1;
-        if (seen && ch + lane < use.c1)
-          asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(id) : "l"(c.table + (size_t)use.b * c.tstride + (kv_chunk_slot(use.s, ch + lane, KF_SH) >> c.page_sh)));
-        return id;
+      const int last = use.s.e0 + use.s.nc - 1;
+      struct Entry { int id; bool on; };                   // on: some row sees some of it
+      auto pages = [&](int ch) {                           // of box lane % boxes of group ch + lane / boxes
+        Entry x = {-1, false};
+        const int k = ch + (lane >> (SH - bs)), j = kv_chunk_slot(use.s, k, SH) + ((lane & (boxes - 1)) << bs);
+        x.on = k < use.c1 && j <= last && (!a.window || j + bmask > use.s.e0 - a.window || j < a.sinks);
+        if (x.on) asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(x.id) : "l"(c.table + (size_t)use.b * c.tstride + (j >> c.page_sh)));
+        return x;
       };
-      int next = pages(use.c0);
+      Entry next = pages(use.c0);
+      // the unit's queries, a lane each; rows behind the last one stay what they are: their results go nowhere
+      const int qb = sp & 1, q0 = 16 * use.qt, nq = min(16, a.G * use.s.nc - q0);
+      if (sp >= 2 && !dead && !mbar_wait(qempty(qb), (uint32_t)((sp >> 1) - 1) & 1u)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
+      dead = __any_sync(0xffffffffu, dead);
+      if (lane == 0) { if (dead) mbar_arrive(qfull(qb)); else kv_expect(qfull(qb), nq * HD * 2); }
+      __syncwarp();
+      if (lane < nq && !dead) {
+        const int qi = q0 + lane, row = kv_row_of(a, qi);
+        kv_bulk(q_s + (qb * 16 + lane) * QR, a.q + (long long)(use.s.first + row) * a.qs + (long long)(use.g * a.G + qi - row * a.G) * HD, HD * 2, qfull(qb));
+      }
+      sp++;
 #pragma unroll 1
-      for (int c0 = use.c0; c0 < use.c1; c0 += 32) {
-        const int n = min(32, use.c1 - c0);
+      for (int c0 = use.c0; c0 < use.c1; c0 += 1 << gb) {
+        const int n = min(1 << gb, use.c1 - c0);
         __syncwarp();
-        hd.ids[lane] = next;
+        hd.ids[lane] = !next.on ? -2 : (unsigned)next.id < (unsigned)c.n_pages ? next.id : -1;   // -2: not wanted, -1: no page
         __syncwarp();
-        next = pages(c0 + 32);
+        next = pages(c0 + (1 << gb));
         if (lane == 0) {                                   // one thread: a warp that walks together takes three times as long a request
 #pragma unroll 1
           for (int k = 0; k < n; k++) {
-            const int id = hd.ids[k], slot = kv_chunk_slot(use.s, c0 + k, KF_SH) & pm;
-            const uint32_t full = bar_s + 8 * st;
-            if (round && !dead && !mbar_wait(full + 256, (round - 1) & 1u)) { dead = true; atomicExch(p.err, 1u); }
-            const bool in = (unsigned)id < (unsigned)c.n_pages && !dead;
-            hd.bad[st] = !in;
-            if (in) {
-              kv_expect(full, SB);
-              kv_tma(ring_s + st * SB, &km, 0, slot, 0, use.g, id, full);
-              kv_tma(ring_s + st * SB + KB, &vm, 0, slot, 0, use.g, id, full);
-            } else {
-              if (seen && !dead) atomicOr(c.err, KV_ERR_PAGE);
-              mbar_arrive(full);
+            const int slot = kv_chunk_slot(use.s, c0 + k, SH) & pm;
+            if (round && !dead && !mbar_wait(empty(st), (round - 1) & 1u)) { dead = true; atomicExch(p.err, 1u); }
+            uint32_t bad = 0;
+            int have = 0;
+#pragma unroll 1
+            for (int x = 0; x < boxes; x++) {
+              const int id = hd.ids[(k << (SH - bs)) + x];
+              if (id >= 0) have++;
+              else if (id == -1) bad |= ((1u << (1 << (bs - 4))) - 1) << (x << (bs - 4));
             }
-            if (++st == NS) { st = 0; round++; }
+            if (bad) atomicOr(c.err, KV_ERR_PAGE);
+            hd.bad[st] = bad;
+            if (have && !dead) {
+              kv_expect(full(st), (uint32_t)have * (2 * HD * 2 << bs));
+#pragma unroll 1
+              for (int x = 0; x < boxes; x++) {
+                const int id = hd.ids[(k << (SH - bs)) + x];
+                if (id < 0) continue;
+                kv_tma(ring_s + st * SB + x * (HD * 2 << bs), &km, 0, slot, 0, use.g, id, full(st));
+                kv_tma(ring_s + st * SB + KB + x * (HD * 2 << bs), &vm, 0, slot, 0, use.g, id, full(st));
+              }
+            } else mbar_arrive(full(st));
+            if (++st == NG) { st = 0; round++; }
           }
         }
-        __syncwarp();
+        st = __shfl_sync(0xffffffffu, st, 0); round = __shfl_sync(0xffffffffu, round, 0); dead = __any_sync(0xffffffffu, dead);
       }
     } while (use.next(c, rw, a));
     if (dead) for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies may be on their way
     return;
   }
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!dead && !mbar_wait(bar, parity)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
+  };
   auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory"); };   // the warps that compute
-  int n0 = 0;                                              // chunks of the stretch before this unit's
+  int n0 = 0, sp = 0;                                      // groups of the stretch before this unit's, units before it
 #pragma unroll 1
   for (;;) {
     const KvSeq &s = use.s;
     const int NQ = a.G * s.nc, q0 = 16 * use.qt, last = s.e0 + s.nc - 1;
-    for (int i = tid; i < 16 * TD; i += 32 * CW) {
-      const int qi = q0 + (i & 15), d = i >> 4, row = kv_row_of(a, qi);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (qi < NQ) v = __ldcg((const uint4 *)(a.q + (long long)(s.first + row) * a.qs + (long long)(use.g * a.G + qi - row * a.G) * HD + 8 * d));
-      *(uint4 *)(q_m + i * 16) = v;
-    }
-    meet();
+    const uint32_t qs = q_s + (sp & 1) * 16 * QR;
+    wait(qfull(sp & 1), (uint32_t)(sp >> 1) & 1u);
     float o[TD][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < TD; i++)
@@ -224,21 +255,23 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       lw[k] = a.window ? e[k] - a.window + 1 : 0;
     }
     const int ea = s.e0 + kv_row_of(a, q0), ez = s.e0 + kv_row_of(a, min(q0 + 15, NQ - 1));      // slots of the unit's first and last row
-    int skip = (warp - n0) % CW;
-    if (skip < 0) skip += CW;
+    const int m1 = (n0 + use.c1 - use.c0) * PG;
+    int m0 = n0 * PG;                                      // 16 slots number m of the stretch are warp m % CW's
+    m0 += (warp + CW - m0 % CW) % CW;
 #pragma unroll 1
-    for (int ch = use.c0 + skip; ch < use.c1; ch += CW) {
-      const int n = n0 + ch - use.c0, st = n % NS, slot = kv_chunk_slot(s, ch, KF_SH);
-      const uint32_t k_s = ring_s + st * SB, v_s = k_s + KB;
-      wait(bar_s + 8 * st, (uint32_t)(n / NS) & 1u);
-      const bool none = hd.bad[st] || dead;
+    for (int mm = m0; mm < m1; mm += CW) {
+      const int n = mm / PG, part = mm % PG, st = n % NG, slot = kv_chunk_slot(s, use.c0 + n - n0, SH) + 16 * part;
+      const uint32_t k_s = ring_s + st * SB + ((16 * part) >> bs) * (HD * 2 << bs) + ((16 * part) & bmask) * 128, v_s = k_s + KB, blk = 128u << bs;   // 64 dims of a box
+      wait(full(st), (uint32_t)(n / NG) & 1u);
+      // (nothing of it is seen, or it was not brought)
+      const bool none = (hd.bad[st] >> part & 1) || dead || slot > last || (a.window && slot + 15 <= s.e0 - a.window && slot >= a.sinks);
       float x[2][4];
       if (!none) {
         // slots that no row sees: their V is taken out, whatever it holds (0 times NaN is NaN)
         if (slot + 15 > last || (a.window && slot <= s.e0 - a.window && slot + 15 >= a.sinks)) {
-          for (int i = lane; i < KF_SLOTS * TD; i += 32) {
+          for (int i = lane; i < 16 * TD; i += 32) {
             const int r = i & 15;
-            if (!kv_any_sees(s, slot + r, a.window, a.sinks)) *(uint4 *)(smem + (v_s - bar_s) + (i >> 7) * (KF_SLOTS * 128) + r * 128 + ((i >> 4) & 7) * 16) = make_uint4(0, 0, 0, 0);
+            if (!kv_any_sees(s, slot + r, a.window, a.sinks)) *(uint4 *)(smem + (v_s - bar_s) + (i >> 7) * blk + r * 128 + ((i >> 4) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
@@ -250,9 +283,9 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
         for (int ks = 0; ks < HD / 16; ks++) {
           uint32_t qa[4], kb[4];
           // queries: matrix mi has queries 8 (mi & 1) .., dims 8 (2 ks + mi / 2) ..; keys: slots 8 (mi / 2) .., dims 8 (2 ks + (mi & 1)) ..
-          kf_ldsm(qa, q_s + (2 * ks + (mi >> 1)) * 256 + (lr + 8 * (mi & 1)) * 16);
+          kf_ldsm(qa, qs + (lr + 8 * (mi & 1)) * QR + (2 * ks + (mi >> 1)) * 16);
           const int unit = 2 * ks + (mi & 1), row = lr + 8 * (mi >> 1);
-          kf_ldsm(kb, k_s + (unit >> 3) * (KF_SLOTS * 128) + row * 128 + (((unit & 7) ^ lr) << 4));
+          kf_ldsm(kb, k_s + (unit >> 3) * blk + row * 128 + (((unit & 7) ^ lr) << 4));
           kf_mma<T>(y[ks & 1][0], qa, kb[0], kb[1]);
           kf_mma<T>(y[ks & 1][1], qa, kb[2], kb[3]);
         }
@@ -272,7 +305,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       if constexpr (WT) {
 #pragma unroll
         for (int w = 0; w < 2; w++)
-          if (q0 + gid + 8 * w < NQ) {
+          if (q0 + gid + 8 * w < NQ && slot <= last) {
             float *d = p.sc + (((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + gid + 8 * w) * p.sstride + slot + j2;
             *(float2 *)d = make_float2(x[0][2 * w], x[0][2 * w + 1]);
             *(float2 *)(d + 8) = make_float2(x[1][2 * w], x[1][2 * w + 1]);
@@ -302,22 +335,24 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
         for (int i = 0; i < TD; i += 2) {
           uint32_t vb[4];                                  // matrix mi: slots 8 (mi & 1) .., dims 8 (i + mi / 2) ..
           const int unit = i + (mi >> 1), row = lr + 8 * (mi & 1);
-          kf_ldsm_t(vb, v_s + (unit >> 3) * (KF_SLOTS * 128) + row * 128 + (((unit & 7) ^ lr) << 4));
+          kf_ldsm_t(vb, v_s + (unit >> 3) * blk + row * 128 + (((unit & 7) ^ lr) << 4));
           kf_mma<T>(o[i], pa, vb[0], vb[1]);
           kf_mma<T>(o[i + 1], pa, vb[2], vb[3]);
         }
       }
-      __syncwarp();                                        // the chunk has been read
-      if (lane == 0) mbar_arrive(bar_s + 256 + 8 * st);
+      __syncwarp();                                        // the slots have been read
+      if (lane == 0) mbar_arrive(empty(st));
     }
     n0 += use.c1 - use.c0;
-    // ---- the warps' sums put together: everything relative to the largest maximum, then 32 dims at a time ----
+    sp++;
+    // ---- the warps' sums put together: everything relative to the largest maximum, then 32 dims at a time, or 64 or 128 where there are so few queries ----
 #pragma unroll
     for (int w = 0; w < 2; w++) {
       l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1); l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
       if (j2 == 0) { hd.m[warp][gid + 8 * w] = m[w]; hd.l[warp][gid + 8 * w] = l[w]; }
     }
     meet();
+    if (tid == 0) mbar_arrive(qempty((sp - 1) & 1));        // the queries have been read
 #pragma unroll
     for (int w = 0; w < 2; w++) {
       float M = -INFINITY, L = 0.0f;
@@ -339,27 +374,31 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       if (use.c1 == s.chunks) u[1] = blockIdx.x;
     }
     const size_t part = ((size_t)blockIdx.x * 2 + (use.c0 == 0)) * 16;
+    const int nr = min(16, NQ - q0), fold = HD == 64 ? (nr <= 8) : nr <= 4 ? 2 : nr <= 8, rows = 16 >> fold;   // 32 << fold dims at a time, of `rows` rows
 #pragma unroll
     for (int d0 = 0; d0 < HD; d0 += 32) {
-      float *d = sums + warp * 16 * KF_ROW;
+      const int at32 = (d0 >> 5) & ((1 << fold) - 1);      // which 32 of those dims
+      float *d = sums + (warp * 16 + at32 * rows) * KF_ROW;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        *(float2 *)(d + gid * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][0], o[d0 / 8 + i][1]);
-        *(float2 *)(d + (gid + 8) * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][2], o[d0 / 8 + i][3]);
+        if (gid < rows) *(float2 *)(d + gid * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][0], o[d0 / 8 + i][1]);
+        if (rows == 16) *(float2 *)(d + (gid + 8) * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][2], o[d0 / 8 + i][3]);
       }
+      if (at32 != (1 << fold) - 1) continue;
       meet();
+      const int first = d0 + 32 - (32 << fold);
 #pragma unroll 1
-      for (int it = tid; it < 256; it += 32 * CW) {        // a row, two dims of the 32
-        const int r = it >> 4, dd = 2 * (it & 15), qi = q0 + r;
-        if (qi >= NQ) break;
+      for (int it = tid; it < 256; it += 32 * CW) {        // a row, two dims
+        const int pos = it >> 4, r = pos & (rows - 1), dd = 2 * (it & 15), dim = first + 32 * (pos >> (4 - fold)) + dd, qi = q0 + r;
+        if (r >= nr) continue;
         float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < CW; k++) { const float2 t = *(const float2 *)(sums + (k * 16 + r) * KF_ROW + dd); v.x += t.x; v.y += t.y; }
-        if (!wholly) { *(float2 *)(p.po + (part + r) * HD + d0 + dd) = v; continue; }
+        for (int k = 0; k < CW; k++) { const float2 t = *(const float2 *)(sums + (k * 16 + pos) * KF_ROW + dd); v.x += t.x; v.y += t.y; }
+        if (!wholly) { *(float2 *)(p.po + (part + r) * HD + dim) = v; continue; }
         const int row = kv_row_of(a, qi), h = use.g * a.G + qi - row * a.G;
         const float L = hd.L[r], inv = L == 0.0f ? 0.0f : 1.0f / L;   // (nothing seen: zeros)
         if (!(fabsf(v.x) + fabsf(v.y) + L < INFINITY)) hd.odd[r] = 1;
-        const long long at = (long long)(s.first + row) * a.os + (long long)h * HD + d0 + dd;
+        const long long at = (long long)(s.first + row) * a.os + (long long)h * HD + dim;
         if (a.out32) *(float2 *)((float *)a.out + at) = make_float2(v.x * inv, v.y * inv);
         else *(uint32_t *)((uint16_t *)a.out + at) = KvEl<T>::of2(v.x * inv, v.y * inv);
       }
@@ -381,7 +420,6 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       if (lane == 0) hd.odd[k] = 0;
     }
     if (!use.next(c, rw, a)) break;
-    meet();                                                // (the queries' and sums' memory is free again)
   }
 }
 
@@ -400,7 +438,7 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
   if (!WT || blockIdx.x < joins) {
     const int qi = blockIdx.x % NQM, gb = blockIdx.x / NQM, g = gb % c.KV, b = gb / c.KV;
     const int2 w = __ldcg((const int2 *)p.unit + (size_t)gb * QTM + (qi >> 4));
-    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
+    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, kf_sh(HD));
     if (qi >= a.G * s.nc || w.x == w.y) return;
     float o[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -440,7 +478,7 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
   }
   if constexpr (WT) {
     const int u = blockIdx.x - joins, wb = u % wblocks, gb = u / wblocks, b = gb / c.KV;
-    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, KF_SH);
+    const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, kf_sh(HD));
     if (wb * 512 >= s.len) return;
     const int NQ = a.G * s.nc;
     const size_t ug = gb;

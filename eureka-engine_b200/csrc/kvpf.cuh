@@ -144,10 +144,10 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     }
   }
   const int bs = min(c.page_sh, SH), boxes = TILE >> bs;   // slots of a page's part of a tile, and how many parts
-  // a loading lane's entry of tile i's pages, asked for a tile before its use; -2: nothing that a row sees
+  // a loading lane's entry of tile i's pages, asked for a tile before its use; on: some row sees some of it
   struct Entry { int id; bool on; };
   auto entry = [&](int i) {
-    Entry x = {-2, false};
+    Entry x = {-1, false};
     if (lane < boxes && i < n) {
       const int j = slot_of(i) + (lane << bs);
       x.on = j <= ez && (!a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks);   // (what is seen is one run of slots and the first ones)
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     }
     return x;
   };
-  Entry first = {-2, false};
+  Entry first = {-1, false};
   if (warp == C::SOFT || warp == C::SOFT + 1) first = entry(0);
   if (tid == 0) {
     for (int i = 0; i < 12; i++) { mbar_init(full(i >= 6, i % 6), 1); mbar_init(empty(i >= 6, i % 6), streams); }
@@ -410,13 +410,13 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
 #pragma unroll 1
     for (int i = 0; i < n; i++) {
       asm volatile("" : "+r"(next.id));                    // (the load is not waited for before)
-      const int id = next.on ? next.id : -2;
+      const int id = !next.on ? -2 : (unsigned)next.id < (unsigned)c.n_pages ? next.id : -1;   // -2: not wanted, -1: no page
       next = entry(i + 1);
       if (round) wait(empty(isv, slot), (round - 1) & 1u);
       else if (HD == 256 && isv && slot == NV - 1) wait(q_full, 0);   // (the queries come through it)
       __syncwarp();
-      const bool in = (unsigned)id < (unsigned)c.n_pages;
-      const unsigned have = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, !in && id != -2);
+      const bool in = id >= 0;
+      const unsigned have = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, id == -1);
       const uint32_t bar = full(isv, slot), at = ring + slot * GB;
       const int j = slot_of(i) & ((1 << c.page_sh) - 1);   // (where a tile has several pages, the first slot of each)
       if (lane == 0) {

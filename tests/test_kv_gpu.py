@@ -279,11 +279,12 @@ def test_every_score_minus_infinity(llb):
     _check_attn(c, r)
 
 
+@pytest.mark.parametrize("bad", [None, -1, -2, -2 ** 31])
 @pytest.mark.parametrize("rows", [1, 80])
-def test_bad_pages_are_not_seen(llb, rows):
+def test_bad_pages_are_not_seen(llb, rows, bad):
     """An entry of a visible slot that is no page: its slots are left out, and the error word says so."""
     c = Cache(llb, "f16", 2, 64, 16, [150], seed=15)
-    c.table[0, 3] = c.n_pages
+    c.table[0, 3] = c.n_pages if bad is None else bad
     r = _attn(llb, c, 4, [rows], seed=16, weights=rows == 1)
     assert llb.kv_errors() == 1
     llb.lib().llb_b200_kv_errors_clear()
