@@ -383,7 +383,7 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   CUtensorMap km, vm;
   const int slots = std::min(kv->page, 1 << kf_sh(HD));
   if (pool_map(&km, kv, kv->k, slots, HD / 64) || pool_map(&vm, kv, kv->v, slots, HD / 64)) return -1;
-  const dim3 grid(few_grid()), block(32 * (kf_warps(HD) + 1));
+  const dim3 grid(few_grid()), block(32 * (kf_warps(HD) + 2));
   const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + 511) / 512;   // (attn_check: they fit)
   if (a.w_out) {
     CU_OK(llb_launch(k_kv_few<T, HD, true>, grid, block, (size_t)kf_smem(HD), g_llb.stream, c, rw, a, p, km, vm));

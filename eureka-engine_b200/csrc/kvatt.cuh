@@ -3,15 +3,15 @@
 // A unit is (sequence, kv head, 16 queries); its queries are the rows' heads side by side, query i G + h is row i, head h of the kv head's
 // G.  What a unit sees is cut into groups of 32 or 64 slots, and the groups of all units, one after the other, into as many equal stretches as
 // there are blocks, so that sequences of any lengths keep every SM busy to the end; a block's stretch may begin and end inside a unit.
-// A thread of the block requests the groups (TMA, a box a page, rows of 128 swizzled bytes) and every unit's queries, on over the ends of units; the other
-// warps take 16 slots of a group each.
+// Two threads of the block request the groups' K and V (TMA, a box a page, rows of 128 swizzled bytes) and every unit's queries, on over the ends of units;
+// the other warps take 16 slots of a group each.
 //   S[query][slot] = Q K^T      m16n8k16, 16 queries x 16 slots
 //   O[query][dim] += P V        P from the registers of S, rounded to the cache's type (the second product takes 16-bit operands)
 // with the maximum and the sum of every query kept in f32.  Where a unit ends the warps' sums are put together, some dims at a time.  A unit that one
 // block has wholly is finished there; the others' sums go to the workspace, and k_kv_join, the second launch, puts them together in the order of the blocks.
 //
 // 16 slots are a chain of 1500 to 2000 cycles for their warp (two products with the softmax between), which is why several warps work on slots of their own; a
-// request takes its thread 100 cycles a box whatever the box's size, 500 for 16 slots' K and V with all around them, which is why groups are 32 KB.
+// request takes its thread 100 to 200 cycles a box whatever the box's size, which is why groups are 32 KB and why K and V have a thread each.
 #pragma once
 #include <cuda.h>
 
@@ -24,12 +24,14 @@ __host__ __device__ constexpr int kf_warps(int HD) { return HD == 256 ? 6 : 8; }
 __host__ __device__ constexpr int kf_ring(int HD) { return HD == 64 ? 8 : 6; }                        // groups that have room
 __host__ __device__ constexpr int kf_bytes(int HD) { return 2 * HD * 2 << kf_sh(HD); }                // of a group: K, then V
 __host__ __device__ constexpr int kf_qrow(int HD) { return HD * 2 + 16; }                             // bytes from a query to the next: four banks on
+struct KfUnit { KvSeq s; int b, g, qt, c0, c1; };   // c0 .. c1 - 1: the block's groups of it; c1 < 0: no more
 #define KF_ROW 40              // floats from a row of the warps' sums to the next: 32 dims, and eight banks on
 struct KfHead {                // before the ring
   uint64_t full[8], empty[8], qfull[2], qempty[2];
-  int sum[16], b, rem;
+  int sum[16], b, rem, dead;
   KvSeq s;
-  int bad[8], odd[16], ids[32];   // bad: a bit for 16 slots of a group whose page is no page
+  KfUnit unit[2];              // what the queries that are there belong to
+  int bad[8], odd[16], ids[2][32];   // bad: a bit for 16 slots of a group whose page is no page
   float m[8][16], l[8][16], M[16], L[16];
 };
 #define KF_HEAD 2048
@@ -105,9 +107,9 @@ template <int SH> struct KfWalk {
 };
 
 template <typename T, int HD, bool WT>
-__global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
+__global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
                                                                       const __grid_constant__ CUtensorMap vm) {
-  constexpr int CW = kf_warps(HD), NT = 32 * (CW + 1), NG = kf_ring(HD), SB = kf_bytes(HD), KB = SB / 2, TD = HD / 8, SH = kf_sh(HD), PG = kf_parts(HD), QR = kf_qrow(HD);   // TD: tiles of eight dims
+  constexpr int CW = kf_warps(HD), NT = 32 * (CW + 2), NG = kf_ring(HD), SB = kf_bytes(HD), KB = SB / 2, TD = HD / 8, SH = kf_sh(HD), PG = kf_parts(HD), QR = kf_qrow(HD);   // TD: tiles of eight dims
   extern __shared__ __align__(1024) uint8_t smem[];
   KfHead &hd = *(KfHead *)smem;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, j2 = 2 * (lane & 3), lr = lane & 7, mi = lane >> 3;
@@ -117,10 +119,11 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
   auto empty = [&](int i) { return bar_s + 64u + 8u * (uint32_t)i; };
   auto qfull = [&](int i) { return bar_s + 128u + 8u * (uint32_t)i; };
   auto qempty = [&](int i) { return bar_s + 144u + 8u * (uint32_t)i; };
-  if (tid < 8) { mbar_init(full(tid), 1); mbar_init(empty(tid), PG); }
+  if (tid < 8) { mbar_init(full(tid), 2); mbar_init(empty(tid), PG); }
   if (tid < 2) { mbar_init(qfull(tid), 1); mbar_init(qempty(tid), 1); }
   if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   if (tid < 16) hd.odd[tid] = 0;
+  if (tid == 0) hd.dead = 0;
   pdl_trigger();
   pdl_wait();
   // ---- the block's stretch: groups of every sequence, summed over the threads' runs of sequences ----
@@ -140,7 +143,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
   __syncthreads();
   int all = 0;
 #pragma unroll
-  for (int w = 0; w <= CW; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
+  for (int w = 0; w < CW + 2; w++) { if (w < warp) to += hd.sum[w]; all += hd.sum[w]; }
   const int per = max(p.least, (all + (int)gridDim.x - 1) / (int)gridDim.x);
   if (blockIdx.x >= (all + per - 1) / per) return;
   const int start = per * blockIdx.x;
@@ -151,22 +154,41 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
     hd.b = b; hd.rem = start - at; hd.s = seq;
   }
   __syncthreads();
-  KfWalk<SH> use;
-  use.b = hd.b;
-  use.s = hd.s;
-  {
-    const int qts = (a.G * use.s.nc + 15) >> 4, u = hd.rem / use.s.chunks;
-    use.g = u / qts; use.qt = u % qts; use.c0 = hd.rem % use.s.chunks;
-    use.left = min(per, all - start);
-    use.take();
-  }
   bool dead = false;
   const int bs = min(c.page_sh, SH), bmask = (1 << bs) - 1;   // log2 of a box's slots: a page's part of a group
-  if (warp == CW) {
-    // ---- the queries and the groups, over the ends of units.  The pages of 32 boxes are asked for at once, those of the next 32 while these are requested ----
+  if (warp >= CW) {
+    // ---- K and the queries, or V, over the ends of units.  The pages of 32 boxes are asked for at once, those of the next 32 while these are requested ----
+    const bool isv = warp > CW;
+    const CUtensorMap *map = isv ? &vm : &km;
+    const uint32_t ring = ring_s + (isv ? KB : 0);
+    KfWalk<SH> use;
+    use.b = hd.b;
+    use.s = hd.s;
+    {
+      const int qts = (a.G * use.s.nc + 15) >> 4, u = hd.rem / use.s.chunks;
+      use.g = u / qts; use.qt = u % qts; use.c0 = hd.rem % use.s.chunks;
+      use.left = min(per, all - start);
+      use.take();
+    }
     const int boxes = 1 << (SH - bs), gb = 5 - (SH - bs), pm = (1 << c.page_sh) - 1;   // of a group; log2 of the groups that 32 boxes are
     int st = 0, sp = 0;
     uint32_t round = 0;
+    auto tell = [&](bool more) {                           // a unit, and its queries, a lane each; rows behind the last one stay what they are: their results go nowhere
+      const int qb = sp & 1, q0 = 16 * use.qt, nq = more ? min(16, a.G * use.s.nc - q0) : 0;
+      if (sp >= 2 && !dead && !mbar_wait(qempty(qb), (uint32_t)((sp >> 1) - 1) & 1u)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
+      dead = __any_sync(0xffffffffu, dead);
+      if (lane == 0) {
+        hd.unit[qb] = {use.s, use.b, use.g, use.qt, use.c0, more ? use.c1 : -1};
+        if (dead || !more) mbar_arrive(qfull(qb));
+        else kv_expect(qfull(qb), nq * HD * 2);
+      }
+      __syncwarp();
+      if (lane < nq && !dead) {
+        const int qi = q0 + lane, row = kv_row_of(a, qi);
+        kv_bulk(q_s + (qb * 16 + lane) * QR, a.q + (long long)(use.s.first + row) * a.qs + (long long)(use.g * a.G + qi - row * a.G) * HD, HD * 2, qfull(qb));
+      }
+      sp++;
+    };
     do {
       const int last = use.s.e0 + use.s.nc - 1;
       struct Entry { int id; bool on; };                   // on: some row sees some of it
@@ -178,22 +200,12 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
         return x;
       };
       Entry next = pages(use.c0);
-      // the unit's queries, a lane each; rows behind the last one stay what they are: their results go nowhere
-      const int qb = sp & 1, q0 = 16 * use.qt, nq = min(16, a.G * use.s.nc - q0);
-      if (sp >= 2 && !dead && !mbar_wait(qempty(qb), (uint32_t)((sp >> 1) - 1) & 1u)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
-      dead = __any_sync(0xffffffffu, dead);
-      if (lane == 0) { if (dead) mbar_arrive(qfull(qb)); else kv_expect(qfull(qb), nq * HD * 2); }
-      __syncwarp();
-      if (lane < nq && !dead) {
-        const int qi = q0 + lane, row = kv_row_of(a, qi);
-        kv_bulk(q_s + (qb * 16 + lane) * QR, a.q + (long long)(use.s.first + row) * a.qs + (long long)(use.g * a.G + qi - row * a.G) * HD, HD * 2, qfull(qb));
-      }
-      sp++;
+      if (!isv) tell(true);
 #pragma unroll 1
       for (int c0 = use.c0; c0 < use.c1; c0 += 1 << gb) {
         const int n = min(1 << gb, use.c1 - c0);
         __syncwarp();
-        hd.ids[lane] = !next.on ? -2 : (unsigned)next.id < (unsigned)c.n_pages ? next.id : -1;   // -2: not wanted, -1: no page
+        hd.ids[isv][lane] = !next.on ? -2 : (unsigned)next.id < (unsigned)c.n_pages ? next.id : -1;   // -2: not wanted, -1: no page
         __syncwarp();
         next = pages(c0 + (1 << gb));
         if (lane == 0) {                                   // one thread: a warp that walks together takes three times as long a request
@@ -205,20 +217,19 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
             int have = 0;
 #pragma unroll 1
             for (int x = 0; x < boxes; x++) {
-              const int id = hd.ids[(k << (SH - bs)) + x];
+              const int id = hd.ids[isv][(k << (SH - bs)) + x];
               if (id >= 0) have++;
               else if (id == -1) bad |= ((1u << (1 << (bs - 4))) - 1) << (x << (bs - 4));
             }
             if (bad) atomicOr(c.err, KV_ERR_PAGE);
-            hd.bad[st] = bad;
+            if (!isv) hd.bad[st] = bad;
             if (have && !dead) {
-              kv_expect(full(st), (uint32_t)have * (2 * HD * 2 << bs));
+              kv_expect(full(st), (uint32_t)have * (HD * 2 << bs));
 #pragma unroll 1
               for (int x = 0; x < boxes; x++) {
-                const int id = hd.ids[(k << (SH - bs)) + x];
+                const int id = hd.ids[isv][(k << (SH - bs)) + x];
                 if (id < 0) continue;
-                kv_tma(ring_s + st * SB + x * (HD * 2 << bs), &km, 0, slot, 0, use.g, id, full(st));
-                kv_tma(ring_s + st * SB + KB + x * (HD * 2 << bs), &vm, 0, slot, 0, use.g, id, full(st));
+                kv_tma(ring + st * SB + x * (HD * 2 << bs), map, 0, slot, 0, use.g, id, full(st));
               }
             } else mbar_arrive(full(st));
             if (++st == NG) { st = 0; round++; }
@@ -227,6 +238,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
         st = __shfl_sync(0xffffffffu, st, 0); round = __shfl_sync(0xffffffffu, round, 0); dead = __any_sync(0xffffffffu, dead);
       }
     } while (use.next(c, rw, a));
+    if (!isv) tell(false);
     if (dead) for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies may be on their way
     return;
   }
@@ -237,10 +249,14 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
   int n0 = 0, sp = 0;                                      // groups of the stretch before this unit's, units before it
 #pragma unroll 1
   for (;;) {
+    wait(qfull(sp & 1), (uint32_t)(sp >> 1) & 1u);
+    const KfUnit use = hd.unit[sp & 1];
+    if (dead) hd.dead = 1;
+    meet();                                                // (one warp's wait that ran out is every warp's end: they meet again and again)
+    if (use.c1 < 0 || hd.dead) break;
     const KvSeq &s = use.s;
     const int NQ = a.G * s.nc, q0 = 16 * use.qt, last = s.e0 + s.nc - 1;
     const uint32_t qs = q_s + (sp & 1) * 16 * QR;
-    wait(qfull(sp & 1), (uint32_t)(sp >> 1) & 1u);
     float o[TD][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < TD; i++)
@@ -419,7 +435,6 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 1), 1) k_kv_few(const KvD
       __syncwarp();
       if (lane == 0) hd.odd[k] = 0;
     }
-    if (!use.next(c, rw, a)) break;
   }
 }
 
