@@ -189,11 +189,19 @@ __device__ __forceinline__ uint32_t kv_key(float w) {
   const uint32_t u = __float_as_uint(w + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// Which slots stay: a block a kv head of a sequence.  The weight that the last one has, by four passes over the keys' bytes (counts in shared
-// memory), then the slots above it and the first of those that equal it, in order.
-template <int NT>
-__global__ void __launch_bounds__(NT) k_kv_pick(const KvDev c, const KvEvict e) {
-  __shared__ int hist[256], part[NT / 32][2], base[2], pick[2];
+// Which slots stay: a block a kv head of a sequence.  The weight that the last one has, by passes over the keys' digits (eleven, eleven and ten bits; counts in
+// shared memory, a warp's equal digits counted together: sums of probabilities have few exponents, and many are zero), then the slots above it and
+// the first of those that equal it, in order.  The keys are kept in shared memory where they have room, so that the weights are read once.
+#define KE_THREADS 1024
+#define KE_KEYS 49152          // most slots whose keys have room
+#define KE_SMEM (2048 * 4 + KE_KEYS * 4)
+template <bool ROOM>
+__global__ void __launch_bounds__(KE_THREADS) k_kv_pick(const KvDev c, const KvEvict e) {
+  constexpr int NT = KE_THREADS;
+  extern __shared__ __align__(16) int dyn[];
+  int *hist = dyn;
+  uint32_t *keys = (uint32_t *)(dyn + 2048);
+  __shared__ int part[32][2], pick[2];
   pdl_trigger();
   pdl_wait();
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -204,51 +212,98 @@ __global__ void __launch_bounds__(NT) k_kv_pick(const KvDev c, const KvEvict e) 
     for (int i = tid; i < len; i += NT) kept[i] = i;
     return;
   }
-  const float *w = e.w + ((size_t)b * c.KV + g) * e.wstride;
-  const int lo = e.sinks, hi = len - e.recent;
-  int want = e.budget - e.sinks - e.recent;    // of lo .. hi - 1, more than it
+  const int lo = e.sinks, hi = len - e.recent, n = hi - lo;
+  const float *w = e.w + ((size_t)b * c.KV + g) * e.wstride + lo;
+  int want = e.budget - e.sinks - e.recent;    // of the n, more than it
   for (int i = tid; i < lo; i += NT) kept[i] = i;
   for (int i = tid; i < e.recent; i += NT) kept[e.budget - e.recent + i] = hi + i;
   if (!want) return;
-  uint32_t key = 0;
-  for (int sh = 24; sh >= 0; sh -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  auto key_at = [&](int i) { return ROOM ? keys[i] : kv_key(__ldcg(w + i)); };
+  uint32_t key = 0, known = 0;                 // the digits so far, and which bits they are
+#pragma unroll 1
+  for (int pass = 0; pass < 3; pass++) {
+    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023 : 2047;
+    for (int i = tid; i < 2048; i += NT) hist[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += NT) {
-      const uint32_t u = kv_key(__ldcg(w + i));
-      if (sh == 24 || u >> (sh + 8) == key >> (sh + 8)) atomicAdd(hist + ((u >> sh) & 255), 1);
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 4 * NT) {
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int i = i0 + k * NT + tid;
+        u[k] = 0;
+        if (i < n) {
+          u[k] = ROOM && pass == 0 ? kv_key(__ldcg(w + i)) : key_at(i);
+          if (ROOM && pass == 0) keys[i] = u[k];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const bool on = i0 + k * NT + tid < n && (u[k] & known) == key;
+        const unsigned act = __ballot_sync(0xffffffffu, on);
+        if (on) {
+          const int d = (u[k] >> sh) & mask;
+          const unsigned same = __match_any_sync(act, d);
+          if (__ffs(same) - 1 == lane) atomicAdd(hist + d, __popc(same));
+        }
+      }
     }
     __syncthreads();
-    if (tid == 0) {
-      int left = want, d = 255;
-      while (hist[d] < left) left -= hist[d--];
-      pick[0] = d; pick[1] = left;
+    if (warp == 0) {                           // from the top: a lane 64 digits, then the lane's own
+      int s = 0;
+      const int d1 = 2047 - 64 * lane;         // the lane's: d1 down to d1 - 63
+#pragma unroll 8
+      for (int k = 0; k < 64; k++) s += hist[d1 - ((k + lane) & 63)];   // (a bank of its own for every lane)
+      int to = s;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) { const int o = __shfl_up_sync(0xffffffffu, to, m); if (lane >= m) to += o; }
+      const bool mine = to >= want && to - s < want;
+      const int who = __ffs(__ballot_sync(0xffffffffu, mine)) - 1, left0 = want - __shfl_sync(0xffffffffu, to - s, who), base = 2047 - 64 * who;
+      // the 64 digits of that lane, two a lane
+      const int a0 = hist[base - 2 * lane], a1 = hist[base - 2 * lane - 1], t2 = a0 + a1;
+      int up = t2;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) { const int o = __shfl_up_sync(0xffffffffu, up, m); if (lane >= m) up += o; }
+      if (up >= left0 && up - t2 < left0) {
+        const int left = left0 - (up - t2);
+        const bool first = a0 >= left;
+        pick[0] = base - 2 * lane - (first ? 0 : 1); pick[1] = first ? left : left - a0;
+      }
     }
     __syncthreads();
     key |= (uint32_t)pick[0] << sh;
+    known |= (uint32_t)mask << sh;
     want = pick[1];                            // of those that equal the key so far
   }
-  if (tid < 2) base[tid] = 0;
+  // a thread a run of slots (an odd number of them: banks), counted, then written
+  const int run = ((n + NT - 1) / NT) | 1, ra = min(n, tid * run), rz = min(n, ra + run);
+  int no = 0, ne = 0;
+#pragma unroll 4
+  for (int i = ra; i < rz; i++) { const uint32_t u = key_at(i); no += u > key; ne += u == key; }
+  int so = no, se = ne;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, so, m), q = __shfl_up_sync(0xffffffffu, se, m);
+    if (lane >= m) { so += o; se += q; }
+  }
+  if (lane == 31) { part[warp][0] = so; part[warp][1] = se; }
   __syncthreads();
-  for (int i0 = lo; i0 < hi; i0 += NT) {
-    const int i = i0 + tid;
-    const uint32_t u = i < hi ? kv_key(__ldcg(w + i)) : 0;
-    const bool over = i < hi && u > key, same = i < hi && u == key;
-    const unsigned mo = __ballot_sync(0xffffffffu, over), ms = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
-    if (lane == 0) { part[warp][0] = __popc(mo); part[warp][1] = __popc(ms); }
-    __syncthreads();
-    int no = base[0] + __popc(mo & below), ne = base[1] + __popc(ms & below), to = 0, te = 0;
-    for (int k = 0; k < NT / 32; k++) {
-      if (k < warp) { no += part[k][0]; ne += part[k][1]; }
-      to += part[k][0]; te += part[k][1];
-    }
-    if (over || (same && ne < want)) kept[lo + no + min(ne, want)] = i;
-    __syncthreads();
-    if (tid == 0) { base[0] += to; base[1] += te; }
-    __syncthreads();
+  so -= no; se -= ne;
+  {
+    int po = lane < warp ? part[lane][0] : 0, pe = lane < warp ? part[lane][1] : 0;   // of the warps before
+#pragma unroll
+    for (int m = 16; m; m >>= 1) { po += __shfl_xor_sync(0xffffffffu, po, m); pe += __shfl_xor_sync(0xffffffffu, pe, m); }
+    so += po; se += pe;
+  }
+#pragma unroll 1
+  for (int i = ra; i < rz; i++) {
+    const uint32_t u = key_at(i);
+    if (u > key) { kept[lo + so + min(se, want)] = lo + i; so++; }
+    else if (u == key) { if (se < want) kept[lo + so + se] = lo + i; se++; }
   }
 }
-// K, V and weights of the kept slots into their new pages: 16 bytes a thread
+// K, V and weights of the kept slots into their new pages: 16 bytes a thread, KM_FLY of K and of V in flight
+#define KM_FLY 4
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, const KvEvict e) {
   pdl_trigger();
@@ -256,14 +311,34 @@ __global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, c
   constexpr int P = HD / 8;    // pieces of a row
   const int g = blockIdx.y, b = blockIdx.z, now = min(kv_len(c, b), e.budget);
   const int *kept = e.kept + ((size_t)b * c.KV + g) * e.kept_stride;
-  for (int u = blockIdx.x * 256 + threadIdx.x; u < now * P; u += gridDim.x * 256) {
-    const int i = u / P, p = u % P, j = __ldcg(kept + i);
-    if (p == 0 && e.w_out) e.w_out[((size_t)b * c.KV + g) * e.w_out_stride + i] = __ldcg(e.w + ((size_t)b * c.KV + g) * e.wstride + j);
-    const int from = kv_page(c, b, j >> c.page_sh), to = kv_page(d, b, i >> d.page_sh);
-    if (from < 0 || to < 0) continue;
-    const size_t x = kv_at(c, from, g, HD) + (size_t)(j & ((1 << c.page_sh) - 1)) * HD + 8 * p, y = kv_at(d, to, g, HD) + (size_t)(i & ((1 << d.page_sh) - 1)) * HD + 8 * p;
-    *(uint4 *)(d.k + y) = __ldcg((const uint4 *)(c.k + x));
-    *(uint4 *)(d.v + y) = __ldcg((const uint4 *)(c.v + x));
+  for (int u0 = blockIdx.x * 256 * KM_FLY + threadIdx.x; u0 < now * P; u0 += gridDim.x * 256 * KM_FLY) {
+    int j[KM_FLY], from[KM_FLY], to[KM_FLY];
+    uint4 k[KM_FLY], v[KM_FLY];
+#pragma unroll
+    for (int f = 0; f < KM_FLY; f++) { const int u = u0 + 256 * f; j[f] = u < now * P ? __ldcg(kept + u / P) : -1; }
+#pragma unroll
+    for (int f = 0; f < KM_FLY; f++) {
+      const int i = (u0 + 256 * f) / P;
+      from[f] = to[f] = -1;
+      if (j[f] >= 0) { from[f] = kv_page(c, b, j[f] >> c.page_sh); to[f] = kv_page(d, b, i >> d.page_sh); }
+    }
+#pragma unroll
+    for (int f = 0; f < KM_FLY; f++) {
+      const int p = (u0 + 256 * f) % P;
+      if (from[f] < 0 || to[f] < 0) continue;
+      const size_t x = kv_at(c, from[f], g, HD) + (size_t)(j[f] & ((1 << c.page_sh) - 1)) * HD + 8 * p;
+      k[f] = __ldcs((const uint4 *)(c.k + x));
+      v[f] = __ldcs((const uint4 *)(c.v + x));
+    }
+#pragma unroll
+    for (int f = 0; f < KM_FLY; f++) {
+      const int u = u0 + 256 * f, i = u / P, p = u % P;
+      if (j[f] >= 0 && p == 0 && e.w_out) e.w_out[((size_t)b * c.KV + g) * e.w_out_stride + i] = __ldcg(e.w + ((size_t)b * c.KV + g) * e.wstride + j[f]);
+      if (from[f] < 0 || to[f] < 0) continue;
+      const size_t y = kv_at(d, to[f], g, HD) + (size_t)(i & ((1 << d.page_sh) - 1)) * HD + 8 * p;
+      *(uint4 *)(d.k + y) = k[f];
+      *(uint4 *)(d.v + y) = v[f];
+    }
   }
 }
 
@@ -275,6 +350,7 @@ template <typename T, int HD> static int few_attr() {
   return 0;
 }
 int kv_setup(void) {
+  CU_OK(cudaFuncSetAttribute(k_kv_pick<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, KE_SMEM));
   if (few_attr<__half, 64>() || few_attr<__half, 128>() || few_attr<__half, 256>() || few_attr<__nv_bfloat16, 64>() || few_attr<__nv_bfloat16, 128>() || few_attr<__nv_bfloat16, 256>()) return -1;
   if (!g_kv_map) {
     cudaDriverEntryPointQueryResult found;
@@ -565,9 +641,14 @@ int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *
   k.w_out = (float *)(uintptr_t)e->w_out; k.w_out_stride = e->w_out_stride;
   k.kept = (int *)(uintptr_t)(e->kept ? e->kept : e->ws); k.kept_stride = e->kept ? e->kept_stride : most;
   k.dst_lens = (int *)(uintptr_t)dst->lens;
-  CU_OK(llb_launch(k_kv_pick<1024>, dim3(c.KV, c.seqs), dim3(1024), (size_t)0, g_llb.stream, c, k));
+  // (keys of up to max_len slots; a block with few of them leaves room for others on its SM)
+  const dim3 heads(c.KV, c.seqs);
+  if (e->max_len <= KE_KEYS) CU_OK(llb_launch(k_kv_pick<true>, heads, dim3(KE_THREADS), (size_t)(2048 + std::max(e->max_len, 1)) * 4, g_llb.stream, c, k));
+  else CU_OK(llb_launch(k_kv_pick<false>, heads, dim3(KE_THREADS), (size_t)2048 * 4, g_llb.stream, c, k));
   if (!most) return 0;
-  const dim3 grid(std::max(1, std::min(256, most * (src->head_dim / 8) / 1024)), c.KV, c.seqs);
+  // blocks of a head: one trip of its pieces each, as long as there are not more blocks than eight an SM
+  const long long pieces = (long long)most * (src->head_dim / 8), room = std::max(1LL, 8LL * g_llb.sms / ((long long)c.KV * c.seqs));
+  const dim3 grid((unsigned)std::max(1LL, std::min(room, (pieces + 256 * KM_FLY - 1) / (256 * KM_FLY))), c.KV, c.seqs);
   if (src->head_dim == 64) CU_OK(llb_launch(k_kv_move<64>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
   else if (src->head_dim == 128) CU_OK(llb_launch(k_kv_move<128>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
   else CU_OK(llb_launch(k_kv_move<256>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));

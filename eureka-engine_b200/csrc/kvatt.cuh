@@ -24,7 +24,7 @@ __host__ __device__ constexpr int kf_warps(int HD) { return HD == 256 ? 6 : 8; }
 __host__ __device__ constexpr int kf_ring(int HD) { return HD == 64 ? 8 : 6; }                        // groups that have room
 __host__ __device__ constexpr int kf_bytes(int HD) { return 2 * HD * 2 << kf_sh(HD); }                // of a group: K, then V
 __host__ __device__ constexpr int kf_qrow(int HD) { return HD * 2 + 16; }                             // bytes from a query to the next: four banks on
-struct KfUnit { KvSeq s; int b, g, qt, c0, c1; };   // c0 .. c1 - 1: the block's groups of it; c1 < 0: no more
+struct KfUnit { KvSeq s; int b, g, qt, c0, c1, last; };   // c0 .. c1 - 1: the block's groups of it; c1 < 0: no more; last: the ring is empty behind it
 #define KF_ROW 40              // floats from a row of the warps' sums to the next: 32 dims, and eight banks on
 struct KfHead {                // before the ring
   uint64_t full[8], empty[8], qfull[2], qempty[2];
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       if (sp >= 2 && !dead && !mbar_wait(qempty(qb), (uint32_t)((sp >> 1) - 1) & 1u)) { dead = true; if (lane == 0) atomicExch(p.err, 1u); }
       dead = __any_sync(0xffffffffu, dead);
       if (lane == 0) {
-        hd.unit[qb] = {use.s, use.b, use.g, use.qt, use.c0, more ? use.c1 : -1};
+        hd.unit[qb] = {use.s, use.b, use.g, use.qt, use.c0, more ? use.c1 : -1, use.left <= 0};
         if (dead || !more) mbar_arrive(qfull(qb));
         else kv_expect(qfull(qb), nq * HD * 2);
       }
@@ -390,35 +390,61 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       if (use.c1 == s.chunks) u[1] = blockIdx.x;
     }
     const size_t part = ((size_t)blockIdx.x * 2 + (use.c0 == 0)) * 16;
-    const int nr = min(16, NQ - q0), fold = HD == 64 ? (nr <= 8) : nr <= 4 ? 2 : nr <= 8, rows = 16 >> fold;   // 32 << fold dims at a time, of `rows` rows
+    const int nr = min(16, NQ - q0);
+    auto result = [&](int r, int dim, float2 v) {          // two dims of a query
+      if (!wholly) { *(float2 *)(p.po + (part + r) * HD + dim) = v; return; }
+      const int qi = q0 + r, row = kv_row_of(a, qi), h = use.g * a.G + qi - row * a.G;
+      const float L = hd.L[r], inv = L == 0.0f ? 0.0f : 1.0f / L;   // (nothing seen: zeros)
+      if (!(fabsf(v.x) + fabsf(v.y) + L < INFINITY)) hd.odd[r] = 1;
+      const long long at = (long long)(s.first + row) * a.os + (long long)h * HD + dim;
+      if (a.out32) *(float2 *)((float *)a.out + at) = make_float2(v.x * inv, v.y * inv);
+      else *(uint32_t *)((uint16_t *)a.out + at) = KvEl<T>::of2(v.x * inv, v.y * inv);
+    };
+    if (use.last) {
+      // nothing is brought any more: all dims at once, in the ring's memory
+      constexpr int RW = HD + 8;
+      static_assert(CW * 16 * RW * 4 <= NG * SB, "the ring's memory");
+      float *all_ = (float *)(smem + KF_HEAD), *d = all_ + warp * 16 * RW;
 #pragma unroll
-    for (int d0 = 0; d0 < HD; d0 += 32) {
-      const int at32 = (d0 >> 5) & ((1 << fold) - 1);      // which 32 of those dims
-      float *d = sums + (warp * 16 + at32 * rows) * KF_ROW;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (gid < rows) *(float2 *)(d + gid * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][0], o[d0 / 8 + i][1]);
-        if (rows == 16) *(float2 *)(d + (gid + 8) * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][2], o[d0 / 8 + i][3]);
+      for (int i = 0; i < TD; i++) {
+        if (gid < nr) *(float2 *)(d + gid * RW + 8 * i + j2) = make_float2(o[i][0], o[i][1]);
+        if (gid + 8 < nr) *(float2 *)(d + (gid + 8) * RW + 8 * i + j2) = make_float2(o[i][2], o[i][3]);
       }
-      if (at32 != (1 << fold) - 1) continue;
       meet();
-      const int first = d0 + 32 - (32 << fold);
-#pragma unroll 1
-      for (int it = tid; it < 256; it += 32 * CW) {        // a row, two dims
-        const int pos = it >> 4, r = pos & (rows - 1), dd = 2 * (it & 15), dim = first + 32 * (pos >> (4 - fold)) + dd, qi = q0 + r;
-        if (r >= nr) continue;
+#pragma unroll 2
+      for (int it = tid; it < nr * (HD / 2); it += 32 * CW) {
+        const int r = it / (HD / 2), dim = 2 * (it % (HD / 2));
         float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < CW; k++) { const float2 t = *(const float2 *)(sums + (k * 16 + pos) * KF_ROW + dd); v.x += t.x; v.y += t.y; }
-        if (!wholly) { *(float2 *)(p.po + (part + r) * HD + dim) = v; continue; }
-        const int row = kv_row_of(a, qi), h = use.g * a.G + qi - row * a.G;
-        const float L = hd.L[r], inv = L == 0.0f ? 0.0f : 1.0f / L;   // (nothing seen: zeros)
-        if (!(fabsf(v.x) + fabsf(v.y) + L < INFINITY)) hd.odd[r] = 1;
-        const long long at = (long long)(s.first + row) * a.os + (long long)h * HD + dim;
-        if (a.out32) *(float2 *)((float *)a.out + at) = make_float2(v.x * inv, v.y * inv);
-        else *(uint32_t *)((uint16_t *)a.out + at) = KvEl<T>::of2(v.x * inv, v.y * inv);
+        for (int k = 0; k < CW; k++) { const float2 t = *(const float2 *)(all_ + (k * 16 + r) * RW + dim); v.x += t.x; v.y += t.y; }
+        result(r, dim, v);
       }
       meet();
+    } else {
+      const int fold = HD == 64 ? (nr <= 8) : nr <= 4 ? 2 : nr <= 8, rows = 16 >> fold;   // 32 << fold dims at a time, of `rows` rows
+#pragma unroll
+      for (int d0 = 0; d0 < HD; d0 += 32) {
+        const int at32 = (d0 >> 5) & ((1 << fold) - 1);    // which 32 of those dims
+        float *d = sums + (warp * 16 + at32 * rows) * KF_ROW;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (gid < rows) *(float2 *)(d + gid * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][0], o[d0 / 8 + i][1]);
+          if (rows == 16) *(float2 *)(d + (gid + 8) * KF_ROW + 8 * i + j2) = make_float2(o[d0 / 8 + i][2], o[d0 / 8 + i][3]);
+        }
+        if (at32 != (1 << fold) - 1) continue;
+        meet();
+        const int first = d0 + 32 - (32 << fold);
+#pragma unroll 1
+        for (int it = tid; it < 256; it += 32 * CW) {      // a row, two dims
+          const int pos = it >> 4, r = pos & (rows - 1), dd = 2 * (it & 15);
+          if (r >= nr) continue;
+          float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int k = 0; k < CW; k++) { const float2 t = *(const float2 *)(sums + (k * 16 + pos) * KF_ROW + dd); v.x += t.x; v.y += t.y; }
+          result(r, first + 32 * (pos >> (4 - fold)) + dd, v);
+        }
+        meet();
+      }
     }
     if (tid < 16 && q0 + tid < NQ) {
       if (!wholly) { p.pm[part + tid] = hd.M[tid]; p.pl[part + tid] = hd.L[tid]; }
@@ -497,6 +523,21 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
     if (wb * 512 >= s.len) return;
     const int NQ = a.G * s.nc;
     const size_t ug = gb;
+    // the slots' first scores, asked for before the queries' sums are there
+    float sum[4] = {0.f, 0.f, 0.f, 0.f}, in[4] = {0.f, 0.f, 0.f, 0.f}, sc[8][4];
+    const float *x = p.sc + ug * NQM * p.sstride + wb * 512 + tid;
+    bool on[4], see[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int j = wb * 512 + k * 128 + tid;
+      on[k] = j < s.len; see[k] = on[k] && NQ && kv_any_sees(s, j, a.window, a.sinks);
+      if (on[k] && a.w_in) in[k] = __ldcg(a.w_in + ug * a.wstride + j);
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        sc[q][k] = -INFINITY;
+        if (see[k] && q < NQ) asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(sc[q][k]) : "l"(x + (size_t)q * p.sstride + k * 128));
+      }
+    }
     if (tid < NQ) {
       const int2 w = __ldcg((const int2 *)p.unit + ug * QTM + (tid >> 4));
       if (w.x == w.y) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
@@ -511,20 +552,16 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
       }
     }
     __syncthreads();
-    float sum[4] = {0.f, 0.f, 0.f, 0.f}, in[4] = {0.f, 0.f, 0.f, 0.f};
-    const float *x = p.sc + ug * NQM * p.sstride + wb * 512 + tid;
-    bool on[4], see[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int j = wb * 512 + k * 128 + tid;
-      on[k] = j < s.len; see[k] = on[k] && kv_any_sees(s, j, a.window, a.sinks);
-      if (on[k] && a.w_in) in[k] = __ldcg(a.w_in + ug * a.wstride + j);
-    }
+    for (int q = 0; q < 8; q++)
+      if (q < NQ)
+#pragma unroll
+        for (int k = 0; k < 4; k++) sum[k] += kv_exp2(sc[q][k] - lse[q]);
 #pragma unroll 4
-    for (int q = 0; q < NQ; q++)
+    for (int q = 8; q < NQ; q++)
 #pragma unroll
       for (int k = 0; k < 4; k++)
-        if (see[k]) sum[k] += kv_exp2(__ldcs(x + (size_t)q * p.sstride + k * 128) - lse[q]);
+        if (see[k]) sum[k] += kv_exp2(__ldcg(x + (size_t)q * p.sstride + k * 128) - lse[q]);
 #pragma unroll
     for (int k = 0; k < 4; k++)
       if (on[k]) a.w_out[ug * a.wstride + wb * 512 + k * 128 + tid] = in[k] + sum[k];
