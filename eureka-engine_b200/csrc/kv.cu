@@ -190,7 +190,7 @@ __device__ __forceinline__ uint32_t kv_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 // Which slots stay: a block a kv head of a sequence.  The weight that the last one has, by passes over the keys' digits (eleven, eleven and ten bits; counts in
-// shared memory, a warp's equal digits counted together: sums of probabilities have few exponents, and many are zero), then the slots above it and
+// shared memory; a warp's zeros are counted together, and so are those that are like its first other weight: many are zero, or all alike), then the slots above it and
 // the first of those that equal it, in order.  The keys are kept in shared memory where they have room, so that the weights are read once.
 #define KE_THREADS 1024
 #define KE_KEYS 49152          // most slots whose keys have room
@@ -240,12 +240,15 @@ __global__ void __launch_bounds__(KE_THREADS) k_kv_pick(const KvDev c, const KvE
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const bool on = i0 + k * NT + tid < n && (u[k] & known) == key;
-        const unsigned act = __ballot_sync(0xffffffffu, on);
-        if (on) {
-          const int d = (u[k] >> sh) & mask;
-          const unsigned same = __match_any_sync(act, d);
-          if (__ffs(same) - 1 == lane) atomicAdd(hist + d, __popc(same));
-        }
+        const bool zero = on && u[k] == 0x80000000u;
+        const int d = (u[k] >> sh) & mask;
+        const unsigned zeros = __ballot_sync(0xffffffffu, zero), act = __ballot_sync(0xffffffffu, on && !zero);
+        if (zeros && lane == 0) atomicAdd(hist + ((0x80000000u >> sh) & mask), __popc(zeros));
+        if (!act) continue;
+        const int d0 = __shfl_sync(0xffffffffu, d, __ffs(act) - 1);
+        const unsigned same = __ballot_sync(0xffffffffu, on && !zero && d == d0);
+        if (lane == __ffs(act) - 1) atomicAdd(hist + d0, __popc(same));
+        else if (on && !zero && d != d0) atomicAdd(hist + d, 1);
       }
     }
     __syncthreads();
@@ -460,7 +463,7 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   const int slots = std::min(kv->page, 1 << kf_sh(HD));
   if (pool_map(&km, kv, kv->k, slots, HD / 64) || pool_map(&vm, kv, kv->v, slots, HD / 64)) return -1;
   const dim3 grid(few_grid()), block(32 * (kf_warps(HD) + 2));
-  const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + 511) / 512;   // (attn_check: they fit)
+  const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + KJ_SLOTS - 1) / KJ_SLOTS;   // (attn_check: they fit)
   if (a.w_out) {
     CU_OK(llb_launch(k_kv_few<T, HD, true>, grid, block, (size_t)kf_smem(HD), g_llb.stream, c, rw, a, p, km, vm));
     CU_OK(llb_launch(k_kv_join<T, HD, true>, dim3(joins + wblocks * c.KV * c.seqs), dim3(128), (size_t)0, g_llb.stream, c, rw, a, p, joins, wblocks));

@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
 __device__ __forceinline__ size_t kf_part(int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }
 
 // Units that several blocks had: a block a query, its four warps the parts in turn, each with what it needs of them asked for at once.  Blocks from
-// `joins` on: what every slot got, 512 slots of a kv head each.
+// `joins` on: what every slot got, KJ_SLOTS of a kv head each.
+#define KJ_SLOTS 2048
 template <typename T, int HD, bool WT>
 __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
   constexpr int E = HD / 32;
@@ -520,24 +521,27 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
   if constexpr (WT) {
     const int u = blockIdx.x - joins, wb = u % wblocks, gb = u / wblocks, b = gb / c.KV;
     const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, kf_sh(HD));
-    if (wb * 512 >= s.len) return;
+    if (wb * KJ_SLOTS >= s.len) return;
     const int NQ = a.G * s.nc;
     const size_t ug = gb;
-    // the slots' first scores, asked for before the queries' sums are there
-    float sum[4] = {0.f, 0.f, 0.f, 0.f}, in[4] = {0.f, 0.f, 0.f, 0.f}, sc[8][4];
-    const float *x = p.sc + ug * NQM * p.sstride + wb * 512 + tid;
+    // four slots a thread, and the first eight queries' scores of them at once; the first slots' before the queries' sums are there
+    float in[4], sc[8][4];
     bool on[4], see[4];
+    auto ask = [&](int j0) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int j = wb * 512 + k * 128 + tid;
-      on[k] = j < s.len; see[k] = on[k] && NQ && kv_any_sees(s, j, a.window, a.sinks);
-      if (on[k] && a.w_in) in[k] = __ldcg(a.w_in + ug * a.wstride + j);
+      for (int k = 0; k < 4; k++) {
+        const int j = j0 + k * 128 + tid;
+        on[k] = j < s.len; see[k] = on[k] && NQ && kv_any_sees(s, j, a.window, a.sinks);
+        in[k] = 0.0f;
+        if (on[k] && a.w_in) asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(in[k]) : "l"(a.w_in + ug * a.wstride + j));
 #pragma unroll
-      for (int q = 0; q < 8; q++) {
-        sc[q][k] = -INFINITY;
-        if (see[k] && q < NQ) asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(sc[q][k]) : "l"(x + (size_t)q * p.sstride + k * 128));
+        for (int q = 0; q < 8; q++) {
+          sc[q][k] = -INFINITY;
+          if (see[k] && q < NQ) asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(sc[q][k]) : "l"(p.sc + (ug * NQM + q) * p.sstride + j));
+        }
       }
-    }
+    };
+    ask(wb * KJ_SLOTS);
     if (tid < NQ) {
       const int2 w = __ldcg((const int2 *)p.unit + ug * QTM + (tid >> 4));
       if (w.x == w.y) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
@@ -552,18 +556,25 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
       }
     }
     __syncthreads();
+#pragma unroll 1
+    for (int j0 = wb * KJ_SLOTS;; ) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < 8; q++)
-      if (q < NQ)
+      for (int q = 0; q < 8; q++)
+        if (q < NQ)
 #pragma unroll
-        for (int k = 0; k < 4; k++) sum[k] += kv_exp2(sc[q][k] - lse[q]);
+          for (int k = 0; k < 4; k++) sum[k] += kv_exp2(sc[q][k] - lse[q]);
 #pragma unroll 4
-    for (int q = 8; q < NQ; q++)
+      for (int q = 8; q < NQ; q++)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (see[k]) sum[k] += kv_exp2(__ldcg(p.sc + (ug * NQM + q) * p.sstride + j0 + k * 128 + tid) - lse[q]);
 #pragma unroll
       for (int k = 0; k < 4; k++)
-        if (see[k]) sum[k] += kv_exp2(__ldcg(x + (size_t)q * p.sstride + k * 128) - lse[q]);
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (on[k]) a.w_out[ug * a.wstride + wb * 512 + k * 128 + tid] = in[k] + sum[k];
+        if (on[k]) a.w_out[ug * a.wstride + j0 + k * 128 + tid] = in[k] + sum[k];
+      j0 += 512;
+      if (j0 >= min(s.len, (wb + 1) * KJ_SLOTS)) break;
+      ask(j0);
+    }
   }
 }
