@@ -346,15 +346,21 @@ __global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, c
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-template <typename T, int HD> static int few_attr() {
-  CU_OK(cudaFuncSetAttribute(k_kv_few<T, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kf_smem(HD)));
-  CU_OK(cudaFuncSetAttribute(k_kv_pf<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kp<HD>::SMEM));
-  CU_OK(cudaFuncSetAttribute(k_kv_few<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kf_smem(HD)));
+// Every kernel is loaded here: one that is first met while a stream is being captured may not be.
+template <typename K> static int kv_load(K k, int smem = 0) {
+  if (smem) CU_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaFuncAttributes at;
+  CU_OK(cudaFuncGetAttributes(&at, k));
   return 0;
 }
+template <typename T, typename X, int HD> static int load_append() { return kv_load(k_kv_append<T, X, HD, false>) || kv_load(k_kv_append<T, X, HD, true>); }
+template <typename T, int HD> static int load_of() {
+  return kv_load(k_kv_few<T, HD, false>, kf_smem(HD)) || kv_load(k_kv_few<T, HD, true>, kf_smem(HD)) || kv_load(k_kv_join<T, HD, false>) || kv_load(k_kv_join<T, HD, true>) ||
+         kv_load(k_kv_pf<T, HD>, Kp<HD>::SMEM) || kv_load(k_kv_pf_join<T, HD>) || load_append<T, float, HD>() || load_append<T, __half, HD>() || load_append<T, __nv_bfloat16, HD>();
+}
+template <int HD> static int load_hd() { return load_of<__half, HD>() || load_of<__nv_bfloat16, HD>() || kv_load(k_kv_move<HD>); }
 int kv_setup(void) {
-  CU_OK(cudaFuncSetAttribute(k_kv_pick<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, KE_SMEM));
-  if (few_attr<__half, 64>() || few_attr<__half, 128>() || few_attr<__half, 256>() || few_attr<__nv_bfloat16, 64>() || few_attr<__nv_bfloat16, 128>() || few_attr<__nv_bfloat16, 256>()) return -1;
+  if (load_hd<64>() || load_hd<128>() || load_hd<256>() || kv_load(k_kv_pick<true>, KE_SMEM) || kv_load(k_kv_pick<false>)) return -1;
   if (!g_kv_map) {
     cudaDriverEntryPointQueryResult found;
     CU_OK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", (void **)&g_kv_map, 12000, cudaEnableDefault, &found));
@@ -516,6 +522,7 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   if (a->el_out != LLB_EL_F32 && a->el_out != kv->el) return llb_fail("kv_attn: el_out %d (f32 or the cache's type)", a->el_out);
   const long long row = (long long)a->heads * kv->head_dim;
   if ((a->rows && (!a->q || !a->out)) || off(a->q, 16) || off(a->out, 16)) return llb_fail("kv_attn: q and out lie on multiples of 16 bytes");
+  if (a->rows && a->q == a->out) return llb_fail("kv_attn: out is q");
   if (a->q_stride < row || a->q_stride % 8) return llb_fail("kv_attn: q_stride %lld for rows of %lld", a->q_stride, row);
   if (a->out_stride < row || a->out_stride % (a->el_out == LLB_EL_F32 ? 4 : 8)) return llb_fail("kv_attn: out_stride %lld for rows of %lld", a->out_stride, row);
   if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");

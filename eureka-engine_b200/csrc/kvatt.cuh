@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
     }
     if (tid < 16 && q0 + tid < NQ) {
       if (!wholly) { p.pm[part + tid] = hd.M[tid]; p.pl[part + tid] = hd.L[tid]; }
-      else if (WT) p.lse[((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + tid] = hd.L[tid] > 0.0f ? hd.M[tid] + log2f(hd.L[tid]) : INFINITY;
+      else if (WT) p.lse[((size_t)use.b * c.KV + use.g) * (a.G * rw.max_rows) + q0 + tid] = hd.L[tid] == 0.0f ? INFINITY : hd.M[tid] + log2f(hd.L[tid]);
     }
     // rows whose result is no number once more, by themselves (kv_attn_row says why)
 #pragma unroll 1
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
         const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll 4
         for (int i = w.x; i <= w.y; i++) { const size_t at = kf_part(i, w.x) + (tid & 15); l += __ldcg(p.pl + at) * exp2f(__ldcg(p.pm + at) - ref); }
-        lse[tid] = l > 0.0f ? M + log2f(l) : INFINITY;
+        lse[tid] = l == 0.0f ? INFINITY : M + log2f(l);
       }
     }
     __syncthreads();

@@ -18,7 +18,7 @@ def _append(llb, **kw):
 
 
 def _attn(llb, **kw):
-    a = dict(rows=5, max_rows=2, max_len=500, heads=8, window=0, sinks=0, scale=0.0, el_out=llb.EL["bf16"], q=P, out=P, q_stride=1024, out_stride=1024, row_start=P,
+    a = dict(rows=5, max_rows=2, max_len=500, heads=8, window=0, sinks=0, scale=0.0, el_out=llb.EL["bf16"], q=P, out=2 * P, q_stride=1024, out_stride=1024, row_start=P,
              ws=P, ws_bytes=1 << 30)
     a.update(kw)
     return llb.KvAttn(**a)
@@ -66,7 +66,7 @@ def test_appends_that_are_refused(pkg, bad, word):
 @pytest.mark.parametrize("bad,word", [
     (dict(rows=-1), "-1 rows"), (dict(heads=6), "6 heads on 4"), (dict(heads=260), "260 heads"), (dict(max_rows=0), "max_rows 0"), (dict(max_len=-1), "max_len -1"),
     (dict(window=-1), "window -1"), (dict(window=8, sinks=-1), "sinks -1"), (dict(sinks=4), "without a window"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(el_out=1), "el_out 1"), (dict(q=0), "multiples of 16"), (dict(out=P + 8), "multiples of 16"), (dict(q_stride=1016), "q_stride 1016"),
+    (dict(scale=float("inf")), "scale"), (dict(el_out=1), "el_out 1"), (dict(q=0), "multiples of 16"), (dict(out=P), "out is q"), (dict(out=P + 8), "multiples of 16"), (dict(q_stride=1016), "q_stride 1016"),
     (dict(q_stride=1028), "q_stride 1028"), (dict(out_stride=1000), "out_stride 1000"), (dict(row_start=P + 2), "row_start"), (dict(w_in=P), "w_in without w_out"),
     (dict(w_out=P, w_stride=499), "w_stride 499"), (dict(w_out=P + 2, w_stride=500), "weights are f32"), (dict(w_out=P, w_stride=500, max_rows=33), "weights of 33 rows")])
 def test_attention_that_is_refused(pkg, bad, word):

@@ -247,6 +247,20 @@ def test_a_later_rows_infinities_do_not_reach_earlier_rows(llb, rows, H, KV, wha
     _check_attn(c, r)
 
 
+@pytest.mark.parametrize("H,KV", [(4, 1), (24, 4)])
+def test_weights_of_a_row_that_is_no_number(llb, H, KV):
+    """The last row's own key is no number: what its slots get is none either, what only the rows before it see is right, and so are other sequences."""
+    c = Cache(llb, "bf16", KV, 128, 16, [60, 70], seed=65)
+    c.k[int(c.table[0, 59 // 16]), 0, 59 % 16] = math.nan
+    r = _attn(llb, c, H, [1, 1], seed=66, weights=True)
+    w = r["w_out"]
+    assert torch.isnan(w[0, 0, :60]).all()
+    total = (w - r["w_in"]).double()
+    assert torch.all((total[1, :, :70].sum(-1) - H // KV).abs() < 1e-4)
+    if KV > 1:
+        assert torch.all((total[0, 1:, :60].sum(-1) - H // KV).abs() < 1e-4)
+
+
 def test_scores_of_minus_infinity_and_large_ones(llb):
     """Keys that overflow a score to minus infinity take no part; scores of thousands do not overflow."""
     c = Cache(llb, "bf16", 1, 128, 16, [200, 200], seed=13)
