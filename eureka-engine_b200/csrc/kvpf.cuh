@@ -88,7 +88,9 @@ __device__ __forceinline__ void kp_exp2_fma(f32x2 y, float &r0, float &r1) {
   r0 = __int_as_float(__float_as_int(a) + (__float_as_int(t0) << 23));
   r1 = __int_as_float(__float_as_int(b) + (__float_as_int(t1) << 23));
 }
+#ifndef KP_FMA_EVERY
 #define KP_FMA_EVERY 4         // every fourth pair of probabilities goes that way
+#endif
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p, int tiles, const __grid_constant__ CUtensorMap km,
@@ -107,12 +109,30 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   uint32_t *tmem_slot = (uint32_t *)(smem + 280);
   volatile uint32_t *dead = (volatile uint32_t *)(smem + 284);
   volatile uint32_t *badm = (volatile uint32_t *)(smem + 288);   // [tile & 15]: 16-slot groups whose page is no page
+  // (what needs nothing of the call: barriers, each of its own thread; a tile's places are given back by both streams)
+  if (tid < 12) { mbar_init(full(tid >= 6, tid % 6), 1); mbar_init(empty(tid >= 6, tid % 6), NQT); }
+  if (tid < 4) { mbar_init(s_full(tid >> 1, tid), 1); mbar_init(p_full(tid >> 1, tid), 4); }
+  if (tid < 2) mbar_init(pv_done(tid), 1);
+  if (tid == 0) { mbar_init(q_full, C::SOFT); *dead = 0; }
+  if (tid < 12) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
+  if (warp == C::SOFT + 2) {                     // tensor memory, while the others look their rows up
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  auto leave = [&]() {                           // nothing to do here
+    t5_fence_before();
+    __syncthreads();
+    if (warp == C::SOFT + 2) {
+      t5_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
+    }
+  };
   // ---- which unit: the last query tiles first, they see the most ----
   const int split = blockIdx.y, u = blockIdx.x, g = u % c.KV, b = u / c.KV % c.seqs, tile = tiles - 1 - u / c.KV / c.seqs;
   const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, SH);
   const int NQ = a.G * s.nc, q0 = tile * QT;
-  if (q0 >= NQ) return;
+  if (q0 >= NQ) { leave(); return; }
   const int ea = s.e0 + kv_row_of(a, q0), ez = s.e0 + kv_row_of(a, min(q0 + QT - 1, NQ - 1));   // slots of the first and the last row
   const KpTiles kt = kp_tiles<SH>(ea, ez, a.window, a.sinks);
   const int per = (kt.n + p.splits - 1) / p.splits, t0 = min(kt.n, split * per), n = min(kt.n, t0 + per) - t0;
@@ -125,6 +145,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       const long long at = (long long)(s.first + kv_row_of(a, qi)) * a.os + (long long)(g * a.G + qi - kv_row_of(a, qi) * a.G) * HD;
       for (int d = 0; d < HD * (a.out32 ? 4 : 2); d += 16) *(uint4 *)((uint8_t *)a.out + at * (a.out32 ? 4 : 2) + d) = make_uint4(0, 0, 0, 0);
     }
+    leave();
     return;
   }
   const int streams = NQT == 2 && q0 + 128 < NQ ? 2 : 1;
@@ -157,18 +178,6 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   };
   Entry first = {-1, false};
   if (warp == C::SOFT || warp == C::SOFT + 1) first = entry(0);
-  if (tid == 0) {
-    for (int i = 0; i < 12; i++) { mbar_init(full(i >= 6, i % 6), 1); mbar_init(empty(i >= 6, i % 6), streams); }
-    for (int x = 0; x < 4; x++) { mbar_init(s_full(x >> 1, x), 1); mbar_init(p_full(x >> 1, x), 4); }
-    mbar_init(pv_done(0), 1); mbar_init(pv_done(1), 1);
-    mbar_init(q_full, 4 * streams);
-    *dead = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == C::SOFT + 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   t5_fence_before();
   __syncthreads();
   t5_fence_after();
@@ -328,7 +337,8 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     __syncwarp();
     t5_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float chk[4] = {l, 0.0f, 0.0f, 0.0f};
+    const f32x2 inv2 = x2_pack(inv, inv), zero2 = x2_pack(0.0f, 0.0f);
+    f32x2 chk[2] = {x2_pack(l, 0.0f), zero2};
     if (p.splits > 1 && qi < NQ) { const size_t part = part_of(qi); p.pm[part] = m; p.pl[part] = l; }
     // whole 128-byte pieces of rows, turned in memory that no product reads any more: the stream's queries', or the rings where it is the only stream
     const bool wide = p.splits > 1 || a.out32;             // 32 dims a piece, or 64
@@ -366,7 +376,11 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       t5_wait_ld();
       if (p.splits == 1) {
 #pragma unroll
-        for (int k = 0; k < 64; k++) { chk[k & 3] += o[k] * 0.0f; o[k] *= inv; }
+        for (int k = 0; k < 64; k += 2) {
+          const f32x2 w = x2_pack(o[k], o[k + 1]);
+          chk[(k >> 1) & 1] = x2_fma(w, zero2, chk[(k >> 1) & 1]);
+          x2_unpack(x2_mul(w, inv2), o[k], o[k + 1]);
+        }
       }
       if (wide) {
 #pragma unroll
@@ -388,7 +402,9 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       }
     }
     // rows whose result is no number once more, by themselves (kv_attn_row says why)
-    unsigned redo = __ballot_sync(0xffffffffu, p.splits == 1 && qi < NQ && !(fabsf((chk[0] + chk[1]) + (chk[2] + chk[3])) < INFINITY));
+    float c0, c1;
+    x2_unpack(x2_add(chk[0], chk[1]), c0, c1);
+    unsigned redo = __ballot_sync(0xffffffffu, p.splits == 1 && qi < NQ && !(fabsf(c0 + c1) < INFINITY));
     while (redo) {
       const int k = __ffs(redo) - 1, qk = q0 + 128 * x0 + 32 * (warp & 3) + k, rk = qk / a.G;
       redo &= redo - 1;
@@ -397,7 +413,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       kv_store<T, HD>(a, s.first + rk, g * a.G + qk % a.G, lane, o, lk);
     }
   } else if (warp < C::SOFT) {
-    // (the second query tile is behind the last query)
+    if (lane == 0) mbar_arrive(q_full);          // the second query tile is behind the last query
   } else if (warp < C::SOFT + 2) {
     // ---- K, or V: the pages' parts of a tile ----
     const bool isv = warp == C::SOFT + 1;
@@ -463,6 +479,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         }
         t5_commit(s_full(x, i));
         t5_commit(empty(false, ks));
+        if (streams < NQT) t5_commit(empty(false, ks));    // (for the stream that is not)
         if (++ks == NK) { ks = 0; kp ^= 1u; }
         return seen;
       };
@@ -483,6 +500,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(O, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
         t5_commit(pv_done(x));
         t5_commit(empty(true, vs));
+        if (streams < NQT) t5_commit(empty(true, vs));
         if (++vs == NV) { vs = 0; vp ^= 1u; }
         // what comes next is waited for while this product runs; the next scores go into the columns of the probabilities that it uses
         seen = false;
