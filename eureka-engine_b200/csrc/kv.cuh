@@ -106,8 +106,12 @@ struct KvSeq {
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvDev &c, const KvRows &r, int b, int window, int sinks, int sh) {
   KvSeq s;
-  s.n = kv_rows(c, r, b, s.first);
-  s.len = kv_len(c, b);
+  const int a = __ldcg(r.start + b), z = __ldcg(r.start + b + 1), n = __ldcg(c.lens + b);   // (all on their way before any is looked at)
+  s.first = a;
+  s.n = a >= 0 && z >= a && z <= r.rows ? z - a : 0;
+  s.len = min(max(n, 0), c.cap);
+  if (s.n != z - a || a < 0) atomicOr(c.err, KV_ERR_ROWS);
+  if (s.len != n) atomicOr(c.err, KV_ERR_LEN);
   s.nc = min(s.n, r.max_rows);
   if (s.n > r.max_rows) atomicOr(c.err, KV_ERR_ROWS);
   s.e0 = s.len - s.n;
