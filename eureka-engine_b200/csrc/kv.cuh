@@ -80,7 +80,6 @@ __device__ __forceinline__ void kv_check_rows(const KvDev &c, const KvRows &r) {
   }
 }
 // what the row at slot e sees
-__device__ __forceinline__ bool kv_sees(int j, int e, int window, int sinks) { return j <= e && (!window || j > e - window || j < sinks); }
 __device__ __forceinline__ int kv_first(int e, int window) { return window && e >= window ? e - window + 1 : 0; }   // first slot of its window
 
 // ---- a call's attention ----------------------------------------------------------------------------

@@ -14,6 +14,10 @@
 // Warps: softmax (4 a query tile), one that loads K, one that loads V, one a stream that issues its MMAs: an MMA is issued when the one before has
 // begun, so that a warp's time between two products (its waits, its commits) is the tensor core's too, unless the other stream's warp has
 // products in line.  Every wait is bounded.
+//
+// Measured, cycles of a step of 64 slots: at head dimension 256 about 1370, of which the products are 16 x 33 + 4 x 130; at 128 (two streams) about 1900, products 2 x (8 x 48 + 4 x 64):
+// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 124 us, 0.9 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
+// heads of 128 on 8: 153 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
 #pragma once
 #include "kvatt.cuh"
 
@@ -69,28 +73,6 @@ __device__ __forceinline__ void kp_ld32(uint32_t taddr, float *v) {
 }
 
 __device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }   // the n lowest bits
-
-// 2^y of two numbers by the FMA pipe (y <= 127): the whole part into the exponent, 2^f on [-1/2, 1/2] by the polynomial of degree four whose largest relative
-// error is smallest (2.7e-6 in f32; coefficients by Remez's exchange).  The special function unit takes a warp's 32 in eight cycles.
-__device__ __forceinline__ void kp_exp2_fma(f32x2 y, float &r0, float &r1) {
-  float a, b;
-  x2_unpack(y, a, b);
-  y = x2_pack(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const f32x2 big = x2_pack(12582912.0f, 12582912.0f), one = x2_pack(-1.0f, -1.0f);
-  const f32x2 t = x2_add(y, big), f = x2_add(y, x2_fma(t, one, big));      // (t's low bits: the whole part)
-  f32x2 v = x2_fma(x2_pack(0.009570102207362652f, 0.009570102207362652f), f, x2_pack(0.05591785907745361f, 0.05591785907745361f));
-  v = x2_fma(v, f, x2_pack(0.240247443318367f, 0.240247443318367f));
-  v = x2_fma(v, f, x2_pack(0.6931217908859253f, 0.6931217908859253f));
-  v = x2_fma(v, f, x2_pack(0.9999992847442627f, 0.9999992847442627f));
-  float t0, t1;
-  x2_unpack(t, t0, t1);
-  x2_unpack(v, a, b);
-  r0 = __int_as_float(__float_as_int(a) + (__float_as_int(t0) << 23));
-  r1 = __int_as_float(__float_as_int(b) + (__float_as_int(t1) << 23));
-}
-#ifndef KP_FMA_EVERY
-#define KP_FMA_EVERY 4         // every fourth pair of probabilities goes that way
-#endif
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p, int tiles, const __grid_constant__ CUtensorMap km,
@@ -296,8 +278,9 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         for (int k = 0; k < 32; k++) {
           float y0, y1;
           const f32x2 y = x2_fma(x2_pack(v[k0 + 2 * k], v[k0 + 2 * k + 1]), sc2, rf2);
-          if (k % KP_FMA_EVERY == KP_FMA_EVERY - 1) kp_exp2_fma(y, y0, y1);
-          else { x2_unpack(y, y0, y1); y0 = kv_exp2(y0); y1 = kv_exp2(y1); }
+          x2_unpack(y, y0, y1);
+          y0 = kv_exp2(y0);
+          y1 = kv_exp2(y1);
           sum[k & 1] = x2_add(sum[k & 1], x2_pack(y0, y1));
           w[k] = KvEl<T>::of2(y0, y1);
         }

@@ -247,6 +247,37 @@ def test_a_later_rows_infinities_do_not_reach_earlier_rows(llb, rows, H, KV, wha
     _check_attn(c, r)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows,window", [(1, 0), (3, 0), (150, 0), (150, 100)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_key_that_is_no_number(llb, hd, rows, window, bad):
+    """One component of one key of every kv head, each at another place among eight slots: a row that sees a score of NaN or of plus infinity is
+    NaN, minus infinity takes no part, and the rows that do not see the slot are right.
+
+    Bounds: a score is off by |q| |K| hd 2^-23 / sqrt(hd) < 8e-4 at most here, a probability by four times that (its own and the sum's) and its rounding
+    to bf16, 2^-8: less than 2^-7 together; then the result's own rounding."""
+    n, KV, G = 190, 8, 2
+    c = Cache(llb, "bf16", KV, hd, 16, [n], seed=71)
+    at = [n - 75 + g for g in range(KV)] if rows > 75 else [n - 75 - g for g in range(KV)]
+    for g, j in enumerate(at):
+        c.k[int(c.table[0, j // 16]), g, j % 16, 5 * g] = bad
+        c.K[0][j, g, 5 * g] = bad
+    r = _attn(llb, c, KV * G, [rows], window=window, seed=72)
+    _clean(llb)
+    out = r["out"][:rows].double().cpu().view(rows, KV, G, hd)
+    for i in range(rows):
+        e = n - rows + i
+        a0 = max(0, e - window + 1) if window else 0
+        q = r["q"][i].double().cpu().view(KV, G, hd)
+        x = torch.einsum("kgd,jkd->kgj", q, c.K[0][a0:e + 1]) * r["scale"]
+        p = torch.softmax(x, -1)
+        V = c.V[0][a0:e + 1].permute(1, 0, 2)
+        want, size = torch.matmul(p, V), torch.matmul(p, V.abs())
+        assert torch.equal(torch.isnan(want), torch.isnan(out[i])), i
+        d = (out[i] - want).abs().nan_to_num(0.0)
+        assert torch.all(d <= (size * 2.0 ** -7 + want.abs() * 2.0 ** -8).nan_to_num(0.0) * 1.01 + 1e-30), i
+
+
 @pytest.mark.parametrize("H,KV", [(4, 1), (24, 4)])
 def test_weights_of_a_row_that_is_no_number(llb, H, KV):
     """The last row's own key is no number: what its slots get is none either, what only the rows before it see is right, and so are other sequences."""
