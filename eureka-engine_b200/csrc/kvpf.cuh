@@ -17,7 +17,7 @@
 //
 // Measured, cycles of a step of 64 slots: at head dimension 256 about 1370, of which the products are 16 x 33 + 4 x 130; at 128 (two streams) about 1900, products 2 x (8 x 48 + 4 x 64):
 // there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 124 us, 0.9 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
-// heads of 128 on 8: 153 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
+// heads of 128 on 8: 147 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
 #pragma once
 #include "kvatt.cuh"
 
@@ -73,6 +73,31 @@ __device__ __forceinline__ void kp_ld32(uint32_t taddr, float *v) {
 }
 
 __device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }   // the n lowest bits
+
+// 2^y of two numbers by the FMA pipe (y <= 127): the whole part makes a power of two, 2^f on [-1/2, 1/2] is the polynomial of degree four whose largest relative
+// error is smallest (2.7e-6 in f32; coefficients by Remez's exchange).  NaN stays NaN through the clamp, the polynomial and the last product.  The special
+// function unit takes a warp's 32 in eight cycles; where two streams' softmax warps share one, every fourth pair goes this way: 4 x up to
+// 2000 rows, window 1024, 32 heads of 128 on 8 take 147 us at pages of 32 and 144 at 64, with none 153.5 and 153; at pages of 16, where copies bound it, 160 and 154.
+// Every second pair is slower than every fourth, and one stream (head dimension 256) gains nothing.
+__device__ __forceinline__ float kp_max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void kp_exp2_fma(f32x2 y, float &r0, float &r1) {
+  float a, b;
+  x2_unpack(y, a, b);
+  y = x2_pack(kp_max_nan(a, -126.0f), kp_max_nan(b, -126.0f));
+  const f32x2 big = x2_pack(12582912.0f, 12582912.0f), one = x2_pack(-1.0f, -1.0f);
+  const f32x2 t = x2_add(y, big), f = x2_add(y, x2_fma(t, one, big));      // (t's low bits: the whole part)
+  f32x2 v = x2_fma(x2_pack(0.009570102207362652f, 0.009570102207362652f), f, x2_pack(0.05591785907745361f, 0.05591785907745361f));
+  v = x2_fma(v, f, x2_pack(0.240247443318367f, 0.240247443318367f));
+  v = x2_fma(v, f, x2_pack(0.6931217908859253f, 0.6931217908859253f));
+  v = x2_fma(v, f, x2_pack(0.9999992847442627f, 0.9999992847442627f));
+  x2_unpack(t, a, b);
+  const f32x2 e = x2_pack(__int_as_float((__float_as_int(a) << 23) + 0x3f800000), __int_as_float((__float_as_int(b) << 23) + 0x3f800000));
+  x2_unpack(x2_mul(v, e), r0, r1);
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, const KvRows rw, const KvAttn a, const KvPfPlan p, int tiles, const __grid_constant__ CUtensorMap km,
@@ -278,9 +303,8 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         for (int k = 0; k < 32; k++) {
           float y0, y1;
           const f32x2 y = x2_fma(x2_pack(v[k0 + 2 * k], v[k0 + 2 * k + 1]), sc2, rf2);
-          x2_unpack(y, y0, y1);
-          y0 = kv_exp2(y0);
-          y1 = kv_exp2(y1);
+          if (NQT == 2 && k % 4 == 3) kp_exp2_fma(y, y0, y1);
+          else { x2_unpack(y, y0, y1); y0 = kv_exp2(y0); y1 = kv_exp2(y1); }
           sum[k & 1] = x2_add(sum[k & 1], x2_pack(y0, y1));
           w[k] = KvEl<T>::of2(y0, y1);
         }
