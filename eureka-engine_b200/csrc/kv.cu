@@ -190,43 +190,60 @@ __device__ __forceinline__ uint32_t kv_key(float w) {
   const uint32_t u = __float_as_uint(w + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// Which slots stay: a block a kv head of a sequence.  The weight that the last one has, by passes over the keys' digits (eleven, eleven and ten bits; counts in
-// shared memory; a warp's zeros are counted together, and so are those that are like its first other weight: many are zero, or all alike), then the slots above it and
-// the first of those that equal it, in order.  The keys are kept in shared memory where they have room, so that the weights are read once.
-// 64 such blocks, up to 20000 slots each: 36 us.
+// Which slots stay: CL blocks, a cluster, a kv head of a sequence, each with its run of the slots.  The weight that the last one has, by passes over the keys' digits
+// (eleven, eleven and ten bits; counts in shared memory, summed over the cluster; a warp's zeros are counted together, and so are those that are like its first other
+// weight: many are zero, or all alike), then the slots above it and the first of those that equal it, in order.  The keys are kept in shared memory where they have
+// room, so that the weights are read once. A cluster of four against one block, with the
+// copies: 4 sequences of up to 60000 slots, 4 heads of 256, 54 us and 158; 16 of 20000 119 and 126; 16 of 8000 45 and 40, so that shorter ones take one block.
 #define KE_THREADS 1024
-#define KE_KEYS 49152          // most slots whose keys have room
-#define KE_SMEM (2048 * 4 + KE_KEYS * 4)
-template <bool ROOM>
-__global__ void __launch_bounds__(KE_THREADS) k_kv_pick(const KvDev c, const KvEvict e) {
+#define KE_CLUSTER 4           // blocks of a head where sequences may have more than
+#define KE_LONG 12288          // slots
+#define KE_KEYS 49152          // most slots of a block whose keys have room
+#define KE_HIST (4 * 2048)     // words: the passes' counts, and their sum over the cluster
+#define KE_SMEM ((KE_HIST + KE_KEYS) * 4)
+template <bool ROOM, int CL>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(KE_THREADS, 2) k_kv_pick(const KvDev c, const KvEvict e) {
   constexpr int NT = KE_THREADS;
   extern __shared__ __align__(16) int dyn[];
-  int *hist = dyn;
-  uint32_t *keys = (uint32_t *)(dyn + 2048);
-  __shared__ int part[32][2], pick[2];
+  uint32_t *keys = (uint32_t *)(dyn + KE_HIST);
+  __shared__ int part[32][2], pick[2], total[2];
   pdl_trigger();
   pdl_wait();
-  const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = blockIdx.x / CL, rank = blockIdx.x % CL, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = kv_len(c, b), now = min(len, e.budget);
   int *kept = e.kept + ((size_t)b * c.KV + g) * e.kept_stride;
-  if (g == 0 && tid == 0) e.dst_lens[b] = now;
+  if (g == 0 && rank == 0 && tid == 0) e.dst_lens[b] = now;
   if (len <= e.budget) {
-    for (int i = tid; i < len; i += NT) kept[i] = i;
+    for (int i = rank * NT + tid; i < len; i += CL * NT) kept[i] = i;
     return;
   }
-  const int lo = e.sinks, hi = len - e.recent, n = hi - lo;
+  int lo = e.sinks;
+  const int hi = len - e.recent, all = hi - lo;
+  int want = e.budget - e.sinks - e.recent;    // of them, more than it
+  for (int i = rank * NT + tid; i < lo; i += CL * NT) kept[i] = i;
+  for (int i = rank * NT + tid; i < e.recent; i += CL * NT) kept[e.budget - e.recent + i] = hi + i;
+  if (!want) return;                           // (as the return before: the whole cluster)
+  // from word `at` of this block's shared memory to the same of block r's
+  auto of_rank = [&](const int *at, int r) {
+    int v;
+    asm volatile("{.reg .u32 a; mapa.shared::cluster.u32 a, %1, %2; ld.shared::cluster.s32 %0, [a];}" : "=r"(v) : "r"(smem_u32(at)), "r"(r) : "memory");
+    return v;
+  };
+  auto meet = [&]() {
+    if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    else __syncthreads();
+  };
+  const int each = (all + CL - 1) / CL, n = max(0, min(each, all - rank * each)), first = lo;   // the block's: n from `lo` on
+  lo += rank * each;
   const float *w = e.w + ((size_t)b * c.KV + g) * e.wstride + lo;
-  int want = e.budget - e.sinks - e.recent;    // of the n, more than it
-  for (int i = tid; i < lo; i += NT) kept[i] = i;
-  for (int i = tid; i < e.recent; i += NT) kept[e.budget - e.recent + i] = hi + i;
-  if (!want) return;
+  for (int i = tid; i < 3 * 2048; i += NT) dyn[i] = 0;
+  __syncthreads();
   auto key_at = [&](int i) { return ROOM ? keys[i] : kv_key(__ldcg(w + i)); };
   uint32_t key = 0, known = 0;                 // the digits so far, and which bits they are
 #pragma unroll 1
   for (int pass = 0; pass < 3; pass++) {
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023 : 2047;
-    for (int i = tid; i < 2048; i += NT) hist[i] = 0;
-    __syncthreads();
+    int *hist = dyn + 2048 * pass;
 #pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 4 * NT) {
       uint32_t u[4];
@@ -253,7 +270,17 @@ __global__ void __launch_bounds__(KE_THREADS) k_kv_pick(const KvDev c, const KvE
         else if (on && !zero && d != d0) atomicAdd(hist + d, 1);
       }
     }
-    __syncthreads();
+    meet();
+    if constexpr (CL > 1) {
+      for (int i = tid; i < 2048; i += NT) {
+        int t = 0;
+#pragma unroll
+        for (int r = 0; r < CL; r++) t += of_rank(hist + i, r);
+        dyn[3 * 2048 + i] = t;
+      }
+      hist = dyn + 3 * 2048;
+      __syncthreads();
+    }
     if (warp == 0) {                           // from the top: a lane 64 digits, then the lane's own
       int s = 0;
       const int d1 = 2047 - 64 * lane;         // the lane's: d1 down to d1 - 63
@@ -300,51 +327,38 @@ __global__ void __launch_bounds__(KE_THREADS) k_kv_pick(const KvDev c, const KvE
     for (int m = 16; m; m >>= 1) { po += __shfl_xor_sync(0xffffffffu, po, m); pe += __shfl_xor_sync(0xffffffffu, pe, m); }
     so += po; se += pe;
   }
+  if constexpr (CL > 1) {                      // of the blocks before
+    if (tid == NT - 1) { total[0] = so + no; total[1] = se + ne; }
+    meet();
+    for (int r = 0; r < rank; r++) { so += of_rank(total, r); se += of_rank(total + 1, r); }
+    meet();                                    // (nobody's memory goes before it was read)
+  }
 #pragma unroll 1
   for (int i = ra; i < rz; i++) {
     const uint32_t u = key_at(i);
-    if (u > key) { kept[lo + so + min(se, want)] = lo + i; so++; }
-    else if (u == key) { if (se < want) kept[lo + so + se] = lo + i; se++; }
+    if (u > key) { kept[first + so + min(se, want)] = lo + i; so++; }
+    else if (u == key) { if (se < want) kept[first + so + se] = lo + i; se++; }
   }
 }
-// K, V and weights of the kept slots into their new pages: 16 bytes a thread, KM_FLY of K and of V in flight.  4096 slots of 4 heads of 256, 16 sequences: 113 us, 4.7 TB/s
-// read and written.
-#define KM_FLY 4
+// K, V and weights of the kept slots into their new pages: 16 bytes of K and of V a thread.  A thread's way is a chain of three trips (which slot, its page, its
+// row), so that many threads with one piece each keep more on its way than few with several: 16 sequences of 4096 slots, 4 heads of 256, take 119 us with the picking
+// at one piece and six blocks an SM, 5 us more at two and five, 30 at four and three.
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv_move(const KvDev c, const KvDev d, const KvEvict e) {
+__global__ void __launch_bounds__(256, 6) k_kv_move(const KvDev c, const KvDev d, const KvEvict e) {
   pdl_trigger();
   pdl_wait();
   constexpr int P = HD / 8;    // pieces of a row
   const int g = blockIdx.y, b = blockIdx.z, now = min(kv_len(c, b), e.budget);
-  const int *kept = e.kept + ((size_t)b * c.KV + g) * e.kept_stride;
-  for (int u0 = blockIdx.x * 256 * KM_FLY + threadIdx.x; u0 < now * P; u0 += gridDim.x * 256 * KM_FLY) {
-    int j[KM_FLY], from[KM_FLY], to[KM_FLY];
-    uint4 k[KM_FLY], v[KM_FLY];
-#pragma unroll
-    for (int f = 0; f < KM_FLY; f++) { const int u = u0 + 256 * f; j[f] = u < now * P ? __ldcg(kept + u / P) : -1; }
-#pragma unroll
-    for (int f = 0; f < KM_FLY; f++) {
-      const int i = (u0 + 256 * f) / P;
-      from[f] = to[f] = -1;
-      if (j[f] >= 0) { from[f] = kv_page(c, b, j[f] >> c.page_sh); to[f] = kv_page(d, b, i >> d.page_sh); }
-    }
-#pragma unroll
-    for (int f = 0; f < KM_FLY; f++) {
-      const int p = (u0 + 256 * f) % P;
-      if (from[f] < 0 || to[f] < 0) continue;
-      const size_t x = kv_at(c, from[f], g, HD) + (size_t)(j[f] & ((1 << c.page_sh) - 1)) * HD + 8 * p;
-      k[f] = __ldcs((const uint4 *)(c.k + x));
-      v[f] = __ldcs((const uint4 *)(c.v + x));
-    }
-#pragma unroll
-    for (int f = 0; f < KM_FLY; f++) {
-      const int u = u0 + 256 * f, i = u / P, p = u % P;
-      if (j[f] >= 0 && p == 0 && e.w_out) e.w_out[((size_t)b * c.KV + g) * e.w_out_stride + i] = __ldcg(e.w + ((size_t)b * c.KV + g) * e.wstride + j[f]);
-      if (from[f] < 0 || to[f] < 0) continue;
-      const size_t y = kv_at(d, to[f], g, HD) + (size_t)(i & ((1 << d.page_sh) - 1)) * HD + 8 * p;
-      *(uint4 *)(d.k + y) = k[f];
-      *(uint4 *)(d.v + y) = v[f];
-    }
+  const size_t head = (size_t)b * c.KV + g;
+  for (int u = blockIdx.x * 256 + threadIdx.x; u < now * P; u += gridDim.x * 256) {
+    const int i = u / P, p = u % P, j = __ldcg(e.kept + head * e.kept_stride + i);
+    const int from = kv_page(c, b, j >> c.page_sh), to = kv_page(d, b, i >> d.page_sh);
+    const bool on = from >= 0 && to >= 0;
+    const size_t x = kv_at(c, on ? from : 0, g, HD) + (size_t)(j & ((1 << c.page_sh) - 1)) * HD + 8 * p, y = kv_at(d, on ? to : 0, g, HD) + (size_t)(i & ((1 << d.page_sh) - 1)) * HD + 8 * p;
+    uint4 k = {}, v = {};
+    if (on) { k = __ldcs((const uint4 *)(c.k + x)); v = __ldcs((const uint4 *)(c.v + x)); }
+    if (p == 0 && e.w_out) e.w_out[head * e.w_out_stride + i] = __ldcg(e.w + head * e.wstride + j);
+    if (on) { *(uint4 *)(d.k + y) = k; *(uint4 *)(d.v + y) = v; }
   }
 }
 
@@ -362,8 +376,9 @@ template <typename T, int HD> static int load_of() {
          kv_load(k_kv_pf<T, HD>, Kp<HD>::SMEM) || kv_load(k_kv_pf_join<T, HD>) || load_append<T, float, HD>() || load_append<T, __half, HD>() || load_append<T, __nv_bfloat16, HD>();
 }
 template <int HD> static int load_hd() { return load_of<__half, HD>() || load_of<__nv_bfloat16, HD>() || kv_load(k_kv_move<HD>); }
+template <int CL> static int load_pick() { return kv_load(k_kv_pick<true, CL>, KE_SMEM) || kv_load(k_kv_pick<false, CL>); }
 int kv_setup(void) {
-  if (load_hd<64>() || load_hd<128>() || load_hd<256>() || kv_load(k_kv_pick<true>, KE_SMEM) || kv_load(k_kv_pick<false>)) return -1;
+  if (load_hd<64>() || load_hd<128>() || load_hd<256>() || load_pick<1>() || load_pick<KE_CLUSTER>()) return -1;
   if (!g_kv_map) {
     cudaDriverEntryPointQueryResult found;
     CU_OK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", (void **)&g_kv_map, 12000, cudaEnableDefault, &found));
@@ -654,14 +669,20 @@ int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *
   k.w_out = (float *)(uintptr_t)e->w_out; k.w_out_stride = e->w_out_stride;
   k.kept = (int *)(uintptr_t)(e->kept ? e->kept : e->ws); k.kept_stride = e->kept ? e->kept_stride : most;
   k.dst_lens = (int *)(uintptr_t)dst->lens;
-  // (keys of up to max_len slots; a block with few of them leaves room for others on its SM)
-  const dim3 heads(c.KV, c.seqs);
-  if (e->max_len <= KE_KEYS) CU_OK(llb_launch(k_kv_pick<true>, heads, dim3(KE_THREADS), (size_t)(2048 + std::max(e->max_len, 1)) * 4, g_llb.stream, c, k));
-  else CU_OK(llb_launch(k_kv_pick<false>, heads, dim3(KE_THREADS), (size_t)2048 * 4, g_llb.stream, c, k));
+  // (keys of a block's slots; a block with few of them leaves room for others on its SM)
+  auto pick = [&](auto cl) {
+    constexpr int CL = decltype(cl)::value;
+    const int own = std::max((e->max_len + CL - 1) / CL, 1);
+    const dim3 heads((unsigned)c.KV * CL, c.seqs);
+    if (own <= KE_KEYS) return llb_launch(k_kv_pick<true, CL>, heads, dim3(KE_THREADS), (size_t)(KE_HIST + own) * 4, g_llb.stream, c, k);
+    return llb_launch(k_kv_pick<false, CL>, heads, dim3(KE_THREADS), (size_t)KE_HIST * 4, g_llb.stream, c, k);
+  };
+  if (e->max_len > KE_LONG) CU_OK(pick(std::integral_constant<int, KE_CLUSTER>()));
+  else CU_OK(pick(std::integral_constant<int, 1>()));
   if (!most) return 0;
-  // blocks of a head: one trip of its pieces each, as long as there are not more blocks than eight an SM
-  const long long pieces = (long long)most * (src->head_dim / 8), room = std::max(1LL, 8LL * g_llb.sms / ((long long)c.KV * c.seqs));
-  const dim3 grid((unsigned)std::max(1LL, std::min(room, (pieces + 256 * KM_FLY - 1) / (256 * KM_FLY))), c.KV, c.seqs);
+  // blocks of a head: one trip each, as long as there are not more blocks than 64 an SM (eight: 6 % slower; one trip whatever the number: 7 %)
+  const long long pieces = (long long)most * (src->head_dim / 8), room = std::max(1LL, 64LL * g_llb.sms / ((long long)c.KV * c.seqs));
+  const dim3 grid((unsigned)std::max(1LL, std::min(room, (pieces + 255) / 256)), c.KV, c.seqs);
   if (src->head_dim == 64) CU_OK(llb_launch(k_kv_move<64>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
   else if (src->head_dim == 128) CU_OK(llb_launch(k_kv_move<128>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));
   else CU_OK(llb_launch(k_kv_move<256>, grid, dim3(256), (size_t)0, g_llb.stream, c, d, k));

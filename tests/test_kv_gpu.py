@@ -669,6 +669,26 @@ def test_evict_of_a_long_sequence(llb):
     _clean(llb)
 
 
+@pytest.mark.parametrize("budget,sinks,recent", [(9000, 16, 500), (19999, 19990, 7), (12999, 12997, 1), (1, 0, 0), (20000, 0, 0)])
+@pytest.mark.parametrize("kind", ["mixed", "equal", "zeros", "nan", "two"])
+def test_evict_of_long_sequences_goes_by_the_order(llb, budget, sinks, recent, kind):
+    """Equal weights stay in the order of their slots, also over the parts that several blocks have, of which some may have no slot to choose from."""
+    lens = [20001, 13000, 5000, 0, 1]
+    w = _weights(len(lens), 2, 20001, 73, ties=0.9 if kind == "mixed" else 0.3)
+    if kind == "equal":
+        w[:] = 0.25
+    elif kind == "zeros":
+        w[:, :, 100:] = 0.0
+        w[0, 0, 1::2] = -0.0
+    elif kind == "nan":
+        w[:, :, 7:19000] = math.nan
+    elif kind == "two":
+        w[:] = torch.where(torch.arange(20001, device="cuda") % 3 == 0, 1.5, 1.25)
+    c = Cache(llb, "f16", 2, 64, 64, lens, seed=74)
+    _evict(llb, c, budget, sinks, recent, w)
+    _clean(llb)
+
+
 def test_evict_reports_pages_and_lengths(llb):
     c = Cache(llb, "bf16", 2, 64, 16, [300], seed=49)
     w = _weights(1, 2, 300, 50, ties=0.0)
