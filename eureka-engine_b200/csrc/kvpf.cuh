@@ -16,8 +16,8 @@
 // products in line.  Every wait is bounded.
 //
 // Measured, cycles of a step of 64 slots: at head dimension 256 about 1370, of which the products are 16 x 33 + 4 x 130; at 128 (two streams) about 1900, products 2 x (8 x 48 + 4 x 64):
-// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 124 us, 0.9 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
-// heads of 128 on 8: 147 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
+// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 122 us, 0.91 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
+// heads of 128 on 8: 152 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
 #pragma once
 #include "kvatt.cuh"
 
@@ -77,7 +77,8 @@ __device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 
 // 2^y of two numbers by the FMA pipe (y <= 127): the whole part makes a power of two, 2^f on [-1/2, 1/2] is the polynomial of degree four whose largest relative
 // error is smallest (2.7e-6 in f32; coefficients by Remez's exchange).  NaN stays NaN through the clamp, the polynomial and the last product.  The special
 // function unit takes a warp's 32 in eight cycles; where two streams' softmax warps share one, every fourth pair goes this way: 4 x up to
-// 2000 rows, window 1024, 32 heads of 128 on 8 take 147 us at pages of 32 and 144 at 64, with none 153.5 and 153; at pages of 16, where copies bound it, 160 and 154.
+// 2000 rows, window 1024, 32 heads of 128 on 8 take 152 us with it and 154 without,
+// called again and again 147 and 153.5 (pages of 64: 144 and 153; of 16, where copies bound it, 160 and 154).
 // Every second pair is slower than every fourth, and one stream (head dimension 256) gains nothing.
 __device__ __forceinline__ float kp_max_nan(float a, float b) {
   float d;
