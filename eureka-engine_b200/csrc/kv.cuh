@@ -21,13 +21,11 @@ struct KvRows { const int *start; int rows, max_rows; };
 // 16-bit types: a value, and two in a word
 template <typename T> struct KvEl;
 template <> struct KvEl<__half> {
-  static __device__ __forceinline__ float to(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   static __device__ __forceinline__ uint16_t of(float v) { return __half_as_ushort(__float2half_rn(v)); }
   static __device__ __forceinline__ float2 to2(uint32_t v) { return __half22float2(*(const __half2 *)&v); }
   static __device__ __forceinline__ uint32_t of2(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *(const uint32_t *)&h; }
 };
 template <> struct KvEl<__nv_bfloat16> {
-  static __device__ __forceinline__ float to(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
   static __device__ __forceinline__ uint16_t of(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
   static __device__ __forceinline__ float2 to2(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
   static __device__ __forceinline__ uint32_t of2(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *(const uint32_t *)&h; }
@@ -126,28 +124,13 @@ __device__ __forceinline__ bool kv_any_sees(const KvSeq &s, int j, int window, i
   return j <= s.e0 + s.nc - 1 && (!window || j > s.e0 - window || j < sinks);
 }
 
-template <typename X, int E> __device__ __forceinline__ void kv_row_in(const X *p, bool wide, float (&x)[E]) {
-  if constexpr (sizeof(X) == 4) {
-    if (wide) {
+template <typename T, int E> __device__ __forceinline__ void kv_row_in(const T *p, float (&x)[E]) {
+  uint32_t w[E / 2];
+  if constexpr (E == 2) w[0] = __ldcg((const uint32_t *)p);
+  else if constexpr (E == 4) { const uint2 t = __ldcg((const uint2 *)p); w[0] = t.x; w[1] = t.y; }
+  else { const uint4 t = __ldcg((const uint4 *)p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
 #pragma unroll
-      for (int i = 0; i < E; i += 2) { const float2 f = __ldcg((const float2 *)(p + i)); x[i] = f.x; x[i + 1] = f.y; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; i++) x[i] = __ldcg((const float *)p + i);
-    }
-  } else {
-    if (wide) {
-      uint32_t w[E / 2];
-      if constexpr (E == 2) w[0] = __ldcg((const uint32_t *)p);
-      else if constexpr (E == 4) { const uint2 t = __ldcg((const uint2 *)p); w[0] = t.x; w[1] = t.y; }
-      else { const uint4 t = __ldcg((const uint4 *)p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
-#pragma unroll
-      for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<X>::to2(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; i++) x[i] = KvEl<X>::to(__ldcg((const uint16_t *)p + i));
-    }
-  }
+  for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<T>::to2(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
 }
 template <typename T, int E> __device__ __forceinline__ void kv_row_out(uint16_t *p, bool wide, const float (&x)[E]) {
   if (wide) {
@@ -175,7 +158,7 @@ __device__ __noinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b,
   constexpr int E = HD / 32;
   const int g = h / a.G, pm = (1 << c.page_sh) - 1;
   float q[E];
-  kv_row_in<T, E>((const T *)a.q + r * a.qs + (long long)h * HD + lane * E, true, q);
+  kv_row_in<T, E>((const T *)a.q + r * a.qs + (long long)h * HD + lane * E, q);
 #pragma unroll
   for (int i = 0; i < E; i++) { q[i] *= a.scale2; o[i] = 0.0f; }
   m = -INFINITY; l = 0.0f;
@@ -188,8 +171,8 @@ __device__ __noinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b,
     if (id < 0) continue;
     const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + lane * E;
     float k[E], v[E];
-    kv_row_in<T, E>((const T *)c.k + p, true, k);
-    kv_row_in<T, E>((const T *)c.v + p, true, v);
+    kv_row_in<T, E>((const T *)c.k + p, k);
+    kv_row_in<T, E>((const T *)c.v + p, v);
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; i++) s += q[i] * k[i];
