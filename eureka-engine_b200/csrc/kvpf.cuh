@@ -75,7 +75,9 @@ __device__ __forceinline__ void kp_ld32(uint32_t taddr, float *v) {
 __device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }   // the n lowest bits
 
 // 2^y of two numbers by the FMA pipe (y <= 127): the whole part makes a power of two, 2^f on [-1/2, 1/2] is the polynomial of degree four whose largest relative
-// error is smallest (2.7e-6 in f32; coefficients by Remez's exchange).  NaN stays NaN through the clamp, the polynomial and the last product.  The special
+// error is smallest (2.7e-6 in f32; coefficients by Remez's exchange).  NaN stays NaN through the clamp, the polynomial and the last product.  At -127, where the
+// clamp takes what is below it, a masked slot's minus infinity too, the power of two is an exact 0: 2^-126 would be a number in bf16, and a slot that a row
+// does not see would have a weight.  The special
 // function unit takes a warp's 32 in eight cycles; where two streams' softmax warps share one, every fourth pair goes this way: 4 x up to
 // 2000 rows, window 1024, 32 heads of 128 on 8 take 152 us with it and 154 without,
 // called again and again 147 and 153.5 (pages of 64: 144 and 153; of 16, where copies bound it, 160 and 154).
@@ -88,7 +90,7 @@ __device__ __forceinline__ float kp_max_nan(float a, float b) {
 __device__ __forceinline__ void kp_exp2_fma(f32x2 y, float &r0, float &r1) {
   float a, b;
   x2_unpack(y, a, b);
-  y = x2_pack(kp_max_nan(a, -126.0f), kp_max_nan(b, -126.0f));
+  y = x2_pack(kp_max_nan(a, -127.0f), kp_max_nan(b, -127.0f));
   const f32x2 big = x2_pack(12582912.0f, 12582912.0f), one = x2_pack(-1.0f, -1.0f);
   const f32x2 t = x2_add(y, big), f = x2_add(y, x2_fma(t, one, big));      // (t's low bits: the whole part)
   f32x2 v = x2_fma(x2_pack(0.009570102207362652f, 0.009570102207362652f), f, x2_pack(0.05591785907745361f, 0.05591785907745361f));

@@ -1,0 +1,60 @@
+"""The paged key-value cache's operators where values, lengths and counts are at the ends of their ranges (bounds as in test_kv_gpu)."""
+import math
+
+import pytest
+import torch
+
+from test_kv_gpu import DT, HALF, TINY, Cache, _attn, _check_attn, _clean, _evict, _ints, _weights
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- rows that see nothing, values that rows do not see ---------------------------------------------------
+@pytest.mark.parametrize("el", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("H,KV", [(4, 2), (1, 1), (6, 1)])
+@pytest.mark.parametrize("rows,lens", [([200], [50]), ([300, 140, 5], [64, 139, 3]), ([70], [69])])
+def test_rows_without_a_slot_beside_rows_with_many(llb, rows, lens, H, KV, hd, el):
+    """Rows at slots below 0 are zeros, to the last bit, also where rows of the same block see slots."""
+    c = Cache(llb, el, KV, hd, 16, lens, seed=101)
+    _check_attn(c, _attn(llb, c, H, rows, seed=102, max_len=140))
+    _check_attn(c, _attn(llb, c, H, rows, seed=102, max_len=140, window=30, sinks=3, el_out="f32"))
+    _clean(llb)
+
+
+@pytest.mark.parametrize("el", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64])
+def test_rows_whose_pages_are_all_bad(llb, page, hd, el):
+    """The first 64 slots are on no page: rows that see only those are zeros, and the rows behind them are right."""
+    n, H, KV = 150, 4, 2
+    c = Cache(llb, el, KV, hd, page, [n], seed=103)
+    c.table[0, :64 // page] = -1
+    r = _attn(llb, c, H, [n], seed=104)
+    assert llb.kv_errors() == 1
+    llb.lib().llb_b200_kv_errors_clear()
+    out = r["out"][:n].double().cpu().view(n, KV, H // KV, hd)
+    assert torch.all(out[:64] == 0)
+    c.lens_list, c.K, c.V = [n - 64], [c.K[0][64:]], [c.V[0][64:]]
+    r["out"], r["q"], r["rows"], r["start"] = r["out"][64:], r["q"][64:], [n - 64], [0, n - 64]
+    _check_attn(c, r)
+    _clean(llb)
+
+
+@pytest.mark.parametrize("el,big", [("bf16", 3.0e38), ("bf16", -2.0 ** 126), ("f16", 65504.0)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,window", [(150, 0), (150, 40), (40, 0), (4, 0)])
+def test_a_later_rows_large_values_do_not_reach_earlier_rows(llb, rows, window, hd, el, big):
+    """V of the last rows' own slots is as large as the type holds: the rows before them do not see it."""
+    KV, G, late = 2, 4, max(1, rows // 8)
+    m = rows + 40
+    c = Cache(llb, el, KV, hd, 16, [m], seed=105)
+    for j in range(m - late, m):
+        c.v[int(c.table[0, j // 16]), :, j % 16] = big
+    r = _attn(llb, c, KV * G, [rows], window=window, seed=106)
+    n = rows - late
+    r["out"][n:rows] = 7.0
+    r["rows"], r["start"] = [n], [0, n]
+    c.lens_list, c.K, c.V = [m - late], [c.K[0][:-late]], [c.V[0][:-late]]
+    _check_attn(c, r)
+    _clean(llb)
