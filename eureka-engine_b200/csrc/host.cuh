@@ -85,8 +85,21 @@ int gemm_launch_moe_dn(cudaStream_t s, int fmt, const MoeArgs &m, int ks);
 // engine.cu: held while work is queued outside a graph, and while an engine captures one
 std::recursive_mutex &llb_enqueue_lock(void);
 
+// an agent's operations on its CTA's barriers, in their order: {0 wait, barrier, phase}, {1 arrive, barrier, times}, {2 arrive, barrier, once a copy requested or an MMA
+// issued here is done}
+struct PfTrace {
+  int *ops, cap, n = 0;
+  void put(int kind, int b, int v) { if (3 * n + 2 < cap) { ops[3 * n] = kind; ops[3 * n + 1] = b; ops[3 * n + 2] = v; } n++; }
+  void wait(int b, int phase) { put(0, b, phase); }
+  void free_again(int b, int use) { if (use > 0) put(0, b, use - 1); }     // a ring's buffer at its use-th use
+  void arrive(int b) { put(1, b, 1); }
+  void later(int b) { put(2, b, 1); }
+};
+
 // kv.cu
 int kv_setup(void);
+int kv_pf_trace(PfTrace &t, int hd, int form, int n, int agent);
+int kv_pf_bar_count(int hd, int bar);
 
 // api.cu: from the first to the last of a series of uploads, the staging buffer of those from host memory is kept
 void upload_hold(bool from_host);

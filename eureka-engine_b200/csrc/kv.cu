@@ -362,6 +362,59 @@ __global__ void __launch_bounds__(256, 6) k_kv_move(const KvDev c, const KvDev d
   }
 }
 
+// ---- what the agents of k_kv_pf do with their barriers ----------------------------------------------
+// (llb_b200_pf_trace.)  form, bits: 1 the second query tile is empty, 2 every step rescales, 4 every step takes V out; n tiles.  Agents: the softmax warps, the loaders of K and
+// V, a thread a stream that issues MMAs.  Barriers: full K 0, V 6; empty K 12, V 18; s_full 24, p_full 28 (+ 2 stream + tile parity); pv_done 32; q_full 34.
+template <int HD> static int kp_trace(PfTrace &t, int form, int n, int agent) {
+  using C = Kp<HD>;
+  const int streams = C::NQT == 2 && !(form & 1) ? 2 : 1, q_full = 34;
+  if (agent >= C::SOFT + 2 + C::NQT || n < 1) return -1;
+  if (agent < C::SOFT) {
+    const int x = agent >> 2;
+    t.arrive(q_full);
+    if (x >= streams) return t.n;
+    for (int i = 0; i < n; i++) {
+      t.wait(24 + 2 * x + (i & 1), i >> 1);
+      if ((form & 2) && i) t.wait(32 + x, i - 1);
+      if (form & 4) t.wait(6 + i % C::NV, i / C::NV);
+      if (i && i == n - 1) t.wait(32 + x, n - 2);
+      t.arrive(28 + 2 * x + (i & 1));
+    }
+    t.wait(32 + x, n - 1);
+  } else if (agent < C::SOFT + 2) {
+    const bool isv = agent > C::SOFT;
+    const int N = isv ? C::NV : C::NK;
+    for (int i = 0; i < n; i++) {
+      t.free_again((isv ? 18 : 12) + i % N, i / N);
+      if (HD == 256 && isv && i == N - 1) t.wait(q_full, 0);
+      t.later((isv ? 6 : 0) + i % N);
+    }
+  } else if (agent < C::SOFT + 2 + streams) {
+    const int x = agent - C::SOFT - 2;
+    auto give = [&](int b) { for (int k = 0; k < (streams < C::NQT ? 2 : 1); k++) t.later(b); };
+    auto score = [&](int i) { t.wait(i % C::NK, i / C::NK); t.later(24 + 2 * x + (i & 1)); give(12 + i % C::NK); };
+    t.wait(q_full, 0);
+    score(0);
+    if (n > 1) score(1);
+    t.wait(6, 0);
+    for (int i = 0; i < n; i++) {
+      t.wait(28 + 2 * x + (i & 1), i >> 1);
+      t.later(32 + x); t.wait(32 + x, i);
+      give(18 + i % C::NV);
+      if (i + 1 < n) t.wait(6 + (i + 1) % C::NV, (i + 1) / C::NV);
+      if (i + 2 < n) score(i + 2);
+    }
+  }
+  return t.n;
+}
+int kv_pf_trace(PfTrace &t, int hd, int form, int n, int agent) {
+  return hd == 64 ? kp_trace<64>(t, form, n, agent) : hd == 128 ? kp_trace<128>(t, form, n, agent) : hd == 256 ? kp_trace<256>(t, form, n, agent) : -1;
+}
+int kv_pf_bar_count(int hd, int bar) {
+  const int nqt = hd == 256 ? 1 : 2;
+  return bar >= 12 && bar < 24 ? nqt : bar >= 28 && bar < 32 ? 4 : bar == 34 ? 4 * nqt : 1;
+}
+
 // ---- host -----------------------------------------------------------------------------------------
 // Every kernel is loaded here: one that is first met while a stream is being captured may not be.
 template <typename K> static int kv_load(K k, int smem = 0) {

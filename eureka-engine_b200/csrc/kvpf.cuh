@@ -336,13 +336,14 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
           if (bm >> (r >> 4) & 1) clear(r, r + 16);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
+      // (the last product is waited for below: it cannot begin, and end, before the one in front of it was seen to be done, whose phase would be missed then)
+      if (i && i == n - 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);
       t5_wait_st();
       t5_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full(x0, i));
     }
     // ---- the rows' results ----
-    if (n > 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);  // (the last two products may both be under way: one phase after the other)
     wait(pv_done(x0), (uint32_t)(n - 1) & 1u);
     __syncwarp();
     t5_fence_after();

@@ -744,17 +744,8 @@ int llb_b200_pf_gemm(int fmt, unsigned long long w, int rows, int K, unsigned lo
 }
 
 // ---- what the agents of the kernels here do with their barriers --------------------------------------
-// For a check without a GPU: every warp's waits and arrivals in its order, with the kernels' own rings and numbering.  ops: {0 wait, barrier, phase},
-// {1 arrive, barrier, times}, {2 arrive, barrier, once a copy requested or an MMA issued here is done}; a pair's second CTA has the same
+// For a check without a GPU: every warp's waits and arrivals in its order (PfTrace), with the kernels' own rings and numbering; a pair's second CTA has the same
 // barriers from PT_BARS on.  Returns the operations' number, 0 for an agent that has none, -1 past the last agent.
-struct PfTrace {
-  int *ops, cap, n = 0;
-  void put(int kind, int b, int v) { if (3 * n + 2 < cap) { ops[3 * n] = kind; ops[3 * n + 1] = b; ops[3 * n + 2] = v; } n++; }
-  void wait(int b, int phase) { put(0, b, phase); }
-  void free_again(int b, int use) { if (use > 0) put(0, b, use - 1); }     // a ring's buffer at its use-th use
-  void arrive(int b) { put(1, b, 1); }
-  void later(int b) { put(2, b, 1); }
-};
 #define PT_BARS 64
 static int pa_trace(PfTrace &t, int NS, int n, int agent) {
   const int full = 0, empty = 8, s_full = 16, p_full = 18, pv_done = 20, o_empty = 22, q_full = 23;
@@ -942,10 +933,11 @@ static int px2_trace(PfTrace &t, int units, int nsl, int agent) {
   return t.n;
 }
 static int px2_count(int b) { return b < 8 ? 8 : b >= 32 && b < 36 ? 16 : b >= 16 && b < 20 ? 2 : b >= 36 && b < 40 || b >= 44 ? 4 : 1; }
-// kernel: 0 k_pf_attn (form: head dimension; units x nsl tiles of positions), 1 k_pfx1 / k_pft of `form` rows, 2 k_pfx2
+// kernel: 0 k_pf_attn (form: head dimension; units x nsl tiles of positions), 1 k_pfx1 / k_pft of `form` rows, 2 k_pfx2, 3 k_kv_pf (kv_pf_trace)
 extern "C" __attribute__((visibility("default")))
 int llb_b200_pf_trace(int kernel, int form, int fmt, int units, int nsl, int agent, int *ops, int cap) {
   PfTrace t{ops, cap};
+  if (kernel == 3) return kv_pf_trace(t, form, fmt, units * nsl, agent);
   if (kernel == 0) return form == 128 || form == 256 ? pa_trace(t, pa_slots(form), units * nsl, agent) : -1;
 #define PT_ALL(F) (form == 32 ? pt_trace<F>(t, units, nsl, agent) : form == 64 ? px1_trace<F, 64>(t, units, nsl, agent) : px1_trace<F, 128>(t, units, nsl, agent))
   if (kernel == 1)
@@ -962,6 +954,7 @@ int llb_b200_pf_trace(int kernel, int form, int fmt, int units, int nsl, int age
 // arrivals that complete a phase of barrier `bar`
 extern "C" __attribute__((visibility("default")))
 int llb_b200_pf_bar_count(int kernel, int form, int fmt, int bar) {
+  if (kernel == 3) return kv_pf_bar_count(form, bar);
   bar %= PT_BARS;
   return kernel == 0 ? pa_count(bar) : kernel == 2 ? px2_count(bar) : form == 32 ? pt_count(bar) : px1_count(bar, px1_unpack(fmt, form));
 }

@@ -365,7 +365,9 @@ LLB_API int llb_b200_gemm_fits(int fmt, int nc, int nsb, int cap);
 LLB_API int llb_b200_gemm3_trace(int nc, int nsl, int tiles, int agent, int *ops, int cap);
 LLB_API int llb_b200_gemm3_bar_count(int nc, int bar);
 /* The same for the prompt path's kernels: 0 k_pf_attn (form: head dimension; units x nsl tiles of 32 positions), 1 k_pfx1 or k_pft (form: 32, 64
- * or 128 rows), 2 k_pfx2; a CTA's `units` work units of nsl super-blocks each.  A pair's second CTA has its barriers 64 numbers on. */
+ * or 128 rows), 2 k_pfx2; a CTA's `units` work units of nsl super-blocks each.  A pair's second CTA has its barriers 64 numbers on.
+ * 3 k_kv_pf (form: head dimension; fmt, bits: 1 the second query tile is empty, 2 every step rescales, 4 every step takes V out; units x nsl tiles of 64 slots);
+ * its products are done in the order in which they were issued: the issuing agent waits for each one's barrier where it would know of it. */
 LLB_API int llb_b200_pf_trace(int kernel, int form, int fmt, int units, int nsl, int agent, int *ops, int cap);
 LLB_API int llb_b200_pf_bar_count(int kernel, int form, int fmt, int bar);
 LLB_API void llb_spec_close(llb_spec *m);
