@@ -522,7 +522,7 @@ static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, K
   const size_t blocks = few_grid(), queries = (size_t)kv->seqs * a->heads * most_rows(a);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
-  p->least = KF_LEAST;
+  p->blocks = (int)blocks; p->least = KF_LEAST;
   p->unit = (int *)take((size_t)kv->seqs * kv->kv_heads * (((size_t)(a->heads / kv->kv_heads) * most_rows(a) + 15) / 16) * 8);
   p->pm = (float *)take(blocks * 2 * 16 * 4);
   p->pl = (float *)take(blocks * 2 * 16 * 4);
@@ -539,7 +539,7 @@ template <typename T, int HD> static int few_go(const llb_kv *kv, const llb_kv_a
   CUtensorMap km, vm;
   const int slots = std::min(kv->page, 1 << kf_sh(HD));
   if (pool_map(&km, kv, kv->k, slots, HD / 64) || pool_map(&vm, kv, kv->v, slots, HD / 64)) return -1;
-  const dim3 grid(few_grid()), block(32 * (kf_warps(HD) + 2));
+  const dim3 grid(p.blocks), block(32 * (kf_warps(HD) + 2));
   const int joins = c.seqs * c.KV * a.G * rw.max_rows, wblocks = (c.cap + KJ_SLOTS - 1) / KJ_SLOTS;   // (attn_check: they fit)
   if (a.w_out) {
     CU_OK(llb_launch(k_kv_few<T, HD, true>, grid, block, (size_t)kf_smem(HD), g_llb.stream, c, rw, a, p, km, vm));
@@ -643,6 +643,8 @@ int llb_b200_kv_errors_clear(void) {
   CU_OK(cudaMemsetAsync(g_kv_err, 0, 4, g_llb.stream));
   return 0;
 }
+
+int llb_b200_kv_join_parts(int first, int last) { return kf_parts_of(first, last, few_grid()); }
 
 int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a) {
   const char *const me = "kv_append";

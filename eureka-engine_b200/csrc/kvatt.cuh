@@ -44,6 +44,7 @@ __host__ __device__ constexpr int kf_smem(int HD) { return KF_HEAD + kf_ring(HD)
 static_assert(kf_smem(256) <= 232448 && kf_smem(128) <= 232448 && kf_smem(64) <= 232448, "shared memory");
 
 struct KvPlan {
+  int blocks;                  // of k_kv_few
   int least;                   // groups of a block's stretch, at least
   int *unit;                   // [seqs][KV][16-query tiles][2]: the first and the last block that had a part of the unit
   float *pm, *pl, *po;         // [2 blocks][16](, [hd])
@@ -466,6 +467,9 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
   }
 }
 
+// How many parts a unit has whose first and last block are noted so.  After a wait ran out (p.err) a unit may not be noted at all, and what stands there is whatever
+// the workspace held: no part, then, or parts that exist.
+__host__ __device__ __forceinline__ int kf_parts_of(int first, int last, int blocks) { return first >= 0 && last >= first && last < blocks ? last - first + 1 : 0; }
 // the part of a unit that block w had, of blocks w0 .. (only the first begins with the unit's first chunk)
 __device__ __forceinline__ size_t kf_part(int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }
 
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
     const int qi = blockIdx.x % NQM, gb = blockIdx.x / NQM, g = gb % c.KV, b = gb / c.KV;
     const int2 w = __ldcg((const int2 *)p.unit + (size_t)gb * QTM + (qi >> 4));
     const KvSeq s = kv_seq(c, rw, b, a.window, a.sinks, kf_sh(HD));
-    if (qi >= a.G * s.nc || w.x == w.y) return;
+    if (qi >= a.G * s.nc || kf_parts_of(w.x, w.y, p.blocks) < 2) return;
     float o[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; k++) o[k] = 0.0f;
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
     ask(wb * KJ_SLOTS);
     if (tid < NQ) {
       const int2 w = __ldcg((const int2 *)p.unit + ug * QTM + (tid >> 4));
-      if (w.x == w.y) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
+      if (kf_parts_of(w.x, w.y, p.blocks) < 2) lse[tid] = __ldcg(p.lse + ug * NQM + tid);
       else {
         float M = -INFINITY, l = 0.0f;
 #pragma unroll 4

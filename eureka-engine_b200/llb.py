@@ -85,7 +85,7 @@ def lib() -> C.CDLL:
             "llb_spec_set_prefill": (i32, [vp, i32]), "llb_spec_fast_rows": (C.c_double, [vp]), "llb_spec_prefill_extra": (i32, [vp, C.c_size_t]),
             "llb_b200_kv_append": (i32, [vp, vp]), "llb_b200_kv_attn": (i32, [vp, vp]), "llb_b200_kv_attn_ws": (sz, [vp, vp]),
             "llb_b200_kv_evict": (i32, [vp, vp, vp]), "llb_b200_kv_evict_ws": (sz, [vp, vp]),
-            "llb_b200_kv_errors": (i32, []), "llb_b200_kv_errors_clear": (i32, []),
+            "llb_b200_kv_errors": (i32, []), "llb_b200_kv_errors_clear": (i32, []), "llb_b200_kv_join_parts": (i32, [i32, i32]),
             "llb_b200_pf_gemm": (i32, [i32, u64, i32, i32, u64, i32, u64, i32]),
             "llb_b200_gemm_fits": (i32, [i32, i32, i32, i32]), "llb_b200_gemm_kernel": (i32, [i32, i32, i32, i32, i32, i32, C.POINTER(i32)]),
             "llb_b200_gemm3_trace": (i32, [i32, i32, i32, i32, C.POINTER(i32), i32]), "llb_b200_gemm3_bar_count": (i32, [i32, i32]),

@@ -234,6 +234,8 @@ LLB_API int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv
  * rows of a sequence (its rows, or those behind, were left out).  Synchronises.  -1 on a CUDA error. */
 LLB_API int llb_b200_kv_errors(void);
 LLB_API int llb_b200_kv_errors_clear(void);
+/* Test entry (no GPU needed): the parts that the joining launch of llb_b200_kv_attn takes of queries whose first and last block are noted so. */
+LLB_API int llb_b200_kv_join_parts(int first, int last);
 
 /* ---- 3. the speculative cycle ----------------------------------------------------------------- */
 /* Replaces host/llb_host.c:1474-1950 for greedy decoding with either of the reference's drafters.

@@ -42,3 +42,11 @@ def test_the_last_products_phase_may_not_pass_before_the_one_before_was_seen(pkg
             assert ops[i - 1] == (WAIT, 32, n - 2)
             ops[i - 1], ops[i] = ops[i], ops[i - 1]
         assert "phase" in check(t, _counts(L, hd))
+
+
+def test_what_a_block_that_gave_up_did_not_note_is_not_followed(pkg):
+    """The join takes its parts' numbers from the workspace; where a wait ran out those may be anything."""
+    parts = pkg.llb.lib().llb_b200_kv_join_parts
+    assert [parts(0, 0), parts(3, 3), parts(3, 9), parts(0, 147)] == [1, 1, 7, 148]
+    for first, last in ((-1, -1), (-1, 5), (0, 148), (148, 148), (5, 4), (0, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1), (-2 ** 31, -2 ** 31), (1 << 20, 1 << 20)):
+        assert parts(first, last) == 0, (first, last)
