@@ -475,6 +475,8 @@ static int kv_check(const llb_kv *kv, const char *what) {
   return 0;
 }
 static long long kv_most(const llb_kv *kv) { return std::min((long long)kv->table_stride * kv->page, (long long)INT_MAX - 256); }
+// ... and of a call that bounds them by max_len: what a call's sizes go by (max_len itself may be anything up to INT_MAX)
+static int kv_slots(const llb_kv *kv, int max_len) { return (int)std::min(kv_most(kv), (long long)max_len); }
 static KvDev kv_dev(const llb_kv *kv, long long cap) {
   KvDev c;
   c.k = (uint16_t *)(uintptr_t)kv->k; c.v = (uint16_t *)(uintptr_t)kv->v;
@@ -527,7 +529,7 @@ static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, K
   p->pm = (float *)take(blocks * 2 * 16 * 4);
   p->pl = (float *)take(blocks * 2 * 16 * 4);
   p->po = (float *)take(blocks * 2 * 16 * kv->head_dim * 4);
-  p->sstride = std::max(16, (a->max_len + 15) & ~15);
+  p->sstride = std::max(16, (kv_slots(kv, a->max_len) + 15) & ~15);
   p->lse = (float *)take(a->w_out ? queries * 4 : 0);
   p->sc = (float *)take(a->w_out ? queries * p->sstride * 4 : 0);
   return at;
@@ -557,7 +559,7 @@ static int pf_tiles(const llb_kv *kv, const llb_kv_attn *a) {
 }
 static size_t pf_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, KvPfPlan *p) {
   const long long sms = g_llb.sms ? g_llb.sms : 148, units = (long long)pf_tiles(kv, a) * kv->kv_heads * kv->seqs;
-  const int slots = a->window ? (int)std::min((long long)a->max_len, (long long)a->window + a->sinks + most_rows(a)) : a->max_len;   // that a unit sees, at most
+  const int len = kv_slots(kv, a->max_len), slots = a->window ? (int)std::min((long long)len, (long long)a->window + a->sinks + most_rows(a)) : len;   // that a unit sees, at most
   p->splits = (int)std::max(1LL, std::min(sms / std::max(units, 1LL), (long long)slots / 512));
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
@@ -599,10 +601,11 @@ static int attn_check(const llb_kv *kv, const llb_kv_attn *a) {
   if (!a->row_start || off(a->row_start, 4)) return llb_fail("kv_attn: row_start is int32 on the device");
   if (a->w_in && !a->w_out) return llb_fail("kv_attn: w_in without w_out");
   const long long queries = (long long)a->heads / kv->kv_heads * most_rows(a), pairs = (long long)kv->seqs * kv->kv_heads;
-  if (queries <= KV_FEW && pairs * ((queries + 15) / 16) > INT_MAX / 2 / (a->max_len / 32 + 3))
-    return llb_fail("kv_attn: %d sequences of %d kv heads with up to %d slots: more than are counted (max_len bounds it)", kv->seqs, kv->kv_heads, a->max_len);
-  if (queries >= 1 << 26 || pairs * (std::min(queries, (queries + 127) / 128 + KV_FEW) + (a->w_out ? (a->max_len + 511) / 512 : 0)) > INT_MAX)
-    return llb_fail("kv_attn: %d sequences of %d kv heads, %d rows, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, most_rows(a), a->max_len);
+  const int len = kv_slots(kv, a->max_len);
+  if (queries <= KV_FEW && pairs * ((queries + 15) / 16) > INT_MAX / 2 / (len / 32 + 3))
+    return llb_fail("kv_attn: %d sequences of %d kv heads with up to %d slots: more than are counted (max_len bounds it)", kv->seqs, kv->kv_heads, len);
+  if (queries >= 1 << 26 || pairs * (std::min(queries, (queries + 127) / 128 + KV_FEW) + (a->w_out ? (len + 511) / 512 : 0)) > INT_MAX)
+    return llb_fail("kv_attn: %d sequences of %d kv heads, %d rows, %d slots: more than one launch holds", kv->seqs, kv->kv_heads, most_rows(a), len);
   if (a->w_out) {
     if (off(a->w_in, 4) || off(a->w_out, 4)) return llb_fail("kv_attn: weights are f32 on the device");
     if (a->w_stride < a->max_len) return llb_fail("kv_attn: w_stride %d for %d slots", a->w_stride, a->max_len);
@@ -627,7 +630,7 @@ static int evict_check(const llb_kv *src, const llb_kv_evict *e) {
   if (e->kept && (off(e->kept, 4) || e->kept_stride < most)) return llb_fail("kv_evict: kept has %d slots a head or more", most);
   return 0;
 }
-static size_t evict_ws(const llb_kv *src, const llb_kv_evict *e) { return 16 + (e->kept ? 0 : (size_t)src->seqs * src->kv_heads * std::min(e->budget, e->max_len) * 4); }
+static size_t evict_ws(const llb_kv *src, const llb_kv_evict *e) { return 16 + (e->kept ? 0 : (size_t)src->seqs * src->kv_heads * std::min(e->budget, kv_slots(src, e->max_len)) * 4); }
 
 extern "C" {
 
@@ -712,7 +715,7 @@ int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *
   if (dst->el != src->el || dst->kv_heads != src->kv_heads || dst->head_dim != src->head_dim || dst->seqs != src->seqs)
     return llb_fail("kv_evict: dst has another type, other heads or other sequences than src");
   if (dst->table == src->table || dst->lens == src->lens) return llb_fail("kv_evict: dst has a table and lens of its own");
-  const int most = std::min(e->budget, e->max_len);
+  const int len = kv_slots(src, e->max_len), most = std::min(e->budget, len);
   if (kv_most(dst) < most) return llb_fail("kv_evict: dst holds %lld slots a sequence, %d may be kept", kv_most(dst), most);
   const size_t need = evict_ws(src, e);
   if (!e->kept && (!e->ws || off(e->ws, 16) || e->ws_bytes < need)) return llb_fail("kv_evict: a workspace of %zu bytes (%zu are needed, on a multiple of 16)", e->ws_bytes, need);
@@ -727,12 +730,12 @@ int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *
   // (keys of a block's slots; a block with few of them leaves room for others on its SM)
   auto pick = [&](auto cl) {
     constexpr int CL = decltype(cl)::value;
-    const int own = std::max((e->max_len + CL - 1) / CL, 1);
+    const int own = std::max((len + CL - 1) / CL, 1);
     const dim3 heads((unsigned)c.KV * CL, c.seqs);
     if (own <= KE_KEYS) return llb_launch(k_kv_pick<true, CL>, heads, dim3(KE_THREADS), (size_t)(KE_HIST + own) * 4, g_llb.stream, c, k);
     return llb_launch(k_kv_pick<false, CL>, heads, dim3(KE_THREADS), (size_t)KE_HIST * 4, g_llb.stream, c, k);
   };
-  if (e->max_len > KE_LONG) CU_OK(pick(std::integral_constant<int, KE_CLUSTER>()));
+  if (len > KE_LONG) CU_OK(pick(std::integral_constant<int, KE_CLUSTER>()));
   else CU_OK(pick(std::integral_constant<int, 1>()));
   if (!most) return 0;
   // blocks of a head: one trip each, as long as there are not more blocks than 64 an SM (eight: 6 % slower; one trip whatever the number: 7 %)

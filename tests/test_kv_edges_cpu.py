@@ -50,3 +50,38 @@ def test_what_a_block_that_gave_up_did_not_note_is_not_followed(pkg):
     assert [parts(0, 0), parts(3, 3), parts(3, 9), parts(0, 147)] == [1, 1, 7, 148]
     for first, last in ((-1, -1), (-1, 5), (0, 148), (148, 148), (5, 4), (0, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1), (-2 ** 31, -2 ** 31), (1 << 20, 1 << 20)):
         assert parts(first, last) == 0, (first, last)
+
+
+def _kv(llb, **kw):
+    a = dict(el=llb.EL["bf16"], kv_heads=1, head_dim=128, page=32, n_pages=64, seqs=1, table_stride=16, k=1 << 20, v=1 << 20, table=1 << 20, lens=1 << 20)
+    a.update(kw)
+    return llb.Kv(**a)
+
+
+def _attn(llb, max_len, **kw):
+    a = dict(rows=1, max_rows=1, max_len=max_len, heads=1, scale=0.0, el_out=llb.EL["bf16"], q=1 << 20, out=2 << 20, q_stride=128, out_stride=128, row_start=1 << 20)
+    a.update(kw)
+    return llb.KvAttn(**a)
+
+
+@pytest.mark.parametrize("max_len", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16, 2 ** 31 - 300, 1 << 30, 513])
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("rows", [1, 600])
+def test_a_workspace_goes_by_the_slots_that_the_table_holds(pkg, rows, weights, max_len):
+    """16 pages of 32 slots: no sequence has more than 512, whatever the call's bound is."""
+    llb = pkg.llb
+    if weights and rows > 64:
+        rows = 64
+    kw = dict(rows=rows, max_rows=rows, **(dict(w_out=1 << 20, w_stride=2 ** 31 - 1) if weights else {}))
+    want = llb.kv_attn_ws(_kv(llb), _attn(llb, 512, **kw))
+    assert not weights or want >= rows * 512 * 4
+    assert llb.kv_attn_ws(_kv(llb), _attn(llb, max_len, **kw)) == want
+
+
+@pytest.mark.parametrize("max_len", [2 ** 31 - 1, 2 ** 31 - 2, 513])
+def test_an_evictions_workspace_goes_by_the_slots_that_the_table_holds(pkg, max_len):
+    llb = pkg.llb
+    e = dict(budget=2 ** 31 - 1, w=1 << 20, w_stride=2 ** 31 - 1)
+    want = llb.kv_evict_ws(_kv(llb, seqs=3), llb.KvEvict(max_len=512, **e))
+    assert want >= 3 * 512 * 4
+    assert llb.kv_evict_ws(_kv(llb, seqs=3), llb.KvEvict(max_len=max_len, **e)) == want

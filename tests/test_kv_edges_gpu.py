@@ -58,3 +58,40 @@ def test_a_later_rows_large_values_do_not_reach_earlier_rows(llb, rows, window, 
     c.lens_list, c.K, c.V = [m - late], [c.K[0][:-late]], [c.V[0][:-late]]
     _check_attn(c, r)
     _clean(llb)
+
+
+@pytest.mark.parametrize("max_len", [2 ** 31 - 1, 2 ** 31 - 2, 1 << 30])
+def test_no_bound_on_the_lengths(llb, max_len):
+    """max_len says no more than the table: the same results as with the lengths' own bound."""
+    for lens, rows in (([700], [1]), ([700], [3]), ([700], [300])):
+        c = Cache(llb, "bf16", 1, 128, 16, lens, seed=114)
+        weights = rows[0] < 8
+        r = _attn(llb, c, 2, rows, seed=115, weights=weights)
+        _check_attn(c, r)
+        kv, a = r["call"]
+        want = r["out"].clone(), r["w_out"].clone() if weights else None
+        r["out"].fill_(7.0)
+        a.max_len = max_len
+        if weights:
+            r["w_out"].fill_(7.0)
+            a.w_stride = max_len                       # (one row of one head: the stride is never taken)
+        ws = torch.full((llb.kv_attn_ws(kv, a),), 255, dtype=torch.uint8, device="cuda")
+        a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
+        llb.kv_attn(kv, a)
+        llb.check(llb.lib().llb_b200_sync(), "sync")
+        _check_attn(c, r)
+        assert rows[0] > 8 or torch.equal(r["out"], want[0])
+        assert not weights or torch.equal(r["w_out"], want[1])
+    for n in (700, 13000):
+        c = Cache(llb, "bf16", 1, 64, 64, [n], seed=116)
+        w = _weights(1, 1, n, 117)
+        d, ids, w2, (src, dst, e, _) = _evict(llb, c, 300, 4, 30, w)
+        want = ids.clone(), w2.clone(), d.slots(0, 300).clone()
+        ids.fill_(-5), w2.fill_(7.0), d.k.fill_(math.nan)
+        e.max_len = e.w_stride = max_len
+        ws = torch.full((llb.kv_evict_ws(src, e),), 255, dtype=torch.uint8, device="cuda")
+        e.ws, e.ws_bytes = ws.data_ptr(), ws.numel()
+        llb.kv_evict(src, dst, e)
+        llb.check(llb.lib().llb_b200_sync(), "sync")
+        assert torch.equal(ids, want[0]) and torch.equal(w2, want[1]) and torch.equal(d.slots(0, 300), want[2])
+    _clean(llb)
