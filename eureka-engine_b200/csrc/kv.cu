@@ -474,7 +474,9 @@ static int kv_check(const llb_kv *kv, const char *what) {
   if (!kv->table || !kv->lens || off(kv->table, 4) || off(kv->lens, 4)) return llb_fail("%s: table and lens are int32 on the device", what);
   return 0;
 }
-static long long kv_most(const llb_kv *kv) { return std::min((long long)kv->table_stride * kv->page, (long long)INT_MAX - 256); }
+// the most slots of a sequence: a slot's number, rounded up to the 2048 that a joining block has or 32 boxes on, is an int
+#define KV_MOST (INT_MAX - 4095)
+static long long kv_most(const llb_kv *kv) { return std::min((long long)kv->table_stride * kv->page, (long long)KV_MOST); }
 // ... and of a call that bounds them by max_len: what a call's sizes go by (max_len itself may be anything up to INT_MAX)
 static int kv_slots(const llb_kv *kv, int max_len) { return (int)std::min(kv_most(kv), (long long)max_len); }
 static KvDev kv_dev(const llb_kv *kv, long long cap) {
@@ -518,6 +520,7 @@ static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int 
 #define KF_LEAST 2             // fewest groups of a block's stretch
 static int most_rows(const llb_kv_attn *a) { return std::min(a->max_rows, std::max(a->rows, 1)); }
 static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * most_rows(a) <= KV_FEW; }
+static_assert(KJ_SLOTS <= 2048 && (KV_MOST + 2047LL) / 2048 * 2048 <= INT_MAX, "a joining block's last slot");
 static int few_grid(void) { return g_llb.sms ? g_llb.sms : 148; }
 // its parts, one behind the other; the size where `base` is 0
 static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, KvPlan *p) {

@@ -159,7 +159,7 @@ typedef struct {
   int page;                    /* slots of a page: 16, 32, 64 or 128 */
   int n_pages;                 /* of the pool */
   int seqs;                    /* 1 .. 65535 */
-  int table_stride;            /* entries of a sequence in the table: table_stride * page slots are the most it can have */
+  int table_stride;            /* entries of a sequence in the table: table_stride * page slots are the most it can have, and 2^31 - 4096 */
   llb_b200_dptr k, v;          /* [n_pages][kv_heads][page][head_dim], 16-byte aligned */
   llb_b200_dptr table;         /* int32 [seqs][table_stride] */
   llb_b200_dptr lens;          /* int32 [seqs] */

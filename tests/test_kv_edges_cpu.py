@@ -85,3 +85,14 @@ def test_an_evictions_workspace_goes_by_the_slots_that_the_table_holds(pkg, max_
     want = llb.kv_evict_ws(_kv(llb, seqs=3), llb.KvEvict(max_len=512, **e))
     assert want >= 3 * 512 * 4
     assert llb.kv_evict_ws(_kv(llb, seqs=3), llb.KvEvict(max_len=max_len, **e)) == want
+
+
+@pytest.mark.parametrize("max_len", [2 ** 31 - 1, 2 ** 31 - 256, 2 ** 31 - 4095])
+def test_no_sequence_has_more_slots_than_are_counted(pkg, max_len):
+    """Tables of more than 2^31 slots (pages may be shared): lengths end where sums of slots and block sizes still fit 32 bits."""
+    llb = pkg.llb
+    kw = dict(w_out=1 << 20, w_stride=2 ** 31 - 1)
+    kv = _kv(llb, page=128, table_stride=1 << 25)
+    want = llb.kv_attn_ws(kv, _attn(llb, 2 ** 31 - 4096, **kw))
+    assert want > (2 ** 31 - 4096) * 4
+    assert llb.kv_attn_ws(kv, _attn(llb, max_len, **kw)) == want

@@ -95,3 +95,30 @@ def test_no_bound_on_the_lengths(llb, max_len):
         llb.check(llb.lib().llb_b200_sync(), "sync")
         assert torch.equal(ids, want[0]) and torch.equal(w2, want[1]) and torch.equal(d.slots(0, 300), want[2])
     _clean(llb)
+
+
+def test_the_longest_sequence(llb):
+    """2^31 - 4096 slots and more, all on one shared page of zeros: a window at the end, and what every slot got."""
+    most, hd = 2 ** 31 - 4096, 64
+    k = torch.zeros(1, 1, 128, hd, dtype=torch.bfloat16, device="cuda")
+    table, rs = torch.zeros(1, 1 << 24, dtype=torch.int32, device="cuda"), _ints([0, 1])
+    q, out = torch.ones(1, hd, dtype=torch.bfloat16, device="cuda"), torch.full((1, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+    w = torch.full((most + 8,), 7.0, device="cuda")
+    w[:most] = 0.5
+    for n in (most, most + 300, 2 ** 31 - 1):
+        lens = _ints([n])
+        kv = llb.Kv(el=2, kv_heads=1, head_dim=hd, page=128, n_pages=1, seqs=1, table_stride=1 << 24, k=k.data_ptr(), v=k.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr())
+        a = llb.KvAttn(rows=1, max_rows=1, max_len=2 ** 31 - 1, heads=1, window=100, sinks=3, el_out=2, q=q.data_ptr(), out=out.data_ptr(), q_stride=hd, out_stride=hd,
+                       row_start=rs.data_ptr(), w_in=w.data_ptr(), w_out=w.data_ptr(), w_stride=2 ** 31 - 1)
+        ws = torch.empty(llb.kv_attn_ws(kv, a), dtype=torch.uint8, device="cuda")
+        a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
+        llb.kv_attn(kv, a)
+        assert llb.kv_errors() == (2 if n > most else 0)
+        llb.lib().llb_b200_kv_errors_clear()
+        assert torch.all(out == 0)
+    got = w[:most] - 0.5
+    seen = torch.cat([got[:3], got[-100:]])
+    assert torch.all((seen - 3 / 103).abs() < 1e-6) and not got[3:-100].any() and torch.all(w[most:] == 7.0)
+    _clean(llb)
+    del w, ws, got, seen
+    torch.cuda.empty_cache()
