@@ -350,8 +350,10 @@ __global__ void __launch_bounds__(256, 6) k_kv_move(const KvDev c, const KvDev d
   constexpr int P = HD / 8;    // pieces of a row
   const int g = blockIdx.y, b = blockIdx.z, now = min(kv_len(c, b), e.budget);
   const size_t head = (size_t)b * c.KV + g;
-  for (int u = blockIdx.x * 256 + threadIdx.x; u < now * P; u += gridDim.x * 256) {
-    const int i = u / P, p = u % P, j = __ldcg(e.kept + head * e.kept_stride + i);
+  // (counted by slots: a sequence may have more pieces than an int holds)
+  const int p = threadIdx.x % P;
+  for (unsigned i = blockIdx.x * (256 / P) + threadIdx.x / P; i < (unsigned)now; i += gridDim.x * (256 / P)) {
+    const int j = __ldcg(e.kept + head * e.kept_stride + i);
     const int from = kv_page(c, b, j >> c.page_sh), to = kv_page(d, b, i >> d.page_sh);
     const bool on = from >= 0 && to >= 0;
     const size_t x = kv_at(c, on ? from : 0, g, HD) + (size_t)(j & ((1 << c.page_sh) - 1)) * HD + 8 * p, y = kv_at(d, on ? to : 0, g, HD) + (size_t)(i & ((1 << d.page_sh) - 1)) * HD + 8 * p;

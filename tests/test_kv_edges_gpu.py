@@ -122,3 +122,25 @@ def test_the_longest_sequence(llb):
     _clean(llb)
     del w, ws, got, seen
     torch.cuda.empty_cache()
+
+
+def test_evict_of_more_pieces_than_an_int_counts(llb):
+    """2^26 + 1000 slots of 32 pieces each are kept.  All of them lie on one page of ones, and go to one page: what is written there is the same
+    from everywhere."""
+    n, hd = (1 << 26) + 1000, 256
+    stride = n // 128 + 1
+    src, dst = (torch.full((1, 1, 128, hd), x, dtype=torch.bfloat16, device="cuda") for x in (1.0, 0.0))
+    tables = [torch.zeros(1, stride, dtype=torch.int32, device="cuda") for _ in range(2)]
+    lens = [_ints([n]), _ints([-9])]
+    w = torch.rand(1, 1, n, device="cuda")
+    w2 = torch.full_like(w, 7.0)
+    kept = torch.full((1, 1, n), -5, dtype=torch.int32, device="cuda")
+    kv = [llb.Kv(el=2, kv_heads=1, head_dim=hd, page=128, n_pages=1, seqs=1, table_stride=stride, k=x.data_ptr(), v=x.data_ptr(), table=t.data_ptr(), lens=m.data_ptr())
+          for x, t, m in zip((src, dst), tables, lens)]
+    e = llb.KvEvict(budget=n, max_len=n, w=w.data_ptr(), w_stride=n, w_out=w2.data_ptr(), w_out_stride=n, kept=kept.data_ptr(), kept_stride=n)
+    llb.kv_evict(kv[0], kv[1], e)
+    llb.check(llb.lib().llb_b200_sync(), "sync")
+    assert int(lens[1]) == n and torch.equal(w2, w)
+    assert torch.equal(kept[0, 0], torch.arange(n, dtype=torch.int32, device="cuda"))
+    assert torch.all(dst == 1)
+    _clean(llb)
