@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(256, 6) k_kv_move(const KvDev c, const KvDev d
 
 // ---- what the agents of k_kv_pf do with their barriers ----------------------------------------------
 // (llb_b200_pf_trace.)  form, bits: 1 the second query tile is empty, 2 every step rescales, 4 every step takes V out; n tiles.  Agents: the softmax warps, the loaders of K and
-// V, a thread a stream that issues MMAs.  Barriers: full K 0, V 6; empty K 12, V 18; s_full 24, p_full 28 (+ 2 stream + tile parity); pv_done 32; q_full 34.
+// V, a thread a stream that issues MMAs.  Barriers: full K 0, V 6; empty K 12, V 18; s_full 24, p_full 28 (+ 2 stream + tile parity); pv_done 32; q_full 34; pv_last 35.
 template <int HD> static int kp_trace(PfTrace &t, int form, int n, int agent) {
   using C = Kp<HD>;
   const int streams = C::NQT == 2 && !(form & 1) ? 2 : 1, q_full = 34;
@@ -379,10 +379,10 @@ template <int HD> static int kp_trace(PfTrace &t, int form, int n, int agent) {
       t.wait(24 + 2 * x + (i & 1), i >> 1);
       if ((form & 2) && i) t.wait(32 + x, i - 1);
       if (form & 4) t.wait(6 + i % C::NV, i / C::NV);
-      if (i && i == n - 1) t.wait(32 + x, n - 2);
       t.arrive(28 + 2 * x + (i & 1));
     }
-    t.wait(32 + x, n - 1);
+    if (n > 1) t.wait(32 + x, n - 2);
+    t.wait(35 + x, 0);
   } else if (agent < C::SOFT + 2) {
     const bool isv = agent > C::SOFT;
     const int N = isv ? C::NV : C::NK;
@@ -401,7 +401,8 @@ template <int HD> static int kp_trace(PfTrace &t, int form, int n, int agent) {
     t.wait(6, 0);
     for (int i = 0; i < n; i++) {
       t.wait(28 + 2 * x + (i & 1), i >> 1);
-      t.later(32 + x); t.wait(32 + x, i);
+      if (i + 1 < n) { t.later(32 + x); t.wait(32 + x, i); }
+      else t.later(35 + x);
       give(18 + i % C::NV);
       if (i + 1 < n) t.wait(6 + (i + 1) % C::NV, (i + 1) / C::NV);
       if (i + 2 < n) score(i + 2);

@@ -115,6 +115,8 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   auto s_full = [&](int x, int i) { return bar_s + 192u + 8u * (uint32_t)(2 * x + (i & 1)); };
   auto p_full = [&](int x, int i) { return bar_s + 224u + 8u * (uint32_t)(2 * x + (i & 1)); };
   auto pv_done = [&](int x) { return bar_s + 256u + 8u * (uint32_t)x; };
+  // a stream's last product has a barrier of its own: both phases of the last two products could pass before a warp that did not have to rescale looks for either
+  auto pv_last = [&](int x) { return bar_s + 352u + 8u * (uint32_t)x; };
   const uint32_t q_full = bar_s + 272u;
   uint32_t *tmem_slot = (uint32_t *)(smem + 280);
   volatile uint32_t *dead = (volatile uint32_t *)(smem + 284);
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   // (what needs nothing of the call: barriers, each of its own thread; a tile's places are given back by both streams)
   if (tid < 12) { mbar_init(full(tid >= 6, tid % 6), 1); mbar_init(empty(tid >= 6, tid % 6), NQT); }
   if (tid < 4) { mbar_init(s_full(tid >> 1, tid), 1); mbar_init(p_full(tid >> 1, tid), 4); }
-  if (tid < 2) mbar_init(pv_done(tid), 1);
+  if (tid < 4) mbar_init(tid < 2 ? pv_done(tid) : pv_last(tid - 2), 1);
   if (tid == 0) { mbar_init(q_full, C::SOFT); *dead = 0; }
   if (tid < 12) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
@@ -336,15 +338,14 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
           if (bm >> (r >> 4) & 1) clear(r, r + 16);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      // (the last product is waited for below: it cannot begin, and end, before the one in front of it was seen to be done, whose phase would be missed then)
-      if (i && i == n - 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);
       t5_wait_st();
       t5_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full(x0, i));
     }
     // ---- the rows' results ----
-    wait(pv_done(x0), (uint32_t)(n - 1) & 1u);
+    if (n > 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);  // (that barrier's last phase.  Without this wait 3011 rows of 24 heads of 256 take 108.2 us for 106.9)
+    wait(pv_last(x0), 0);
     __syncwarp();
     t5_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         const uint32_t P = S0 + (uint32_t)(TILE * (i & 1));
 #pragma unroll
         for (int d = 0; d < TILE / 16; d++) t5_mma_f16_ts(O, P + 8 * d, vd + 128 * d, ido, i != 0 || d != 0);
-        t5_commit(pv_done(x));
+        t5_commit(i + 1 < n ? pv_done(x) : pv_last(x));
         t5_commit(empty(true, vs));
         if (streams < NQT) t5_commit(empty(true, vs));
         if (++vs == NV) { vs = 0; vp ^= 1u; }
