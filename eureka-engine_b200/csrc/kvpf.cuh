@@ -324,15 +324,16 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         const int rs = i % NV;
         wait(full(true, rs), (uint32_t)(i / NV) & 1u);
         const uint32_t at = ringv_s + rs * GB;
-        auto clear = [&](int ra, int rz) {                 // rows ra .. rz - 1 of the tile
+        auto clear = [&](int ra, int rz) {                 // rows ra .. rz - 1, those of them that the tile has
+          ra = min(max(ra, 0), TILE); rz = min(max(rz, 0), TILE);
 #pragma unroll 1
           for (int w = ra * (HD / 8) + (tid & 127); w < rz * (HD / 8); w += 128) {
             const int r = w / (HD / 8), d = w % (HD / 8);  // a row's 16 bytes, in the order in which they lie
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (d >> 3) * BLK + r * 128 + ((d & 7) << 4)), "r"(0) : "memory");
           }
         };
-        clear(max(0, ez + 1 - slot), TILE);
-        if (a.window) clear(max(0, a.sinks - slot), min(TILE, ea - a.window + 1 - slot));
+        clear(ez + 1 - slot, TILE);
+        if (a.window) clear(a.sinks - slot, ea - a.window + 1 - slot);
 #pragma unroll 1
         for (int r = 0; bm && r < TILE; r += 16)
           if (bm >> (r >> 4) & 1) clear(r, r + 16);

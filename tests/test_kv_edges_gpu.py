@@ -144,3 +144,51 @@ def test_evict_of_more_pieces_than_an_int_counts(llb):
     assert torch.equal(kept[0, 0], torch.arange(n, dtype=torch.int32, device="cuda"))
     assert torch.all(dst == 1)
     _clean(llb)
+
+
+# ---- windows, lengths and counts at the ends of their ranges ----------------------------------------------
+@pytest.mark.parametrize("sinks", [2 ** 26, 2 ** 27, 2 ** 28 + 3, 2 ** 31 - 1])
+@pytest.mark.parametrize("window", [1, 40, 2 ** 27, 2 ** 30])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_more_first_tokens_than_there_are_slots(llb, hd, window, sinks):
+    """... make every slot up to the row's own seen, whatever the window."""
+    c = Cache(llb, "bf16", 2, hd, 16, [150, 300, 90], seed=118)
+    _check_attn(c, _attn(llb, c, 4, [150, 130, 1], window=window, sinks=sinks, seed=119))
+    _check_attn(c, _attn(llb, c, 4, [3, 1, 2], window=window, sinks=sinks, seed=119, weights=True))
+    _clean(llb)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_rows_far_behind_their_first_tokens(llb, hd):
+    """Rows at slots from 2^28 on, all slots on shared pages: two for the first tokens, one in between, two for the window."""
+    n, rows, window, sinks, page = (1 << 28) + 133, 133, 60, 37, 64
+    g = torch.Generator(device="cuda").manual_seed(120)
+    k, v = (torch.randn(5, 1, page, hd, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    k[2], v[2] = math.nan, math.nan
+    last = -(-n // page)
+    table = torch.full((1, last), 2, dtype=torch.int32, device="cuda")
+    table[0, 0], table[0, 1] = 0, 1
+    table[0, last - 4:] = _ints([3, 4, 3, 4])
+    lens, rs = _ints([n]), _ints([0, rows])
+    q = torch.randn(rows, hd, device="cuda", dtype=torch.bfloat16, generator=g)
+    out = torch.full_like(q, 7.0)
+    kv = llb.Kv(el=2, kv_heads=1, head_dim=hd, page=page, n_pages=5, seqs=1, table_stride=last, k=k.data_ptr(), v=v.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr())
+    a = llb.KvAttn(rows=rows, max_rows=rows, max_len=n, heads=1, window=window, sinks=sinks, el_out=2, q=q.data_ptr(), out=out.data_ptr(), q_stride=hd, out_stride=hd, row_start=rs.data_ptr())
+    ws = torch.full((llb.kv_attn_ws(kv, a),), 255, dtype=torch.uint8, device="cuda")
+    a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
+    llb.kv_attn(kv, a)
+    llb.check(llb.lib().llb_b200_sync(), "sync")
+    _clean(llb)
+    # the same with the slots in between left out: the first tokens, then the window's slots
+    skip = (last - 4) * page - 2 * page
+    K, V = (torch.cat([x[0, 0], x[1, 0], x[3, 0], x[4, 0], x[3, 0], x[4, 0]]).double().cpu() for x in (k, v))
+    j = torch.arange(len(K))
+    for i in range(rows):
+        e = n - rows + i - skip
+        idx = ((j <= e) & ((j > e - window) | (j < sinks))).nonzero()[:, 0]
+        x = (q[i].double().cpu() @ K[idx].T) * hd ** -0.5
+        p = torch.softmax(x, 0)
+        want, size = p @ V[idx], p @ V[idx].abs()
+        # scores below 10 are off by hd 2^-23 of |q| |K| / sqrt(hd) < 40 at most, a probability by four times that and 2^-8; then the result's rounding
+        bound = size * (4 * 40 * hd * 2.0 ** -23 + 2.0 ** -8) + want.abs() * 2.0 ** -8
+        assert torch.all((out[i].double().cpu() - want).abs() <= bound * 1.01 + 1e-30), i
