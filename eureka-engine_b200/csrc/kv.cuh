@@ -80,6 +80,10 @@ __device__ __forceinline__ void kv_check_rows(const KvDev &c, const KvRows &r) {
 // what the row at slot e sees
 __device__ __forceinline__ int kv_first(int e, int window) { return window && e >= window ? e - window + 1 : 0; }   // first slot of its window
 
+// last slot before its window, or some slot below 0.  Rows at slots below 0 see nothing: what several rows see begins with the first at slot 0 or above (and the
+// difference stays an int for every window)
+__device__ __forceinline__ int kv_before(int e, int window) { return max(e, 0) - window; }
+
 // ---- a call's attention ----------------------------------------------------------------------------
 struct KvAttn {
   const uint16_t *q;
@@ -121,7 +125,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvDev &c, const KvRows &r, int b, 
 __device__ __forceinline__ int kv_chunk_slot(const KvSeq &s, int ch, int sh) { return (ch < s.cs ? ch : (s.lo >> sh) + ch - s.cs) << sh; }
 // whether some row of the sequence sees slot j
 __device__ __forceinline__ bool kv_any_sees(const KvSeq &s, int j, int window, int sinks) {
-  return j <= s.e0 + s.nc - 1 && (!window || j > s.e0 - window || j < sinks);
+  return j <= s.e0 + s.nc - 1 && (!window || j > kv_before(s.e0, window) || j < sinks);
 }
 
 template <typename T, int E> __device__ __forceinline__ void kv_row_in(const T *p, float (&x)[E]) {

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       auto pages = [&](int ch) {                           // of box lane % boxes of group ch + lane / boxes
         Entry x = {-1, false};
         const int k = ch + (lane >> (SH - bs)), j = kv_chunk_slot(use.s, k, SH) + ((lane & (boxes - 1)) << bs);
-        x.on = k < use.c1 && j <= last && (!a.window || j + bmask > use.s.e0 - a.window || j < a.sinks);
+        x.on = k < use.c1 && j <= last && (!a.window || j + bmask > kv_before(use.s.e0, a.window) || j < a.sinks);
         if (x.on) asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(x.id) : "l"(c.table + (size_t)use.b * c.tstride + (j >> c.page_sh)));
         return x;
       };
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
     for (int k = 0; k < 2; k++) {
       const int qi = q0 + gid + 8 * k;
       e[k] = qi < NQ ? s.e0 + kv_row_of(a, qi) : -1;
-      lw[k] = a.window ? e[k] - a.window + 1 : 0;
+      lw[k] = a.window ? kv_before(e[k], a.window) + 1 : 0;
     }
     const int ea = s.e0 + kv_row_of(a, q0), ez = s.e0 + kv_row_of(a, min(q0 + 15, NQ - 1));      // slots of the unit's first and last row
     const int m1 = (n0 + use.c1 - use.c0) * PG;
@@ -283,11 +283,11 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       const uint32_t k_s = ring_s + st * SB + ((16 * part) >> bs) * (HD * 2 << bs) + ((16 * part) & bmask) * 128, v_s = k_s + KB, blk = 128u << bs;   // 64 dims of a box
       wait(full(st), (uint32_t)(n / NG) & 1u);
       // (nothing of it is seen, or it was not brought)
-      const bool none = (hd.bad[st] >> part & 1) || dead || slot > last || (a.window && slot + 15 <= s.e0 - a.window && slot >= a.sinks);
+      const bool none = (hd.bad[st] >> part & 1) || dead || slot > last || (a.window && slot + 15 <= kv_before(s.e0, a.window) && slot >= a.sinks);
       float x[2][4];
       if (!none) {
         // slots that no row sees: their V is taken out, whatever it holds (0 times NaN is NaN)
-        if (slot + 15 > last || (a.window && slot <= s.e0 - a.window && slot + 15 >= a.sinks)) {
+        if (slot + 15 > last || (a.window && slot <= kv_before(s.e0, a.window) && slot + 15 >= a.sinks)) {
           for (int i = lane; i < 16 * TD; i += 32) {
             const int r = i & 15;
             if (!kv_any_sees(s, slot + r, a.window, a.sinks)) *(uint4 *)(smem + (v_s - bar_s) + (i >> 7) * blk + r * 128 + ((i >> 4) & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = (y[0][i >> 2][i & 3] + y[1][i >> 2][i & 3]) * a.scale2;
       }
-      const bool whole = !none && slot + 15 <= ea && (!a.window || slot > ez - a.window || slot + 15 < a.sinks) && q0 + 15 < NQ;
+      const bool whole = !none && slot + 15 <= ea && (!a.window || slot > kv_before(ez, a.window) || slot + 15 < a.sinks) && q0 + 15 < NQ;
       if (!whole) {
 #pragma unroll
         for (int t = 0; t < 2; t++)

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
   const KpTiles kt = kp_tiles<SH>(ea, ez, a.window, a.sinks);
   const int per = (kt.n + p.splits - 1) / p.splits, t0 = min(kt.n, split * per), n = min(kt.n, t0 + per) - t0;
   auto slot_of = [&](int i) { i += t0; return (i < kt.cs ? i : kt.lo + i - kt.cs) << SH; };
-  auto seen = [&](int j) { return j <= ez && (!a.window || j > ea - a.window || j < a.sinks); };   // by some row of the block
+  auto seen = [&](int j) { return j <= ez && (!a.window || j > kv_before(ea, a.window) || j < a.sinks); };   // by some row of the block
   auto part_of = [&](int qi) { return (((size_t)b * c.KV + g) * ((size_t)a.G * rw.max_rows) + qi) * p.splits + split; };
   if (!n) {
     for (int qi = q0 + tid; qi < min(q0 + QT, NQ); qi += C::THREADS) {
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     Entry x = {-1, false};
     if (lane < boxes && i < n) {
       const int j = slot_of(i) + (lane << bs);
-      x.on = j <= ez && (!a.window || j + (1 << bs) - 1 > ea - a.window || j < a.sinks);   // (what is seen is one run of slots and the first ones)
+      x.on = j <= ez && (!a.window || j + (1 << bs) - 1 > kv_before(ea, a.window) || j < a.sinks);   // (what is seen is one run of slots and the first ones)
       if (x.on) asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(x.id) : "l"(c.table + (size_t)b * c.tstride + (j >> c.page_sh)));
     }
     return x;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
 
   if (warp < 4 * streams) {
     // ---- softmax: a thread a query ----
-    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = s.e0 + kv_row_of(a, min(qi, NQ - 1)), lw = a.window ? e - a.window + 1 : 0;
+    const int x0 = warp >> 2, qi = q0 + 128 * x0 + (tid & 127), e = s.e0 + kv_row_of(a, min(qi, NQ - 1)), lw = a.window ? kv_before(e, a.window) + 1 : 0;
     const uint32_t lq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     // the queries: into shared memory as the product reads them, or through the last place of V's ring into tensor memory, 128 dims at a time
     {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       for (int k = 0; k < TILE; k += 32) kp_ld32(S + k, v + k);
       t5_wait_ld();
       const uint32_t bm = badm[i & 15];
-      if (bm || slot + TILE - 1 > ra || (a.window && slot <= rz - a.window && slot + TILE - 1 >= a.sinks)) {
+      if (bm || slot + TILE - 1 > ra || (a.window && slot <= kv_before(rz, a.window) && slot + TILE - 1 >= a.sinks)) {
 #pragma unroll
         for (int k0 = 0; k0 < TILE; k0 += 32) {            // a bit a slot: seen
           const int j = slot + k0;
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       l += a0 + a1;
       // slots that no row of the block sees: their V is taken out, whatever the page holds, before the first product with the tile
       // (every stream's warps do it: what is zero is written as zero again)
-      if (bm || slot + TILE - 1 > ez || (a.window && slot <= ea - a.window && slot + TILE - 1 >= a.sinks)) {
+      if (bm || slot + TILE - 1 > ez || (a.window && slot <= kv_before(ea, a.window) && slot + TILE - 1 >= a.sinks)) {
         const int rs = i % NV;
         wait(full(true, rs), (uint32_t)(i / NV) & 1u);
         const uint32_t at = ringv_s + rs * GB;
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
           }
         };
         clear(ez + 1 - slot, TILE);
-        if (a.window) clear(a.sinks - slot, ea - a.window + 1 - slot);
+        if (a.window) clear(a.sinks - slot, kv_before(ea, a.window) + 1 - slot);
 #pragma unroll 1
         for (int r = 0; bm && r < TILE; r += 16)
           if (bm >> (r >> 4) & 1) clear(r, r + 16);

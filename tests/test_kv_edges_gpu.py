@@ -192,3 +192,13 @@ def test_rows_far_behind_their_first_tokens(llb, hd):
         # scores below 10 are off by hd 2^-23 of |q| |K| / sqrt(hd) < 40 at most, a probability by four times that and 2^-8; then the result's rounding
         bound = size * (4 * 40 * hd * 2.0 ** -23 + 2.0 ** -8) + want.abs() * 2.0 ** -8
         assert torch.all((out[i].double().cpu() - want).abs() <= bound * 1.01 + 1e-30), i
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3, 2 ** 30])
+@pytest.mark.parametrize("rows,lens", [([200, 130], [50, 130]), ([4, 3], [2, 0]), ([3, 2], [600, 1])])
+@pytest.mark.parametrize("sinks", [0, 5])
+def test_a_window_larger_than_every_length(llb, rows, lens, sinks, window):
+    """... sees all slots up to the row's own, also behind rows at slots below 0."""
+    c = Cache(llb, "bf16", 2, 128, 16, lens, seed=107)
+    _check_attn(c, _attn(llb, c, 4, rows, window=window, sinks=sinks, seed=108, max_len=640, weights=max(rows) < 8))
+    _clean(llb)
