@@ -201,6 +201,7 @@ __device__ __forceinline__ uint32_t kv_key(float w) {
 #define KE_KEYS 49152          // most slots of a block whose keys have room
 #define KE_HIST (4 * 2048)     // words: the passes' counts, and their sum over the cluster
 #define KE_SMEM ((KE_HIST + KE_KEYS) * 4)
+static_assert(KE_LONG <= KE_KEYS, "one block's keys always have room");
 template <bool ROOM, int CL>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(KE_THREADS, 2) k_kv_pick(const KvDev c, const KvEvict e) {
   constexpr int NT = KE_THREADS;
@@ -432,9 +433,8 @@ template <typename T, int HD> static int load_of() {
          kv_load(k_kv_pf<T, HD>, Kp<HD>::SMEM) || kv_load(k_kv_pf_join<T, HD>) || load_append<T, float, HD>() || load_append<T, __half, HD>() || load_append<T, __nv_bfloat16, HD>();
 }
 template <int HD> static int load_hd() { return load_of<__half, HD>() || load_of<__nv_bfloat16, HD>() || kv_load(k_kv_move<HD>); }
-template <int CL> static int load_pick() { return kv_load(k_kv_pick<true, CL>, KE_SMEM) || kv_load(k_kv_pick<false, CL>); }
 int kv_setup(void) {
-  if (load_hd<64>() || load_hd<128>() || load_hd<256>() || load_pick<1>() || load_pick<KE_CLUSTER>()) return -1;
+  if (load_hd<64>() || load_hd<128>() || load_hd<256>() || kv_load(k_kv_pick<true, 1>, KE_SMEM) || kv_load(k_kv_pick<true, KE_CLUSTER>, KE_SMEM) || kv_load(k_kv_pick<false, KE_CLUSTER>)) return -1;
   if (!g_kv_map) {
     cudaDriverEntryPointQueryResult found;
     CU_OK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", (void **)&g_kv_map, 12000, cudaEnableDefault, &found));
@@ -734,15 +734,11 @@ int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *
   k.kept = (int *)(uintptr_t)(e->kept ? e->kept : e->ws); k.kept_stride = e->kept ? e->kept_stride : most;
   k.dst_lens = (int *)(uintptr_t)dst->lens;
   // (keys of a block's slots; a block with few of them leaves room for others on its SM)
-  auto pick = [&](auto cl) {
-    constexpr int CL = decltype(cl)::value;
-    const int own = std::max((len + CL - 1) / CL, 1);
-    const dim3 heads((unsigned)c.KV * CL, c.seqs);
-    if (own <= KE_KEYS) return llb_launch(k_kv_pick<true, CL>, heads, dim3(KE_THREADS), (size_t)(KE_HIST + own) * 4, g_llb.stream, c, k);
-    return llb_launch(k_kv_pick<false, CL>, heads, dim3(KE_THREADS), (size_t)KE_HIST * 4, g_llb.stream, c, k);
-  };
-  if (len > KE_LONG) CU_OK(pick(std::integral_constant<int, KE_CLUSTER>()));
-  else CU_OK(pick(std::integral_constant<int, 1>()));
+  const int blocks = len > KE_LONG ? KE_CLUSTER : 1, own = std::max((len + blocks - 1) / blocks, 1);
+  const dim3 heads((unsigned)c.KV * blocks, c.seqs);
+  if (blocks == 1) CU_OK(llb_launch(k_kv_pick<true, 1>, heads, dim3(KE_THREADS), (size_t)(KE_HIST + own) * 4, g_llb.stream, c, k));
+  else if (own <= KE_KEYS) CU_OK(llb_launch(k_kv_pick<true, KE_CLUSTER>, heads, dim3(KE_THREADS), (size_t)(KE_HIST + own) * 4, g_llb.stream, c, k));
+  else CU_OK(llb_launch(k_kv_pick<false, KE_CLUSTER>, heads, dim3(KE_THREADS), (size_t)KE_HIST * 4, g_llb.stream, c, k));
   if (!most) return 0;
   // blocks of a head: one trip each, as long as there are not more blocks than 64 an SM (eight: 6 % slower; one trip whatever the number: 7 %)
   const long long pieces = (long long)most * (src->head_dim / 8), room = std::max(1LL, 64LL * g_llb.sms / ((long long)c.KV * c.seqs));

@@ -202,3 +202,18 @@ def test_a_window_larger_than_every_length(llb, rows, lens, sinks, window):
     c = Cache(llb, "bf16", 2, 128, 16, lens, seed=107)
     _check_attn(c, _attn(llb, c, 4, rows, window=window, sinks=sinks, seed=108, max_len=640, weights=max(rows) < 8))
     _clean(llb)
+
+
+@pytest.mark.parametrize("kind", ["mixed", "equal", "nan"])
+def test_evict_of_a_sequence_whose_keys_have_no_room(llb, kind):
+    """More slots than four blocks' shared memory holds keys of (4 x 49152): the weights are read in every pass."""
+    lens = [200001, 196609, 5000]
+    w = _weights(3, 1, 200001, 112, ties=0.5)
+    if kind == "equal":
+        w.fill_(0.25)
+    elif kind == "nan":
+        w[:, :, 1000:199000:2] = math.nan
+    c = Cache(llb, "bf16", 1, 64, 128, lens, seed=113)
+    for budget, sinks, recent in ((9000, 16, 500), (150000, 0, 0)):
+        _evict(llb, c, budget, sinks, recent, w, page2=128)
+    _clean(llb)
