@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       if (!wholly) { *(float2 *)(p.po + (part + r) * HD + dim) = v; return; }
       const int qi = q0 + r, row = kv_row_of(a, qi), h = use.g * a.G + qi - row * a.G;
       const float L = hd.L[r], inv = L == 0.0f ? 0.0f : 1.0f / L;   // (nothing seen: zeros)
-      if (!(fabsf(v.x) + fabsf(v.y) + L < INFINITY)) hd.odd[r] = 1;
+      if (kv_again<T>(v.x) || kv_again<T>(v.y)) hd.odd[r] = 1;
       const long long at = (long long)(s.first + row) * a.os + (long long)h * HD + dim;
       if (a.out32) *(float2 *)((float *)a.out + at) = make_float2(v.x * inv, v.y * inv);
       else *(uint32_t *)((uint16_t *)a.out + at) = KvEl<T>::of2(v.x * inv, v.y * inv);
@@ -457,10 +457,12 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
 #pragma unroll 1
     for (int k = warp; wholly && k < 16; k += CW) {
       if (!hd.odd[k]) continue;
-      const int rk = kv_row_of(a, q0 + k), hk = use.g * a.G + q0 + k - rk * a.G;
-      float v[HD / 32], mk, lk;
-      kv_attn_row<T, HD>(c, a, use.b, s.first + rk, hk, s.e0 + rk, lane, v, mk, lk);
-      kv_store<T, HD>(a, s.first + rk, hk, lane, v, lk);
+      if (hd.L[k] == hd.L[k]) {
+        const int rk = kv_row_of(a, q0 + k), hk = use.g * a.G + q0 + k - rk * a.G;
+        float v[HD / 32], mk, lk;
+        kv_attn_row<T, HD>(c, a, use.b, s.first + rk, hk, s.e0 + rk, lane, v, mk, lk);
+        kv_store<T, HD>(a, s.first + rk, hk, lane, v, lk);
+      }
       __syncwarp();
       if (lane == 0) hd.odd[k] = 0;
     }

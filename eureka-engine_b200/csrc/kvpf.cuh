@@ -417,7 +417,20 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
     // rows whose result is no number once more, by themselves (kv_attn_row says why)
     float c0, c1;
     x2_unpack(x2_add(chk[0], chk[1]), c0, c1);
-    unsigned redo = __ballot_sync(0xffffffffu, p.splits == 1 && qi < NQ && !(fabsf(c0 + c1) < INFINITY));
+    bool again = p.splits == 1 && qi < NQ && l == l && !(fabsf(c0 + c1) < INFINITY);
+    if (__is_same(T, __half) && __any_sync(0xffffffffu, again)) {   // (NaN, or only infinities?)
+      bool nan = false;
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 32) {
+        float o[32];
+        kp_ld32(lq + C::O + (uint32_t)(x0 * HD + d), o);
+        t5_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; k++) nan |= kv_again<T>(o[k]);
+      }
+      again = again && nan;
+    }
+    unsigned redo = __ballot_sync(0xffffffffu, again);
     while (redo) {
       const int k = __ffs(redo) - 1, qk = q0 + 128 * x0 + 32 * (warp & 3) + k, rk = qk / a.G;
       redo &= redo - 1;

@@ -190,7 +190,7 @@ typedef struct {
 LLB_API int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a);
 /* Attention of a call's rows: the row at slot e sees slots j <= e, with window > 0 only those with j > e - window or j < sinks.
  * out = sum_j softmax_j(scale q . K_j) V_j for head h on kv head h / (heads / kv_heads), which must not overlap q; a row that sees nothing gets zeros.  K and V may
- * hold anything, infinities and NaN included, where a row does not see them.  Scores, softmax and sums are f32; the probabilities take
+ * hold anything, infinities and NaN included, where a row does not see them.  Scores (q . K_j before its scale, too), softmax and sums are f32; the probabilities take
  * part in the second product in the cache's type.
  * w_out (0: not wanted): w_out[b][g][j] = w_in[b][g][j] + the probabilities that slot j got, summed over the rows of the sequence and
  * the heads of kv head g, for j < lens[b]; other entries are left as they are.  w_in may be w_out, or 0 for zeros. */

@@ -217,3 +217,51 @@ def test_evict_of_a_sequence_whose_keys_have_no_room(llb, kind):
     for budget, sinks, recent in ((9000, 16, 500), (150000, 0, 0)):
         _evict(llb, c, budget, sinks, recent, w, page2=128)
     _clean(llb)
+
+
+def _best(llb, kv, a, times=5):
+    stream = torch.cuda.ExternalStream(llb.lib().llb_b200_stream())
+    best = math.inf
+    for _ in range(times):
+        t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        t[0].record(stream)
+        llb.kv_attn(kv, a)
+        t[1].record(stream)
+        t[1].synchronize()
+        best = min(best, t[0].elapsed_time(t[1]))
+    return best
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("rows,n,KV", [(1, 100000, 2), (1, 3000, 2), (3, 60000, 1), (700, 2000, 2)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_key_that_is_no_number_costs_no_time(llb, hd, rows, n, KV, bad):
+    """Rows that see it are NaN, as before it, in about the time of the same call without it (one slot after the other it is hundreds of times as much)."""
+    H = 2 * KV
+    c = Cache(llb, "bf16", KV, hd, 128, [n], seed=110)
+    r = _attn(llb, c, H, [rows], seed=111, behind=0)
+    before = _best(llb, *r["call"])
+    c.k[int(c.table[0, 0]), :, 7, 3] = bad
+    r["q"].abs_()                                      # (an infinite key's score is plus infinity)
+    after = _best(llb, *r["call"])
+    assert torch.isnan(r["out"]).all()
+    assert after < 4 * before + 0.02, (before, after)
+    _clean(llb)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("rows,n", [(1, 100000), (1, 3000), (3, 60000)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_an_infinite_value_that_every_row_sees(llb, hd, rows, n, bad):
+    """f16, where values beyond its range become infinite: that dimension is infinite, the others are as they were, in about the same time."""
+    c = Cache(llb, "f16", 2, hd, 128, [n], seed=121)
+    c.k[int(c.table[0, 0]), :, 7] = 0.0                # (scores of 0: probabilities above half a step of f16's smallest numbers)
+    r = _attn(llb, c, 4, [rows], seed=122, behind=0, scale=0.1)
+    want = r["out"].view(rows, 4, hd).clone()
+    before = _best(llb, *r["call"])
+    c.v[int(c.table[0, 0]), :, 7, 5] = bad
+    after = _best(llb, *r["call"])
+    want[:, :, 5] = bad
+    assert torch.equal(r["out"].view(rows, 4, hd), want)
+    assert after < 4 * before + 0.02, (before, after)
+    _clean(llb)
