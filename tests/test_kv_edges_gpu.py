@@ -265,3 +265,27 @@ def test_an_infinite_value_that_every_row_sees(llb, hd, rows, n, bad):
     assert torch.equal(r["out"].view(rows, 4, hd), want)
     assert after < 4 * before + 0.02, (before, after)
     _clean(llb)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 60000), (3, 20000), (300, 20000), (80, 3000)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_probabilities_below_the_smallest_f16(llb, hd, rows, n):
+    """One slot has nearly all of the weight and V = 0, the others exp(-17.5) = 2^-25.2 of it each and V = 1: what they add up to is the result.
+
+    Bounds.  A score of 17.5 is off by hd 2^-23 of it, its power of two by 2^-21 of itself.  A probability is rounded to f16 after a multiplication by
+    2^7 or more: 2^-11 of it, or half a step of 2^-24, which is 2^-32 of the largest.  Sums of n terms by n 2^-23; then the result's rounding."""
+    c = Cache(llb, "f16", 1, hd, 64, [n], seed=109)
+    c.k.fill_(0.0), c.v.fill_(1.0)
+    c.k[..., 0] = -17.5
+    p0 = int(c.table[0, 0])
+    c.k[p0, 0, 5], c.v[p0, 0, 5] = 0.0, 0.0
+    q = torch.zeros(rows, hd)
+    q[:, 0] = 1.0
+    r = _attn(llb, c, 1, [rows], q=q, scale=1.0, behind=0)
+    seen = torch.arange(n - rows + 1, n + 1, dtype=torch.float64) - 1
+    tail = seen * math.exp(-17.5)
+    want = tail / (1.0 + tail)
+    bound = want * (17.5 * hd * 2.0 ** -23 + 2.0 ** -20 + 2 * 2.0 ** -11 + n * 2.0 ** -22) + n * 2.0 ** -32 + 2.0 ** -25
+    d = (r["out"].double().cpu() - want[:, None]).abs()
+    assert torch.all(d <= bound[:, None]), (float(d.max()), float(want.max()), float(bound.max()))
+    _clean(llb)
