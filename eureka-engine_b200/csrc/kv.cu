@@ -464,6 +464,15 @@ struct KvScope {
   if (backend_graph_bail()) return -1
 
 static bool off(llb_b200_dptr p, unsigned n) { return p % n != 0; }
+// Whether `rows` rows of wa bytes, sa bytes apart from a on, may share a byte with rows of wb bytes, sb apart from b on.  Rows that lie beside each other in one buffer (equal
+// strides) do not.
+static bool rows_meet(llb_b200_dptr a, long long sa, long long wa, llb_b200_dptr b, long long sb, long long wb, long long rows) {
+  if (!a || !b || rows < 1 || wa < 1 || wb < 1) return false;
+  if (a + (unsigned long long)((rows - 1) * sa + wa) <= b || b + (unsigned long long)((rows - 1) * sb + wb) <= a) return false;
+  if (rows == 1 || sa != sb || wa > sa || wb > sb) return true;
+  const long long d = (long long)((b > a ? b - a : a - b) % (unsigned long long)sa), from_a = b > a || !d ? d : sa - d;   // where b's rows begin in a's
+  return from_a < wa || from_a + wb > sa;
+}
 static int kv_check(const llb_kv *kv, const char *what) {
   if (!kv) return llb_fail("%s: no cache", what);
   if (kv->el != LLB_EL_F16 && kv->el != LLB_EL_BF16) return llb_fail("%s: el %d (a cache is of f16 or bf16)", what, kv->el);
@@ -675,6 +684,10 @@ int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a) {
   if (!a->row_start || off(a->row_start, 4) || off(a->pos, 4)) return llb_fail("kv_append: row_start and pos are int32 on the device");
   KV_BEGIN;
   if (!a->rows) return 0;
+  const long long heads_w = (long long)kv->kv_heads * hd * es, qo_w = 2LL * a->heads * hd, qo_s = 2 * a->q_out_stride;
+  if (a->q && (rows_meet(a->q, a->q_stride * es, ((a->heads - 1LL) * a->q_head_stride + hd) * es, a->q_out, qo_s, qo_w, a->rows) ||
+               rows_meet(a->k, a->k_stride * es, heads_w, a->q_out, qo_s, qo_w, a->rows) || rows_meet(a->v, a->v_stride * es, heads_w, a->q_out, qo_s, qo_w, a->rows)))
+    return llb_fail("kv_append: q_out overlaps q, k or v");
   const KvDev c = kv_dev(kv, LLONG_MAX);
   const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, a->rows};
   KvAppend k;
@@ -705,6 +718,10 @@ int llb_b200_kv_attn(const llb_kv *kv, const llb_kv_attn *a) {
   KV_BEGIN;
   if (!a->rows && !a->w_out) return 0;
   const KvDev c = kv_dev(kv, a->max_len);
+  const long long row = (long long)a->heads * kv->head_dim, ow = a->el_out == LLB_EL_F32 ? 4 : 2;
+  if (rows_meet(a->q, 2 * a->q_stride, 2 * row, a->out, ow * a->out_stride, ow * row, a->rows)) return llb_fail("kv_attn: out overlaps q");
+  if (a->w_in != a->w_out && rows_meet(a->w_in, 4LL * a->w_stride, 4LL * c.cap, a->w_out, 4LL * a->w_stride, 4LL * c.cap, (long long)kv->seqs * kv->kv_heads))
+    return llb_fail("kv_attn: w_out overlaps w_in and is not w_in");
   const KvRows rw{(const int *)(uintptr_t)a->row_start, a->rows, most_rows(a)};
   KvAttn k;
   k.q = (const uint16_t *)(uintptr_t)a->q; k.out = (void *)(uintptr_t)a->out;
@@ -726,6 +743,8 @@ int llb_b200_kv_evict(const llb_kv *src, const llb_kv *dst, const llb_kv_evict *
   const size_t need = evict_ws(src, e);
   if (!e->kept && (!e->ws || off(e->ws, 16) || e->ws_bytes < need)) return llb_fail("kv_evict: a workspace of %zu bytes (%zu are needed, on a multiple of 16)", e->ws_bytes, need);
   KV_BEGIN;
+  if (rows_meet(src->lens, 4LL * src->seqs, 4LL * src->seqs, dst->lens, 4LL * src->seqs, 4LL * src->seqs, 1)) return llb_fail("kv_evict: dst's lens overlap src's");
+  if (rows_meet(e->w, 4LL * e->w_stride, 4LL * len, e->w_out, 4LL * e->w_out_stride, 4LL * most, (long long)src->seqs * src->kv_heads)) return llb_fail("kv_evict: w_out overlaps w");
   const KvDev c = kv_dev(src, e->max_len), d = kv_dev(dst, LLONG_MAX);
   KvEvict k;
   k.budget = e->budget; k.sinks = e->sinks; k.recent = e->recent;

@@ -184,7 +184,7 @@ typedef struct {
   llb_b200_dptr invfreq;             /* f64 [rope_dim / 2] */
   llb_b200_dptr row_start;
   llb_b200_dptr pos;                 /* int32 [seqs], the position of a sequence's first row; 0: a row's position is its slot */
-  llb_b200_dptr q_out;               /* [rows][q_out_stride], the cache's type */
+  llb_b200_dptr q_out;               /* [rows][q_out_stride], the cache's type; shares no memory with q, k or v */
   long long q_out_stride;            /* elements, heads * head_dim or more */
 } llb_kv_append;
 LLB_API int llb_b200_kv_append(const llb_kv *kv, const llb_kv_append *a);
@@ -203,7 +203,7 @@ typedef struct {
   llb_b200_dptr q, out;              /* [rows][stride], heads of head_dim side by side; q in the cache's type; 16-byte aligned */
   long long q_stride, out_stride;    /* elements, heads * head_dim or more, whole 16 bytes */
   llb_b200_dptr row_start;
-  llb_b200_dptr w_in, w_out;         /* f32 [seqs][kv_heads][w_stride]; heads / kv_heads * max_rows is 64 at most then */
+  llb_b200_dptr w_in, w_out;         /* f32 [seqs][kv_heads][w_stride], one and the same or apart; heads / kv_heads * max_rows is 64 at most then */
   int w_stride;                      /* max_len or more */
   llb_b200_dptr ws;                  /* llb_b200_kv_attn_ws bytes, 16-byte aligned; needed from the call's first kernel to its last: calls on the one stream can share it */
   size_t ws_bytes;
@@ -220,7 +220,7 @@ typedef struct {
   int max_len;                       /* the most slots of a sequence */
   llb_b200_dptr w;                   /* f32 [seqs][kv_heads][w_stride] */
   int w_stride;                      /* max_len or more */
-  llb_b200_dptr w_out;               /* f32 [seqs][kv_heads][w_out_stride], the kept slots' weights; 0: not wanted; not w */
+  llb_b200_dptr w_out;               /* f32 [seqs][kv_heads][w_out_stride], the kept slots' weights; 0: not wanted; apart from w */
   int w_out_stride;                  /* min(budget, max_len) or more */
   llb_b200_dptr kept;                /* int32 [seqs][kv_heads][kept_stride], the slots of src that were kept; 0: not wanted */
   int kept_stride;                   /* min(budget, max_len) or more */

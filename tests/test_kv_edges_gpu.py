@@ -289,3 +289,78 @@ def test_many_probabilities_below_the_smallest_f16(llb, hd, rows, n):
     d = (r["out"].double().cpu() - want[:, None]).abs()
     assert torch.all(d <= bound[:, None]), (float(d.max()), float(want.max()), float(bound.max()))
     _clean(llb)
+
+
+# ---- outputs over inputs -----------------------------------------------------------------------------------
+def _refused(llb, call, word):
+    with pytest.raises(llb.LlbError, match=word):
+        call()
+
+
+def _append_call(llb, c, x, out, rs, q=0, k=0, v=0, out_at=0, H=4, es=4, stride=None, out_stride=None):
+    stride = stride or x.stride(0)
+    w = c.KV * c.hd
+    return llb.KvAppend(rows=rs[1], heads=H, el_in=llb.EL["f32"], rope_dim=0, eps=1e-6, q=x.data_ptr() + es * q, k=x.data_ptr() + es * (k or H * c.hd), v=x.data_ptr() + es * (v or H * c.hd + w),
+                        q_stride=stride, k_stride=stride, v_stride=stride, q_head_stride=c.hd, row_start=rs[0].data_ptr(), q_out=out.data_ptr() + out_at, q_out_stride=out_stride or out.stride(0))
+
+
+def test_appended_queries_may_lie_beside_their_rows_and_not_over_them(llb):
+    c = Cache(llb, "bf16", 2, 64, 16, [5], seed=123)
+    H, R = 4, 5
+    rs = (_ints([0, R]), R)
+    wide = torch.zeros(R, 800, device="cuda")             # rows of 512 numbers, and 128 more words that 256 queries in 16 bits take
+    wide[:, :512] = torch.randn(R, 512, device="cuda")
+    apart = torch.zeros(R, 256, dtype=torch.bfloat16, device="cuda")
+    llb.kv_append(c.desc(), _append_call(llb, c, wide, apart, rs))
+    beside = wide.view(torch.bfloat16)
+    llb.kv_append(c.desc(), _append_call(llb, c, wide, beside, rs, out_at=4 * 512))
+    llb.check(llb.lib().llb_b200_sync(), "sync")
+    assert torch.equal(beside[:, 1024:1280], apart)
+    for at in (0, 4 * 255, 4 * 256, 4 * 511, 4 * 700, 4 * 800):      # over q, k, v, and over the next row's q
+        _refused(llb, lambda: llb.kv_append(c.desc(), _append_call(llb, c, wide, beside, rs, out_at=at)), "overlaps")
+    _refused(llb, lambda: llb.kv_append(c.desc(), _append_call(llb, c, wide, beside, rs, out_at=4 * 512, out_stride=1602)), "overlaps")
+    _clean(llb)
+
+
+def test_attention_over_its_queries_or_weights_is_refused(llb):
+    c = Cache(llb, "bf16", 2, 64, 16, [40, 30], seed=124)
+    r = _attn(llb, c, 4, [1, 1], seed=125, weights=True)
+    _check_attn(c, r)
+    kv, a = r["call"]
+    want = r["out"].clone(), r["w_out"].clone()
+    buf = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
+    buf[:, :256] = r["q"][:, :256]
+    a.q, a.q_stride, a.out_stride = buf.data_ptr(), 512, 512
+    for at in (16, 2 * 248, 2 * 264, 2 * 512):
+        a.out = buf.data_ptr() + at
+        _refused(llb, lambda: llb.kv_attn(kv, a), "out overlaps q")
+    a.out = buf.data_ptr() + 2 * 256
+    for d in (4, -4, 4 * (r["w_in"].shape[2] - 1)):
+        a.w_in = a.w_out + d
+        _refused(llb, lambda: llb.kv_attn(kv, a), "w_out overlaps")
+    a.w_in = r["w_in"].data_ptr()
+    r["w_out"].fill_(7.0)
+    llb.kv_attn(kv, a)
+    llb.check(llb.lib().llb_b200_sync(), "sync")
+    assert torch.equal(buf[:2, 256:], want[0][:2, :256]) and torch.equal(r["w_out"], want[1])
+    _clean(llb)
+
+
+def test_evictions_over_their_inputs_are_refused(llb):
+    c = Cache(llb, "bf16", 2, 64, 16, [300, 90], seed=126)
+    w = _weights(2, 2, 300, 127)
+    d, ids, w2, (src, dst, e, ws) = _evict(llb, c, 100, 4, 20, w)
+    want = w2[..., :100].clone()
+    for at in (4, 4 * 299, -4 * 50):
+        e.w_out = w.data_ptr() + at
+        _refused(llb, lambda: llb.kv_evict(src, dst, e), "w_out overlaps w")
+    both = torch.zeros(2, 2, 512, device="cuda")           # a head's weights, and the kept slots' behind them
+    both[..., :300] = w
+    e.w, e.w_stride, e.w_out, e.w_out_stride = both.data_ptr(), 512, both.data_ptr() + 4 * 300, 512
+    llb.kv_evict(src, dst, e)
+    llb.check(llb.lib().llb_b200_sync(), "sync")
+    for b, n in enumerate((100, 90)):
+        assert torch.equal(both[b, :, 300:300 + n], want[b, :, :n])
+    dst.lens = src.lens + 4
+    _refused(llb, lambda: llb.kv_evict(src, dst, e), "lens overlap")
+    _clean(llb)
