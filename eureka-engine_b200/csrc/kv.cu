@@ -66,11 +66,12 @@ __global__ void __launch_bounds__(256, ROW ? 2 : 1) k_kv_append(const KvDev c, c
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope >> 1, r = ROW ? blockIdx.x * 8 + warp : blockIdx.x;
   const int b = r < rw.rows ? kv_find(rw, c.seqs, r, lane) : -1;
   if (b < 0) return;                           // behind the last row, or row_start is not what it should be
-  const int slot = kv_len(c, b) - __ldcg(rw.start + b + 1) + r, pos = a.pos ? __ldcg(a.pos + b) + r - __ldcg(rw.start + b) : slot;
+  const int slot = kv_len(c, b) - __ldcg(rw.start + b + 1) + r;
+  const double pos = a.pos ? (double)__ldcg(a.pos + b) + (r - __ldcg(rw.start + b)) : slot;   // (a first position near 2^31 has later ones above it)
   const int id = slot >= 0 ? kv_page(c, b, slot >> c.page_sh) : -1;
 #pragma unroll 1
   for (int p = lane; p < half; p += 32) {
-    const double n = (double)pos * __ldg(a.invfreq + p) * 0.15915494309189533577;   // turns
+    const double n = pos * __ldg(a.invfreq + p) * 0.15915494309189533577;   // turns
     float s, co;
     sincospif((float)(2.0 * (n - rint(n))), &s, &co);
     turn[warp][p] = make_float2(co, s);

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_kv_gpu import DT, HALF, TINY, Cache, _attn, _check_attn, _clean, _evict, _ints, _weights
+from test_kv_gpu import Cache, _append, _attn, _check_attn, _clean, _evict, _ints, _weights
 
 pytestmark = pytest.mark.gpu
 
@@ -363,4 +363,12 @@ def test_evictions_over_their_inputs_are_refused(llb):
         assert torch.equal(both[b, :, 300:300 + n], want[b, :, :n])
     dst.lens = src.lens + 4
     _refused(llb, lambda: llb.kv_evict(src, dst, e), "lens overlap")
+    _clean(llb)
+
+
+@pytest.mark.parametrize("rows", [[30, 40], [3000, 1]])
+def test_positions_that_pass_the_largest_int(llb, rows):
+    """A sequence's first row is at a position that an int holds, the rows behind it are where they are."""
+    c = Cache(llb, "f16", 1, 64, 64, rows, seed=128)
+    _append(llb, c, 1, rows, "f32", seed=129, pos=[2 ** 31 - 10, 2 ** 31 - 1], behind=0)
     _clean(llb)
