@@ -195,7 +195,8 @@ __device__ __forceinline__ uint32_t kv_key(float w) {
 // (eleven, eleven and ten bits; counts in shared memory, summed over the cluster; a warp's zeros are counted together, and so are those that are like its first other
 // weight: many are zero, or all alike), then the slots above it and the first of those that equal it, in order.  The keys are kept in shared memory where they have
 // room, so that the weights are read once. A cluster of four against one block, with the
-// copies: 4 sequences of up to 60000 slots, 4 heads of 256, 54 us and 158; 16 of 20000 119 and 126; 16 of 8000 45 and 40, so that shorter ones take one block.
+// copies: 4 sequences of up to 60000 slots, 4 heads of 256, 54 us and 158; 16 of 20000 119 and 126; 16 of 8000 45 and 40, so that shorter ones take one block.  (The rule looks at the
+// length alone.  One sequence of 10000 slots, 2 heads of 128: 17 and 20; 64 of 10000, 8 heads: 326 and 238.)
 #define KE_THREADS 1024
 #define KE_CLUSTER 4           // blocks of a head where sequences may have more than
 #define KE_LONG 12288          // slots
@@ -421,7 +422,8 @@ int kv_pf_bar_count(int hd, int bar) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-// Every kernel is loaded here: one that is first met while a stream is being captured may not be.
+// Every kernel is loaded here: one that is first met while a stream is being captured may not be.  (78 instances: llb_b200_init takes 4 to 15 ms more of some 40, and 4 MiB of the
+// device's memory.)
 template <typename K> static int kv_load(K k, int smem = 0) {
   if (smem) CU_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaFuncAttributes at;
@@ -529,8 +531,18 @@ static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int 
   return r == CUDA_SUCCESS ? 0 : llb_fail("kv: tensor map of %d pages: error %d", kv->n_pages, (int)r);
 }
 // ---- which kernel, and its workspace ----
-#define KV_FEW 64              // queries a kv head up to which a call goes to k_kv_few
-#define KF_LEAST 2             // fewest groups of a block's stretch
+// Queries a kv head up to which a call goes to k_kv_few, which alone gives slots' weights (64 queries at most).  It brings K and V once for every 16 queries, k_kv_pf once for 128
+// or 256.  Both kernels, us, k_kv_few first; 8 queries a kv head, 16, 32, 64:
+//   16 sequences of 8000 slots, 8 kv heads of 128, pages of 64:      95, 92   102, 92   183, 93   348, 95      window 2048: 39, 33   46, 39   75, 39   127, 38
+//   2 of 30000, the same heads:                                      52, 56    53, 56    89, 58   129, 60
+//   16 of 8000, 2 kv heads of 256, pages of 64:                      57, 56    60, 58    98, 61   176, 63      window 2048: 23, 21   26, 24   34, 25    53, 28
+//   1 of 1500, 8 kv heads of 128; 2 of 256:                          11, 20    11, 20    12, 20    14, 20;                  18, 19   20, 20   20, 20    20, 21
+// Up to 16 queries the two are near each other, and k_kv_few is ahead where few blocks have work; for 17 to 64 queries without weights a border at 16 would be faster but for short
+// contexts.
+#define KV_FEW 64
+// Fewest groups of a block's stretch.  One token, us, with one, two and four: 700 slots, 2 kv heads of 128: 9.7, 11.4, 12.9; 4 of 256: 14.3, 12.5, 14.8; 4000 slots 13.5, 12.9, 13.5
+// and 19.7, 19.6, 19.6; four sequences of 300, 2 of 128: 9.6, 11.6, 13.2; 4 of 256: 11.5, 11.5, 14.5
+#define KF_LEAST 2
 static int most_rows(const llb_kv_attn *a) { return std::min(a->max_rows, std::max(a->rows, 1)); }
 static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * most_rows(a) <= KV_FEW; }
 static_assert(KJ_SLOTS <= 2048 && (KV_MOST + 2047LL) / 2048 * 2048 <= INT_MAX, "a joining block's last slot");

@@ -19,8 +19,8 @@
 // products in line.  Every wait is bounded.
 //
 // Measured, cycles of a step of 64 slots: at head dimension 256 about 1370, of which the products are 16 x 33 + 4 x 130; at 128 (two streams) about 1900, products 2 x (8 x 48 + 4 x 64):
-// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 122 us, 0.91 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
-// heads of 128 on 8: 152 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
+// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 121 us, 0.92 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
+// heads of 128 on 8: 151 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
 #pragma once
 #include "kvatt.cuh"
 
