@@ -554,6 +554,7 @@ static size_t few_plan(const llb_kv *kv, const llb_kv_attn *a, uintptr_t base, K
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 15) & ~(size_t)15; return base + was; };
   p->blocks = (int)blocks; p->least = KF_LEAST;
   p->unit = (int *)take((size_t)kv->seqs * kv->kv_heads * (((size_t)(a->heads / kv->kv_heads) * most_rows(a) + 15) / 16) * 8);
+  p->span = (int2 *)take(blocks * 2 * 8);
   p->pm = (float *)take(blocks * 2 * 16 * 4);
   p->pl = (float *)take(blocks * 2 * 16 * 4);
   p->po = (float *)take(blocks * 2 * 16 * kv->head_dim * 4);

@@ -160,47 +160,46 @@ __device__ __forceinline__ float kv_warp_sum(float v) {
 // Whether a sum of products may be none of the row's: NaN, and in bf16 infinity too (V near 2^127 times probabilities relative to an old maximum; f16 has no
 // values whose sums overflow, an infinity comes from a slot that the row sees)
 template <typename T> __device__ __forceinline__ bool kv_again(float x) { return __is_same(T, __half) ? x != x : !(fabsf(x) < INFINITY); }
-// The row at slot e and head h over the slots that it sees, in their order, by a warp; lane's dimensions E lane ..
-// The attention kernels take a row to it whose sum of probabilities is a number and whose result is none: their products multiply V by a probability of zero where a
-// row does not see a slot that another one does, which is NaN where that slot holds an infinity or NaN.  (Where the sum is no number, a score that the row sees is
-// NaN or plus infinity, and so is every dimension of the result: nothing to do again.)
-// A token behind 100000 slots, 4 heads of 128: a NaN key, or an infinite V in f16, 37 us as without it (58 and 60 ms when such rows came here); a NaN in V alone, or an
-// infinite V in bf16, comes here and takes 48 ms.  Two slots' K and V on their way at once: with four the join of 16 x 4 rows is 1.3 us slower though no row comes here.
+// Chunks c0 .. c1 - 1, of 1 << sh slots, of what several rows see: the first cs of them of first tokens, then those from number lo on (KvSeq, KpTiles).
+struct KvSpan { int c0, c1, cs, lo, sh; };
+// What the row at slot e and head h sees of a span, slot after slot, by a warp; lane's dimensions E lane ..  o, m, l: the sums, relative to 2^m.
+// The attention kernels take a row to it, or the part of it that one block had, whose sum of probabilities is a number and whose result is none: their products multiply
+// V by a probability of zero where a row does not see a slot that another one does, which is NaN where that slot holds an infinity or NaN.  (Where the sum is no number, a
+// score that the row sees is NaN or plus infinity, and so is every dimension of the result: nothing to do again.)
+// A token behind 100000 slots, 4 heads of 128: a NaN key, or an infinite V in f16, 37 us as without it (58 and 60 ms when such rows were done again, wholly).
+// Inlined: as a function of its own, though no row comes to it, it cost the kernels the registers and the order of their code that a call asks for (48 sequences of up to 6000
+// slots with weights 159 us for 134, 3011 rows of 24 heads of 256 106 for 102, 4 x up to 2000 rows of 32 heads of 128 148 for 133).
 template <typename T, int HD>
-__device__ __noinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float *o, float &m, float &l) {
-  constexpr int E = HD / 32, U = 2;
-  const int g = h / a.G, pm = (1 << c.page_sh) - 1;
+__device__ __forceinline__ void kv_attn_row(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, const KvSpan &sp, int lane, float (&o)[HD / 32], float &m, float &l) {
+  constexpr int E = HD / 32;
+  const int g = h / a.G, pm = (1 << c.page_sh) - 1, lw = a.window ? kv_before(e, a.window) + 1 : 0;
   float q[E];
   kv_row_in<T, E>((const T *)a.q + r * a.qs + (long long)h * HD + lane * E, q);
 #pragma unroll
   for (int i = 0; i < E; i++) { q[i] *= a.scale2; o[i] = 0.0f; }
   m = -INFINITY; l = 0.0f;
-  const int lo = kv_first(e, a.window), ns = min(a.sinks, lo), all = ns + e + 1 - lo;
   int id = -1, at = -1;
 #pragma unroll 1
-  for (int n0 = 0; n0 < all; n0 += U) {
-    uint32_t k[U][E / 2], v[U][E / 2];
-    bool on[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int n = n0 + u, j = n < ns ? n : lo + n - ns;
-      if (n < all && j >> c.page_sh != at) { at = j >> c.page_sh; id = kv_page(c, b, at); }
-      on[u] = n < all && id >= 0;
-      const size_t p = on[u] ? kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + lane * E : 0;
-      if (on[u]) { kv_words<E / 2>(c.k + p, k[u]); kv_words<E / 2>(c.v + p, v[u]); }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (!on[u]) continue;
+  for (int ch = sp.c0; ch < sp.c1; ch++) {
+    const int j0 = (ch < sp.cs ? ch : sp.lo + ch - sp.cs) << sp.sh;
+#pragma unroll 1
+    for (int j = j0; j < j0 + (1 << sp.sh); j++) {
+      if (j > e || (j < lw && j >= a.sinks)) continue;
+      if (j >> c.page_sh != at) { at = j >> c.page_sh; id = kv_page(c, b, at); }
+      if (id < 0) continue;
+      const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + lane * E;
+      float k[E], v[E];
+      kv_row_in<T, E>((const T *)c.k + p, k);
+      kv_row_in<T, E>((const T *)c.v + p, v);
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<T>::to2(k[u][i]); s += q[2 * i] * f.x; s += q[2 * i + 1] * f.y; }
+      for (int i = 0; i < E; i++) s += q[i] * k[i];
       s = kv_warp_sum(s);
       const float mn = fmaxf(m, s), cf = m == -INFINITY ? 0.0f : exp2f(m - mn), w = s == -INFINITY ? 0.0f : exp2f(s - mn);
       l = l * cf + w;
       // (0 times an infinity is no number either: a slot that is seen and whose probability is 0 counts as in the definition, exp(s) V)
 #pragma unroll
-      for (int i = 0; i < E / 2; i++) { const float2 f = KvEl<T>::to2(v[u][i]); o[2 * i] = o[2 * i] * cf + w * f.x; o[2 * i + 1] = o[2 * i + 1] * cf + w * f.y; }
+      for (int i = 0; i < E; i++) o[i] = o[i] * cf + w * v[i];
       m = mn;
     }
   }
@@ -218,12 +217,18 @@ template <typename T, int HD> __device__ __forceinline__ void kv_store(const KvA
     for (int i = 0; i < E; i += 2) *(float2 *)(p + i) = make_float2(o[i], o[i + 1]);
   } else kv_row_out<T, E>((uint16_t *)a.out + at, true, o);
 }
-// ... from its sums (base 2: m the maximum that l and o are relative to)
-template <typename T, int HD>
-__device__ __forceinline__ void kv_finish(const KvDev &c, const KvAttn &a, int b, int r, int h, int e, int lane, float (&o)[HD / 32], float m, float l) {
+// one more part's sums (relative to 2^pm) to a row's
+template <int E> __device__ __forceinline__ void kv_add_part(float (&o)[E], float &m, float &l, const float (&v)[E], float pm, float pl) {
+  const float t = fmaxf(m, pm), ref = t == -INFINITY ? 0.0f : t, f = exp2f(m - ref), fp = exp2f(pm - ref);
+  l = l * f + pl * fp;
+  m = t;
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] = o[i] * f + v[i] * fp;
+}
+// whether a row's sums may be none of its own (l a number, o none): the whole warp
+template <typename T, int E> __device__ __forceinline__ bool kv_again_any(const float (&o)[E], float l) {
   bool again = false;
 #pragma unroll
-  for (int i = 0; i < HD / 32; i++) again |= kv_again<T>(o[i]);
-  if (__any_sync(0xffffffffu, again) && l == l) kv_attn_row<T, HD>(c, a, b, r, h, e, lane, o, m, l);
-  kv_store<T, HD>(a, r, h, lane, o, l);
+  for (int i = 0; i < E; i++) again |= kv_again<T>(o[i]);
+  return __any_sync(0xffffffffu, again) && l == l;
 }

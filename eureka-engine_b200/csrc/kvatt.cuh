@@ -48,6 +48,7 @@ struct KvPlan {
   int blocks;                  // of k_kv_few
   int least;                   // groups of a block's stretch, at least
   int *unit;                   // [seqs][KV][16-query tiles][2]: the first and the last block that had a part of the unit
+  int2 *span;                  // [2 blocks]: the groups of its unit that a part has, from and to
   float *pm, *pl, *po;         // [2 blocks][16](, [hd])
   float *sc;                   // [seqs][KV][G max_rows][sstride]: scores, where weights are wanted
   float *lse;                  // [seqs][KV][G max_rows]: of units that one block has wholly
@@ -109,6 +110,8 @@ template <int SH> struct KfWalk {
     return true;
   }
 };
+
+__device__ __forceinline__ KvSpan kf_span(const KvSeq &s, int c0, int c1, int sh) { return {c0, c1, s.cs, s.lo >> sh, sh}; }
 
 template <typename T, int HD, bool WT>
 __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, const __grid_constant__ CUtensorMap km,
@@ -392,6 +395,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       int *u = p.unit + (((size_t)use.b * c.KV + use.g) * ((a.G * rw.max_rows + 15) >> 4) + use.qt) * 2;
       if (use.c0 == 0) u[0] = blockIdx.x;
       if (use.c1 == s.chunks) u[1] = blockIdx.x;
+      p.span[blockIdx.x * 2 + (use.c0 == 0)] = make_int2(use.c0, use.c1);
     }
     const size_t part = ((size_t)blockIdx.x * 2 + (use.c0 == 0)) * 16;
     const int nr = min(16, NQ - q0);
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
       if (hd.L[k] == hd.L[k]) {
         const int rk = kv_row_of(a, q0 + k), hk = use.g * a.G + q0 + k - rk * a.G;
         float v[HD / 32], mk, lk;
-        kv_attn_row<T, HD>(c, a, use.b, s.first + rk, hk, s.e0 + rk, lane, v, mk, lk);
+        kv_attn_row<T, HD>(c, a, use.b, s.first + rk, hk, s.e0 + rk, kf_span(s, 0, s.chunks, SH), lane, v, mk, lk);
         kv_store<T, HD>(a, s.first + rk, hk, lane, v, lk);
       }
       __syncwarp();
@@ -477,10 +481,10 @@ __host__ __device__ __forceinline__ int kf_parts_of(int first, int last, int blo
 __device__ __forceinline__ size_t kf_part(int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }
 
 // Units that several blocks had: a block a query, its four warps the parts in turn, each with what it needs of them asked for at once.  Blocks from
-// `joins` on: what every slot got, KJ_SLOTS of a kv head each.
+// `joins` on: what every slot got, KJ_SLOTS of a kv head each.  (Eight blocks an SM: with six, 16 x 4 rows of 16 heads, 1024 blocks, take 1.7 us more.)
 #define KJ_SLOTS 2048
 template <typename T, int HD, bool WT>
-__global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
+__global__ void __launch_bounds__(128, WT ? 4 : 8) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
   constexpr int E = HD / 32;
   __shared__ float sm[4], sl[4], so[4][HD], lse[64];
   pdl_trigger();
@@ -523,8 +527,25 @@ __global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw,
 #pragma unroll
       for (int i = 0; i < 4; i++) o[k] += so[i][lane * E + k] * f[i];
     }
-    const int row = kv_row_of(a, qi);
-    kv_finish<T, HD>(c, a, b, s.first + row, g * a.G + qi - row * a.G, s.e0 + row, lane, o, M, l);
+    const int row = kv_row_of(a, qi), h = g * a.G + qi - row * a.G;
+    if (kv_again_any<T, E>(o, l)) {                        // the parts whose sums are no numbers once more, by themselves
+      m = -INFINITY; l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < E; k++) o[k] = 0.0f;
+#pragma unroll 1
+      for (int i = w.x; i <= w.y; i++) {
+        const size_t at = kf_part(i, w.x) + (qi & 15);
+        float pm = __ldcg(p.pm + at), pl = __ldcg(p.pl + at), v[E];
+#pragma unroll
+        for (int k = 0; k < E; k += 2) { const float2 t = __ldcg((const float2 *)(p.po + at * HD + lane * E + k)); v[k] = t.x; v[k + 1] = t.y; }
+        if (kv_again_any<T, E>(v, pl)) {
+          const int2 part = __ldcg(p.span + 2 * i + (i == w.x));
+          kv_attn_row<T, HD>(c, a, b, s.first + row, h, s.e0 + row, kf_span(s, max(part.x, 0), min(part.y, s.chunks), kf_sh(HD)), lane, v, pm, pl);
+        }
+        kv_add_part<E>(o, m, l, v, pm, pl);
+      }
+    }
+    kv_store<T, HD>(a, s.first + row, h, lane, o, l);
     return;
   }
   if constexpr (WT) {

@@ -36,6 +36,8 @@ template <int HD> struct Kp {
 };
 static_assert(Kp<256>::SMEM <= 232448 && Kp<128>::SMEM <= 232448 && Kp<64>::SMEM <= 232448, "shared memory");
 
+template <typename T> constexpr float kp_up = __is_same(T, __half) ? 7.0f : 0.0f;   // P, and so a stream's sums, are taken times two to this
+
 struct KvPfPlan {
   int splits;                  // blocks a unit's tiles of slots are spread over
   float *pm, *pl, *po;         // [seqs][KV][queries][splits](, [hd]), where there are several; queries: G max_rows
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
           t5_wait_st();
         }
       }
-      const float ref = (m == -INFINITY ? 0.0f : -m) + (__is_same(T, __half) ? 7.0f : 0.0f);   // (P as the comment at the top has it)
+      const float ref = (m == -INFINITY ? 0.0f : -m) + kp_up<T>;
       const f32x2 sc2 = x2_pack(a.scale2, a.scale2), rf2 = x2_pack(ref, ref);
       f32x2 sum[2] = {0, 0};
 #pragma unroll
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       const int k = __ffs(redo) - 1, qk = q0 + 128 * x0 + 32 * (warp & 3) + k, rk = qk / a.G;
       redo &= redo - 1;
       float o[HD / 32], mk, lk;
-      kv_attn_row<T, HD>(c, a, b, s.first + rk, g * a.G + qk % a.G, s.e0 + rk, lane, o, mk, lk);
+      kv_attn_row<T, HD>(c, a, b, s.first + rk, g * a.G + qk % a.G, s.e0 + rk, {0, kt.n, kt.cs, kt.lo, SH}, lane, o, mk, lk);
       kv_store<T, HD>(a, s.first + rk, g * a.G + qk % a.G, lane, o, lk);
     }
   } else if (warp < C::SOFT) {
@@ -584,5 +586,27 @@ __global__ void __launch_bounds__(128) k_kv_pf_join(const KvDev c, const KvRows 
 #pragma unroll
     for (int k = 0; k < E; k += 2) { const float2 v = __ldcg((const float2 *)(p.po + (at + w) * HD + lane * E + k)); o[k] += v.x * f; o[k + 1] += v.y * f; }
   }
-  kv_finish<T, HD>(c, a, b, r, h, kv_len(c, b) - n + i, lane, o, M, l);
+  if (kv_again_any<T, E>(o, l)) {                          // the splits whose sums are no numbers once more, by themselves
+    constexpr int QT = 128 * Kp<HD>::NQT, SH = Kp<HD>::SH;
+    const int e0 = kv_len(c, b) - n, NQ = a.G * min(n, rw.max_rows), q0 = (i * a.G + h % a.G) / QT * QT;
+    const KpTiles kt = kp_tiles<SH>(e0 + kv_row_of(a, q0), e0 + kv_row_of(a, min(q0 + QT - 1, NQ - 1)), a.window, a.sinks);
+    const int per = (kt.n + p.splits - 1) / p.splits;
+    M = -INFINITY; l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; k++) o[k] = 0.0f;
+#pragma unroll 1
+    for (int w = 0; w < p.splits; w++) {
+      float pm = __ldcg(p.pm + at + w), pl = __ldcg(p.pl + at + w), v[E];
+      if (pm == -INFINITY) continue;
+#pragma unroll
+      for (int k = 0; k < E; k += 2) { const float2 t = __ldcg((const float2 *)(p.po + (at + w) * HD + lane * E + k)); v[k] = t.x; v[k + 1] = t.y; }
+      if (kv_again_any<T, E>(v, pl)) {
+        const int t0 = min(kt.n, w * per);
+        kv_attn_row<T, HD>(c, a, b, r, h, e0 + i, {t0, min(kt.n, t0 + per), kt.cs, kt.lo, SH}, lane, v, pm, pl);
+        pm += kp_up<T>;                                    // (as the others' sums are)
+      }
+      kv_add_part<E>(o, M, l, v, pm, pl);
+    }
+  }
+  kv_store<T, HD>(a, r, h, lane, o, l);
 }

@@ -372,3 +372,27 @@ def test_positions_that_pass_the_largest_int(llb, rows):
     c = Cache(llb, "f16", 1, 64, 64, rows, seed=128)
     _append(llb, c, 1, rows, "f32", seed=129, pos=[2 ** 31 - 10, 2 ** 31 - 1], behind=0)
     _clean(llb)
+
+
+@pytest.mark.parametrize("el", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,n,H,KV,hd", [(4, 60000, 2, 1, 128), (4, 60000, 8, 2, 256), (5, 30000, 4, 4, 64), (100, 60000, 2, 1, 128), (100, 40000, 2, 1, 256), (80, 30000, 2, 2, 64)])
+def test_a_row_that_is_no_number_behind_a_long_sequence(llb, rows, n, H, KV, hd, el):
+    """K and V of a call's own last row are NaN: the rows before it are what they are without it, and only the part of their slots that holds it is looked at once more."""
+    c = Cache(llb, el, KV, hd, 128, [n], seed=130)
+    r = _attn(llb, c, H, [rows], seed=131, behind=0)
+    want = r["out"].clone()
+    before = _best(llb, *r["call"])
+    j = n - 1
+    for pool in (c.k, c.v):
+        pool[int(c.table[0, j // 128]), :, j % 128] = math.nan
+    after = _best(llb, *r["call"])
+    assert torch.isnan(r["out"][rows - 1]).all()
+    r["out"][rows - 1] = 7.0
+    r["rows"], r["start"] = [rows - 1], [0, rows - 1]
+    c.lens_list, c.K, c.V = [n - 1], [c.K[0][:-1]], [c.V[0][:-1]]
+    _check_attn(c, r)
+    # a part of 148 of the slots, at most 32 rows of it one after the other, each slot about 0.5 us
+    part = -(-n * KV // 148) + 512
+    assert after < 4 * before + 1e-3 * part * (1 if rows < 8 else 32), (before, after)
+    assert torch.equal(torch.isnan(want), torch.zeros_like(want, dtype=torch.bool))
+    _clean(llb)
