@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
         piece(2 * d);
       }
     }
-    // rows whose result is no number once more, by themselves (kv_attn_row says why)
+    // rows whose result is no number once more (kv_attn_row says why)
     float c0, c1;
     x2_unpack(x2_add(chk[0], chk[1]), c0, c1);
     bool again = p.splits == 1 && qi < NQ && l == l && !(fabsf(c0 + c1) < INFINITY);
@@ -435,14 +435,10 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       }
       again = again && nan;
     }
-    unsigned redo = __ballot_sync(0xffffffffu, again);
-    while (redo) {
-      const int k = __ffs(redo) - 1, qk = q0 + 128 * x0 + 32 * (warp & 3) + k, rk = qk / a.G;
-      redo &= redo - 1;
-      float o[HD / 32], mk, lk;
-      kv_attn_row<T, HD>(c, a, b, s.first + rk, g * a.G + qk % a.G, s.e0 + rk, {0, kt.n, kt.cs, kt.lo, SH}, lane, o, mk, lk);
-      kv_store<T, HD>(a, s.first + rk, g * a.G + qk % a.G, lane, o, lk);
-    }
+    const unsigned redo = __ballot_sync(0xffffffffu, again);
+#pragma unroll 1
+    for (int half = 0; redo && half < 32; half += 16)
+      if (redo >> half & 0xffff) kv_attn_rows16<T, HD>(c, a, b, g, s.first, s.e0, q0 + 128 * x0 + 32 * (warp & 3) + half, NQ, {0, kt.n, kt.cs, kt.lo, SH}, lane, redo >> half & 0xffff);
   } else if (warp < C::SOFT) {
     if (lane == 0) mbar_arrive(q_full);          // the second query tile is behind the last query
   } else if (warp < C::SOFT + 2) {

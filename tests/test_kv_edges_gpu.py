@@ -396,3 +396,36 @@ def test_a_row_that_is_no_number_behind_a_long_sequence(llb, rows, n, H, KV, hd,
     assert after < 4 * before + 1e-3 * part * (1 if rows < 8 else 32), (before, after)
     assert torch.equal(torch.isnan(want), torch.zeros_like(want, dtype=torch.bool))
     _clean(llb)
+
+
+@pytest.mark.parametrize("el,bad", [("bf16", math.nan), ("f16", math.nan), ("bf16", math.inf), ("f16", -math.inf)])
+@pytest.mark.parametrize("rows,lens,H,KV,hd,window", [([1200], [1500], 16, 8, 256, 0), ([1200], [1500], 32, 16, 128, 0), ([700, 300], [1100, 420], 64, 16, 64, 200),
+                                                      ([4] * 40, [300 + 7 * b for b in range(40)], 16, 8, 128, 0), ([3] * 40, [500] * 40, 24, 4, 256, 100), ([15, 2] * 60, [90, 300] * 60, 4, 4, 64, 33)])
+def test_rows_in_front_of_a_row_that_is_no_number(llb, rows, lens, H, KV, hd, window, el, bad):
+    """In the middle of the first sequence's rows K and V are no numbers: what is in front of it is right, and so are all other sequences; in a few times the call's time (one row
+    and one slot after the other it is hundreds)."""
+    c = Cache(llb, el, KV, hd, 16, lens, seed=132)
+    r = _attn(llb, c, H, rows, seed=133, window=window, behind=0)
+    before = _best(llb, *r["call"])
+    at = rows[0] // 2                                      # (row `at` and those behind it see that slot)
+    j = lens[0] - rows[0] + at
+    for pool in (c.k, c.v):
+        pool[int(c.table[0, j // 16]), :, j % 16] = bad
+    after = _best(llb, *r["call"])
+    end = rows[0] if not window else min(rows[0], at + window)
+    if bad != bad:
+        assert torch.isnan(r["out"][at:end]).all()
+    r["out"][at:end] = 7.0
+    r["start"] = [0] + r["start"][1:]
+    # the rows in front, as a sequence that ends before the slot; the others as they are
+    keep = c.lens_list, c.K, c.V, r["rows"]
+    c.lens_list, c.K, c.V, r["rows"] = [j], [c.K[0][:j]], [c.V[0][:j]], [at]
+    full, start = r["out"], r["start"]
+    r["out"], r["start"] = full[:at], [0, at]
+    _check_attn(c, r)
+    c.lens_list, c.K, c.V, r["rows"] = list(keep[0][1:]), keep[1][1:], keep[2][1:], keep[3][1:]
+    if r["rows"]:
+        r["out"], r["q"], r["start"] = full[rows[0]:], r["q"][rows[0]:], [s - rows[0] for s in start[1:]]
+        _check_attn(c, r)
+    assert after < 8 * before + 1.5, (before, after)
+    _clean(llb)
