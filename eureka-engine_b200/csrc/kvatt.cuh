@@ -115,14 +115,13 @@ __device__ __forceinline__ KvSpan kf_span(const KvSeq &s, int c0, int c1, int sh
 
 // The same as kv_attn_row for 16 queries of kv head g from q0 on (query i G + h: row i, head h; `first` and e0: the sequence's first row and its slot), 16 slots at a time,
 // stored where `rows` has the query's bit: scores by products (a key that is no number is one column of them), V added up in f32 by those that see its slot alone.
-// 3000 rows of 4 heads of 256 on 2 whose middle one has a V of NaN: 3.6 ms, and 39 ms row by row and slot by slot (47 us where all is numbers).
+// 3000 rows of 4 heads of 256 on 2 whose middle one has a V of NaN: 5.6 ms, and 39 ms row by row and slot by slot (47 us where all is numbers).
 template <typename T, int HD>
 __device__ __forceinline__ void kv_attn_rows16(const KvDev &c, const KvAttn &a, int b, int g, int first, int e0, int q0, int NQ, const KvSpan &sp, int lane, unsigned rows) {
   const int gid = lane >> 2, j2 = 2 * (lane & 3), pm = (1 << c.page_sh) - 1;
   const uint16_t *q[2];
   long long at[2];                                         // the lane's two queries: gid and gid + 8
   int e[2], lw[2];
-  float o[HD / 8][4], m[2], l[2];
 #pragma unroll
   for (int w = 0; w < 2; w++) {
     const int qi = min(q0 + gid + 8 * w, NQ - 1), row = kv_row_of(a, qi);
@@ -131,88 +130,90 @@ __device__ __forceinline__ void kv_attn_rows16(const KvDev &c, const KvAttn &a, 
     at[w] = r * a.os + h + j2;
     e[w] = e0 + row;
     lw[w] = a.window ? kv_before(e[w], a.window) + 1 : 0;
-    m[w] = -INFINITY; l[w] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < HD / 8; t++) o[t][2 * w] = o[t][2 * w + 1] = 0.0f;
   }
   auto sees = [&](int w, int j) { return j <= e[w] && (j >= lw[w] || j < a.sinks); };
+  constexpr int DN = HD == 256 ? 16 : HD / 8;              // eight dims at a time: at head dimension 256 half of them (the registers are the attention kernel's too)
 #pragma unroll 1
-  for (int ch = sp.c0; ch < sp.c1; ch++) {
-    const int j0 = (ch < sp.cs ? ch : sp.lo + ch - sp.cs) << sp.sh;
+  for (int d0 = 0; d0 < HD; d0 += 8 * DN) {
+    float o[DN][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll 1
-    for (int j = j0; j < j0 + (1 << sp.sh); j += 16) {
-      bool on[2][4], any = false;                          // [query][slots j + j2, j + j2 + 1, and eight on]
+    for (int ch = sp.c0; ch < sp.c1; ch++) {
+      const int j0 = (ch < sp.cs ? ch : sp.lo + ch - sp.cs) << sp.sh;
+#pragma unroll 1
+      for (int j = j0; j < j0 + (1 << sp.sh); j += 16) {
+        bool on[2][4], any = false;                          // [query][slots j + j2, j + j2 + 1, and eight on]
 #pragma unroll
-      for (int i = 0; i < 8; i++) any |= on[i >> 2][i & 3] = sees(i >> 2, j + j2 + (i & 1) + 8 * ((i >> 1) & 1));
-      if (!__any_sync(0xffffffffu, any)) continue;
-      const int id = kv_page(c, b, j >> c.page_sh);        // (16 slots: one page's)
-      if (id < 0) continue;
-      const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + j2;
-      float x[2][4] = {};
+        for (int i = 0; i < 8; i++) any |= on[i >> 2][i & 3] = sees(i >> 2, j + j2 + (i & 1) + 8 * ((i >> 1) & 1));
+        if (!__any_sync(0xffffffffu, any)) continue;
+        const int id = kv_page(c, b, j >> c.page_sh);        // (16 slots: one page's)
+        if (id < 0) continue;
+        const size_t p = kv_at(c, id, g, HD) + (size_t)(j & pm) * HD + j2;
+        float x[2][4] = {};
 #pragma unroll 2
-      for (int d = 0; d < HD; d += 16) {
-        const uint32_t qa[4] = {__ldcg((const uint32_t *)(q[0] + d)), __ldcg((const uint32_t *)(q[1] + d)), __ldcg((const uint32_t *)(q[0] + d + 8)), __ldcg((const uint32_t *)(q[1] + d + 8))};
+        for (int d = 0; d < HD; d += 16) {
+          const uint32_t qa[4] = {__ldcg((const uint32_t *)(q[0] + d)), __ldcg((const uint32_t *)(q[1] + d)), __ldcg((const uint32_t *)(q[0] + d + 8)), __ldcg((const uint32_t *)(q[1] + d + 8))};
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const uint16_t *k = c.k + p + (8 * t + gid) * HD + d;
+            kf_mma<T>(x[t], qa, __ldcg((const uint32_t *)k), __ldcg((const uint32_t *)(k + 8)));
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          float t = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float &v = x[i >> 1][2 * w + (i & 1)];
+            v = on[w][i] ? v * a.scale2 : -INFINITY;
+            t = fmaxf(t, v);
+          }
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+          t = fmaxf(fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)), m[w]);
+          const float ref = t == -INFINITY ? 0.0f : t, cf = m[w] == -INFINITY ? 0.0f : exp2f(m[w] - ref);
+          m[w] = t;
+          l[w] *= cf;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float &v = x[i >> 1][2 * w + (i & 1)];
+            v = exp2f(v - ref);
+            l[w] += v;
+          }
+#pragma unroll
+          for (int k = 0; k < DN; k++) { o[k][2 * w] *= cf; o[k][2 * w + 1] *= cf; }
+        }
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const uint16_t *k = c.k + p + (8 * t + gid) * HD + d;
-          kf_mma<T>(x[t], qa, __ldcg((const uint32_t *)k), __ldcg((const uint32_t *)(k + 8)));
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        float t = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float &v = x[i >> 1][2 * w + (i & 1)];
-          v = on[w][i] ? v * a.scale2 : -INFINITY;
-          t = fmaxf(t, v);
-        }
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-        t = fmaxf(fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)), m[w]);
-        const float ref = t == -INFINITY ? 0.0f : t, cf = m[w] == -INFINITY ? 0.0f : exp2f(m[w] - ref);
-        m[w] = t;
-        l[w] *= cf;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float &v = x[i >> 1][2 * w + (i & 1)];
-          v = exp2f(v - ref);
-          l[w] += v;
-        }
-#pragma unroll
-        for (int k = 0; k < HD / 8; k++) { o[k][2 * w] *= cf; o[k][2 * w + 1] *= cf; }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
 #pragma unroll 1
-        for (int i = 0; i < 8; i += 2) {                   // slots j + 8 t + i and the next: their probabilities are the quad's thread i / 2's
-          float pr[4];
+          for (int i = 0; i < 8; i += 2) {                   // slots j + 8 t + i and the next: their probabilities are the quad's thread i / 2's
+            float pr[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++) pr[k] = __shfl_sync(0xffffffffu, x[t][k], (lane & ~3) | (i >> 1));
+            for (int k = 0; k < 4; k++) pr[k] = __shfl_sync(0xffffffffu, x[t][k], (lane & ~3) | (i >> 1));
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const int n = 8 * t + i + u;
-            const bool s0 = sees(0, j + n), s1 = sees(1, j + n);
-            const uint16_t *v = c.v + p + n * HD;
+            for (int u = 0; u < 2; u++) {
+              const int n = 8 * t + i + u;
+              const bool s0 = sees(0, j + n), s1 = sees(1, j + n);
+              const uint16_t *v = c.v + p + n * HD + d0;
 #pragma unroll
-            for (int k = 0; k < HD / 8; k++) {
-              const float2 f = KvEl<T>::to2(__ldcg((const uint32_t *)(v + 8 * k)));
-              if (s0) { o[k][0] += pr[u] * f.x; o[k][1] += pr[u] * f.y; }
-              if (s1) { o[k][2] += pr[2 + u] * f.x; o[k][3] += pr[2 + u] * f.y; }
+              for (int k = 0; k < DN; k++) {
+                const float2 f = KvEl<T>::to2(__ldcg((const uint32_t *)(v + 8 * k)));
+                if (s0) { o[k][0] += pr[u] * f.x; o[k][1] += pr[u] * f.y; }
+                if (s1) { o[k][2] += pr[2 + u] * f.x; o[k][3] += pr[2 + u] * f.y; }
+              }
             }
           }
         }
       }
     }
-  }
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1); l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
-    if (!(rows >> (gid + 8 * w) & 1)) continue;
-    const float inv = l[w] == 0.0f ? 0.0f : 1.0f / l[w];
+    for (int w = 0; w < 2; w++) {
+      l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1); l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
+      if (!(rows >> (gid + 8 * w) & 1)) continue;
+      const float inv = l[w] == 0.0f ? 0.0f : 1.0f / l[w];
 #pragma unroll
-    for (int k = 0; k < HD / 8; k++) {
-      if (a.out32) *(float2 *)((float *)a.out + at[w] + 8 * k) = make_float2(o[k][2 * w] * inv, o[k][2 * w + 1] * inv);
-      else *(uint32_t *)((uint16_t *)a.out + at[w] + 8 * k) = KvEl<T>::of2(o[k][2 * w] * inv, o[k][2 * w + 1] * inv);
+      for (int k = 0; k < DN; k++) {
+        if (a.out32) *(float2 *)((float *)a.out + at[w] + d0 + 8 * k) = make_float2(o[k][2 * w] * inv, o[k][2 * w + 1] * inv);
+        else *(uint32_t *)((uint16_t *)a.out + at[w] + d0 + 8 * k) = KvEl<T>::of2(o[k][2 * w] * inv, o[k][2 * w + 1] * inv);
+      }
     }
   }
 }
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(32 * (kf_warps(HD) + 2), 1) k_kv_few(const KvD
     // rows whose result is no number once more (kv_attn_row says why)
     if (wholly && warp == 0) {
       const unsigned again = __ballot_sync(0xffffffffu, lane < 16 && hd.odd[lane & 15] && hd.L[lane & 15] == hd.L[lane & 15]);
-      if (again) kv_attn_rows16<T, HD>(c, a, use.b, use.g, s.first, s.e0, q0, NQ, kf_span(s, 0, s.chunks, SH), lane, again);
+      if (__builtin_expect(again != 0, 0)) kv_attn_rows16<T, HD>(c, a, use.b, use.g, s.first, s.e0, q0, NQ, kf_span(s, 0, s.chunks, SH), lane, again);
       if (lane < 16) hd.odd[lane] = 0;
     }
   }
@@ -578,10 +579,10 @@ __host__ __device__ __forceinline__ int kf_parts_of(int first, int last, int blo
 __device__ __forceinline__ size_t kf_part(int w, int w0) { return ((size_t)w * 2 + (w == w0)) * 16; }
 
 // Units that several blocks had: a block a query, its four warps the parts in turn, each with what it needs of them asked for at once.  Blocks from
-// `joins` on: what every slot got, KJ_SLOTS of a kv head each.  (Eight blocks an SM: with six, 16 x 4 rows of 16 heads, 1024 blocks, take 1.7 us more.)
+// `joins` on: what every slot got, KJ_SLOTS of a kv head each.
 #define KJ_SLOTS 2048
 template <typename T, int HD, bool WT>
-__global__ void __launch_bounds__(128, WT ? 4 : 8) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
+__global__ void __launch_bounds__(128) k_kv_join(const KvDev c, const KvRows rw, const KvAttn a, const KvPlan p, int joins, int wblocks) {
   constexpr int E = HD / 32;
   __shared__ float sm[4], sl[4], so[4][HD], lse[64];
   pdl_trigger();
