@@ -429,3 +429,50 @@ def test_rows_in_front_of_a_row_that_is_no_number(llb, rows, lens, H, KV, hd, wi
         _check_attn(c, r)
     assert after < 8 * before + 1.5, (before, after)
     _clean(llb)
+
+
+# ---- captured -------------------------------------------------------------------------------------------------
+def test_captured_prompts_and_evictions_run_again_on_other_contents(llb):
+    """A prompt over several blocks a row, verify rows with weights and an eviction captured together, replayed with other values, lengths, pages and weights."""
+    c = Cache(llb, "bf16", 2, 128, 16, [9000, 700], seed=134)
+    prompt, few = _attn(llb, c, 4, [90, 40], seed=135, behind=0, max_len=9000), _attn(llb, c, 4, [3, 2], seed=136, behind=0, weights=True, max_len=9000)
+    w = _weights(2, 2, 9000, 137)
+    c.K, c.V = [k[:9000] for k in c.K], [v[:9000] for v in c.V]
+    d, ids, w2, ev = _evict(llb, c, 500, 4, 60, w)
+    held = [prompt["out"], few["out"], few["w_out"], d.k, d.v, d.lens, ids, w2]
+
+    def step():
+        llb.kv_attn(*prompt["call"])
+        llb.kv_attn(*few["call"])
+        llb.kv_evict(*ev[:3])
+
+    stream = torch.cuda.ExternalStream(llb.lib().llb_b200_stream())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for n in ((8000, 650), (3000, 41), (8999, 300)):
+        c.lens.copy_(_ints(list(n)))
+        w.copy_(_weights(2, 2, 9000, 138 + n[0]))
+        prompt["q"].normal_()
+        c.table[0, :100] = c.table[0, :100].flip(0)
+        torch.cuda.synchronize()
+        step()
+        llb.check(llb.lib().llb_b200_sync(), "sync")
+        want = [t.clone() for t in held]
+        for t in held:
+            t.fill_(3)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        again = [t.clone() for t in held]
+        for t in held:
+            t.fill_(3)
+        torch.cuda.synchronize()
+        step()
+        llb.check(llb.lib().llb_b200_sync(), "sync")
+        for a, b in zip(again, held):
+            assert torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0)) if a.is_floating_point() else torch.equal(a, b)
+        assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
+    del graph
+    _clean(llb)
